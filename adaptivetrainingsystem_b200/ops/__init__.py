@@ -11,6 +11,8 @@ from .moe import (expert_capacity, gate_logits, route, load_balancing_loss, plan
                   slot_dot, moe_ffn, moe_ffn_reference)
 from .serving import (decode_attention, decode_attention_available, decode_attention_reference, sample_tokens,  # noqa: E402,F401
                       sample_reference)
+from .sampling import sample_rows, sample_rows_reference  # noqa: E402,F401
+from .paged import PagePlan, PagePool, page_plan, paged_append, paged_attention  # noqa: E402,F401
 from . import fp8  # noqa: E402,F401
 from . import int8  # noqa: E402,F401
 from . import int4  # noqa: E402,F401

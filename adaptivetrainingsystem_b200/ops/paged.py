@@ -1,0 +1,322 @@
+"""Paged key / value cache: page tables kept on the GPU, the write of new tokens into their pages, and attention over them
+(``csrc/paged.cu``).
+
+A pool of pages holds the keys and values of many sequences ("rows"): token ``i`` of row ``r`` lies in slot
+``tables[r, i // page_size] * page_size + i % page_size`` of ``[pages, page_size, n_kv, d]`` tensors, one pair per layer; free pages are a
+stack.  A step feeds every row some new tokens (none, one, or a portion of a prompt), packed one row after the other:
+
+* :func:`page_plan` takes the pages that the step needs, and says where each new token goes;
+* :func:`paged_append` rotates queries and keys and writes keys and values to their slots;
+* :func:`paged_attention` lets every new token attend to its row's tokens up to itself.
+
+Nothing of a step depends on lengths that the host would have to read, so a step of single tokens can be captured in a CUDA graph and
+replayed while rows come and go.  Tensors on the CPU run the PyTorch definitions below, which are also the oracles of the kernel tests.
+The reference has no cache (it runs the whole context again for every token, reference ``Chat.py:379-452``); its vendored serving engine keeps
+whole rows per request (``colossalai/inference/kv_cache/kvcache_manager.py:11-106``).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_vp, _ci, _cll, _cf = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+MAX_ROWS, MAX_TOKENS = 4096, 1 << 18
+_REFUSED = {1: "a row gets more tokens than its table or the packed batch holds", 2: "not enough free pages", 3: "the stack of free pages is inconsistent"}
+
+
+def _fn(name: str, argtypes):
+    f = getattr(_lib.cuda_lib(), name)
+    f.restype, f.argtypes = _ci, argtypes
+    return f
+
+
+def _p(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _on(device: torch.device):
+    """Launches go to the tensors' device, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(t: torch.Tensor, name: str, shape, device) -> None:
+    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous() and t.device == device,
+          f"{name}: a contiguous int32 tensor {list(shape)} on {device} is needed")
+
+
+class PagePool:
+    """Page tables of ``rows`` rows of up to ``max_len`` tokens over ``pages`` pages of ``page_size`` tokens (a power of two).  ``tables``
+    [rows, max_len / page_size], ``lengths`` [rows] (tokens a row holds) and the stack ``free`` live on the device; ``state`` holds the number of free
+    pages and the refusal code of the last committed step."""
+
+    def __init__(self, rows: int, max_len: int, pages: int, page_size: int = 64, device="cuda"):
+        _need(page_size >= 1 and page_size & (page_size - 1) == 0, f"page_size {page_size}: a power of two is needed")
+        _need(1 <= rows <= MAX_ROWS, f"{rows} rows: 1 to {MAX_ROWS} are possible")
+        width = -(-max_len // page_size)
+        _need(max_len >= 1 and pages >= 1 and pages * page_size < 1 << 31 and rows * width < 1 << 31 and width * page_size < 1 << 31,
+              "pages and rows: at least one page and one token, and slots below 2^31")
+        self.rows, self.pages, self.page_size, self.width = rows, pages, page_size, width
+        self.max_len = max_len
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        i32 = dict(dtype=torch.int32, device=device)
+        self.tables = torch.zeros(rows, width, **i32)
+        self.lengths = torch.zeros(rows, **i32)
+        self.free = torch.arange(pages - 1, -1, -1, **i32)   # page 0 is handed out first
+        self.state = torch.tensor([pages, 0, 0, 0], **i32)
+
+    def pages_for(self, tokens: int) -> int:
+        return -(-tokens // self.page_size)
+
+    def check(self) -> None:
+        """Raises if the last committed step was refused (reads the device)."""
+        code = int(self.state[1])
+        if code:
+            raise RuntimeError(f"the step was refused: {_REFUSED.get(code, code)}")
+
+
+@dataclass
+class PagePlan:
+    """What the operators of one step read.  ``max_new`` / ``max_len``: the longest portion and the longest row of the step as far as the host
+    knows them (upper bounds that choose kernels and grids; by default the packed batch and the tables' width)."""
+    starts: torch.Tensor            # int32 [rows + 1]: row r's new tokens are packed at starts[r] .. starts[r + 1]
+    slots: torch.Tensor             # int32 [tokens], -1: no row's token
+    positions: torch.Tensor         # int32 [tokens]
+    lengths: torch.Tensor           # int32 [rows]: tokens of the row, the new ones among them
+    tables: torch.Tensor            # int32 [rows, width]
+    page_size: int
+    max_new: Optional[int] = None
+    max_len: Optional[int] = None
+    info: Optional[torch.Tensor] = None   # int32 [2]: free pages after the step, refusal code
+
+    @property
+    def count(self) -> torch.Tensor:
+        """int32 [1]: free pages after the step."""
+        return self.info[:1]
+
+    def check(self) -> None:
+        """Raises if the step was refused (reads the device)."""
+        code = int(self.info[1])
+        if code:
+            raise RuntimeError(f"the step was refused: {_REFUSED.get(code, code)}")
+
+
+# ----------------------------------------------------------------------------------------------------------
+# page tables and slots
+# ----------------------------------------------------------------------------------------------------------
+def page_plan(pool: PagePool, fresh: torch.Tensor, tokens: int, commit: bool = True, max_new: Optional[int] = None, max_len: Optional[int] = None) -> PagePlan:
+    """Plans a step.  ``fresh`` int32 [rows]: new tokens of every row; 0: the row sits out; -1: the row is closed, its pages go back.
+    ``tokens``: rows of the packed batch, at least as many as there are new tokens (slots behind them are -1).
+
+    Closed rows push their pages onto the stack in row order, then rows take from its top in row order.  With ``commit`` the pool moves on in
+    the same launch; without, its tables hold the step's pages but lengths and free pages stay, so the step can be planned again (or another
+    one instead).  A step that does not fit is refused as a whole: no row has tokens in it, nothing changes, and :meth:`PagePlan.check`
+    (without ``commit``) or :meth:`PagePool.check` raises."""
+    _need(0 <= tokens <= MAX_TOKENS, f"{tokens} tokens in a step: at most {MAX_TOKENS}")
+    _ints(fresh, "fresh", (pool.rows,), pool.device)
+    i32 = dict(dtype=torch.int32, device=pool.device)
+    R = pool.rows
+    # one allocation: starts, slots, positions, info, lengths
+    buf = torch.empty(2 * R + 3 + 2 * tokens, **i32)
+    starts, slots, positions = buf[:R + 1], buf[R + 1:R + 1 + tokens], buf[R + 1 + tokens:R + 1 + 2 * tokens]
+    info = buf[R + 1 + 2 * tokens:R + 3 + 2 * tokens]
+    lengths = pool.lengths if commit else buf[R + 3 + 2 * tokens:]
+    plan = PagePlan(starts, slots, positions, lengths, pool.tables, pool.page_size, max_new, max_len, info)
+    if not pool.device.type == "cuda":
+        _page_plan_reference(pool, fresh, plan, commit)
+        return plan
+    f = _fn("ats_page_plan", [_vp] * 10 + [_ci] * 6 + [_vp])
+    with _on(pool.device):
+        _lib.check(f(_p(pool.lengths), _p(fresh), _p(pool.tables), _p(pool.free), _p(pool.state), _p(starts), _p(slots), _p(positions), _p(lengths), _p(info), R,
+                     pool.width, pool.pages, pool.page_size, tokens, int(commit), _lib.stream_ptr(pool.device)), "ats_page_plan")
+    return plan
+
+
+def _page_plan_reference(pool: PagePool, fresh: torch.Tensor, plan: PagePlan, commit: bool) -> None:
+    ps, room, T = pool.page_size, pool.width * pool.page_size, plan.slots.numel()
+    old, new, n = pool.lengths.tolist(), fresh.tolist(), int(pool.state[0])
+    plan.slots.fill_(-1)
+    plan.positions.zero_()
+    plan.starts.zero_()
+    bad = any(o < 0 or o > room or f < -1 or o + max(f, 0) > room for o, f in zip(old, new)) or sum(max(f, 0) for f in new) > T
+    refused, stack = int(bad), pool.free[:max(n, 0)].tolist()
+    if not refused:
+        for r, f in enumerate(new):
+            if f < 0:
+                stack += pool.tables[r, :-(-old[r] // ps)].tolist()
+        need = sum(-(-(o + f) // ps) - -(-o // ps) for o, f in zip(old, new) if f >= 0)
+        refused = 2 if need > len(stack) else 3 if n < 0 or len(stack) > pool.pages else 0
+    after = list(old)
+    if not refused:
+        at = 0
+        for r, (o, f) in enumerate(zip(old, new)):
+            plan.starts[r] = at
+            if f < 0:
+                after[r] = 0
+                continue
+            for j in range(-(-o // ps), -(-(o + f) // ps)):
+                pool.tables[r, j] = stack.pop()
+            for i in range(f):
+                pos = o + i
+                page = int(pool.tables[r, pos // ps])
+                plan.positions[at + i] = pos
+                plan.slots[at + i] = page * ps + pos % ps if 0 <= page < pool.pages else -1
+            at += f
+            after[r] = o + f
+        plan.starts[pool.rows] = at
+        if len(stack) > n:
+            pool.free[n:len(stack)] = torch.tensor(stack[n:], dtype=torch.int32)
+        n = len(stack)
+    plan.lengths.copy_(torch.tensor(after, dtype=torch.int32))
+    plan.info.copy_(torch.tensor([n, refused], dtype=torch.int32))
+    if commit:
+        pool.state[0], pool.state[1] = n, refused
+
+
+# ----------------------------------------------------------------------------------------------------------
+# writing new tokens
+# ----------------------------------------------------------------------------------------------------------
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, like: torch.Tensor):
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.shape[1] == plan.page_size,
+          "k_pages, v_pages: contiguous [pages, page_size, n_kv, d] tensors of the plan's page size are needed")
+    _need(k_pages.dtype == v_pages.dtype == like.dtype and k_pages.device == v_pages.device == like.device, "pages and tokens: one type, one device")
+    pages, ps, n_kv, d = k_pages.shape
+    _need(pages * ps < 1 << 31, "slots have to stay below 2^31")
+    R, T = plan.tables.shape[0], like.shape[0]
+    _ints(plan.tables, "plan.tables", plan.tables.shape, like.device)
+    _ints(plan.lengths, "plan.lengths", (R,), like.device)
+    _ints(plan.starts, "plan.starts", (R + 1,), like.device)
+    _ints(plan.slots, "plan.slots", (T,), like.device)
+    _ints(plan.positions, "plan.positions", (T,), like.device)
+    return pages, ps, n_kv, d
+
+
+def _kernel_type(t: torch.Tensor) -> None:
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{t.dtype}: the paged kernels take bfloat16 and float32")
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """A [T, heads, d] (or [T, width]) tensor as its kernel takes it: rows of contiguous heads that start at multiples of 16 bytes."""
+    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == t.shape[2])
+    if inner and (t.shape[0] == 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous()
+
+
+def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], plan: PagePlan, k_pages: torch.Tensor, v_pages: torch.Tensor, n_q: int,
+                 n_kv: int, d: int) -> torch.Tensor:
+    """qkv [T, (n_q + 2 n_kv) d], the packed projection of a step's new tokens -> queries [T, n_q, d]; keys and values go to ``plan.slots``
+    of ``k_pages`` / ``v_pages`` [pages, page_size, n_kv, d] (slot -1: nowhere).  Queries and keys are rotated at ``plan.positions`` with the
+    tables ``cos`` / ``sin`` [max position, d / 2] fp32 (halves of a head, d a multiple of 16); with ``cos`` = ``None`` they are rotated already and the
+    queries are a view of ``qkv``."""
+    T = qkv.shape[0]
+    _need(qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * d, f"qkv: [tokens, {(n_q + 2 * n_kv) * d}] is needed")
+    pages, ps, hk, dk = _check_pages(k_pages, v_pages, plan, qkv)
+    _need((hk, dk) == (n_kv, d), f"pages hold {hk} heads of {dk}, the projection {n_kv} of {d}")
+    if cos is not None:
+        _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d // 2 and cos.dtype == sin.dtype == torch.float32
+              and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == qkv.device and d % 16 == 0,
+              "cos, sin: contiguous float32 tables [positions, d / 2] on the projection's device, d a multiple of 16")
+    if not qkv.is_cuda:
+        return _paged_append_reference(qkv, cos, sin, plan, k_pages, v_pages, n_q, n_kv, d)
+    _kernel_type(qkv)
+    _need(8 <= d <= 256 and d % 8 == 0, f"heads of {d}: multiples of 8 up to 256")
+    src = _rows_of(qkv)
+    q = torch.empty(T, n_q, d, dtype=qkv.dtype, device=qkv.device) if cos is not None else src[:, :n_q * d].unflatten(1, (n_q, d))
+    if T == 0:
+        return q
+    f = _fn("ats_paged_append", [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp])
+    with _on(qkv.device):
+        _lib.check(f(_p(src), src.stride(0) if T > 1 else src.shape[1], _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _p(plan.positions), _p(plan.slots), _p(q), _p(k_pages), _p(v_pages), T, n_q, n_kv, d,
+                     pages * ps, int(qkv.dtype == torch.float32), _p(_lib.status_tensor(qkv.device)), _lib.stream_ptr(qkv.device)), "ats_paged_append")
+    return q
+
+
+def _paged_append_reference(qkv, cos, sin, plan, k_pages, v_pages, n_q, n_kv, d):
+    T = qkv.shape[0]
+    qk, v = qkv[:, :(n_q + n_kv) * d].reshape(T, n_q + n_kv, d), qkv[:, (n_q + n_kv) * d:].reshape(T, n_kv, d)
+    if cos is not None:
+        pos = plan.positions.long()
+        if T and int(pos.max()) >= cos.shape[0]:
+            raise ValueError(f"position {int(pos.max())} lies behind the rotary tables ({cos.shape[0]})")
+        c, s = cos[pos][:, None], sin[pos][:, None]
+        a, b = qk.float().chunk(2, -1)
+        qk = torch.cat([a * c - b * s, b * c + a * s], -1).to(qkv.dtype)
+    live = plan.slots >= 0
+    slots = plan.slots[live].long()
+    k_pages.view(-1, n_kv, d)[slots] = qk[live, n_q:]
+    v_pages.view(-1, n_kv, d)[slots] = v[live]
+    return qk[:, :n_q]
+
+
+# ----------------------------------------------------------------------------------------------------------
+# attention
+# ----------------------------------------------------------------------------------------------------------
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, n_q, d], a step's queries (rotated; rows may be views of a wider projection) -> [T, n_q, d].  Token i of a row's new tokens attends to the
+    row's tokens up to itself, in the pages of ``plan.tables``; its keys and values are there already.  ``scale`` (default 1 / sqrt(d)) times the scores.
+    Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given.  Heads of up to 256 dimensions (multiples of 8)."""
+    _need(q.dim() == 3, "q: [tokens, heads, d] is needed")
+    pages, ps, n_kv, d = _check_pages(k_pages, v_pages, plan, q)
+    T, n_q = q.shape[:2]
+    _need(q.shape[2] == d and n_q >= n_kv and n_q % n_kv == 0, f"{n_q} query heads of {q.shape[2]} over {n_kv} key heads of {d}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    _need(scale > 0 and math.isfinite(scale), "scale: a positive number")
+    if out is not None:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and (T == 0 or _rows_of(out) is out),
+              "out: like q, rows of contiguous heads that start at multiples of 16 bytes")
+    if not q.is_cuda:
+        return _paged_attention_reference(q, k_pages, v_pages, plan, scale, out)
+    _kernel_type(q)
+    _need(8 <= d <= 256 and d % 8 == 0, f"heads of {d}: multiples of 8 up to 256")
+    keep_tail = out is not None
+    if out is None:
+        out = torch.empty(T, n_q, d, dtype=q.dtype, device=q.device)
+    if T == 0:
+        return out
+    q = _rows_of(q)
+    ldq, ldo = (t.stride(0) if T > 1 else n_q * d for t in (q, out))
+    f = _fn("ats_paged_attn_any", [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp])
+    with _on(q.device):
+        _lib.check(f(_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, plan.tables.shape[0], n_q, n_kv, d,
+                     plan.tables.shape[1], pages, ps, scale, int(keep_tail), int(q.dtype == torch.float32), _p(_lib.status_tensor(q.device)),
+                     _lib.stream_ptr(q.device)), "ats_paged_attn_any")
+    return out
+
+
+def _paged_attention_reference(q, k_pages, v_pages, plan, scale, out):
+    T, n_q, d = q.shape
+    n_kv, ps = k_pages.shape[2], plan.page_size
+    if out is None:
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    starts, lengths = plan.starts.tolist(), plan.lengths.tolist()
+    rep = n_q // n_kv
+    for r, total in enumerate(lengths):
+        a, b = starts[r], starts[r + 1]
+        if a == b:
+            continue
+        table = plan.tables[r, :-(-total // ps)].long()
+        k = k_pages[table].reshape(-1, n_kv, d)[:total].float().repeat_interleave(rep, 1)
+        v = v_pages[table].reshape(-1, n_kv, d)[:total].float().repeat_interleave(rep, 1)
+        s = torch.einsum("qhd,khd->hqk", q[a:b].float() * scale, k)
+        seen = torch.arange(total, device=q.device)[None] <= torch.arange(total - (b - a), total, device=q.device)[:, None]
+        out[a:b] = torch.einsum("hqk,khd->qhd", torch.softmax(s.masked_fill(~seen, float("-inf")), -1), v).to(q.dtype)
+    return out

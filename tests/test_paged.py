@@ -1,0 +1,159 @@
+"""Paged cache operators on the CPU: the definitions, the life of a pool, refusals."""
+import math
+import random
+
+import pytest
+import torch
+
+from adaptivetrainingsystem_b200 import ops
+from paged_utils import attend64, make_plan, rows_of_pages, sample64
+
+
+def _random_step(g, pool, lengths, tokens_left=60):
+    fresh = []
+    for n in lengths:
+        kind = g.random()
+        f = -1 if kind < 0.15 and n else 0 if kind < 0.4 else 1 if kind < 0.8 else g.randint(1, 12)
+        if f > 0 and (f > tokens_left or n + f > pool.width * pool.page_size):
+            f = 0
+        tokens_left -= max(f, 0)
+        fresh.append(f)
+    return fresh
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+def test_plan_life_of_a_pool(page):
+    """However rows come, grow and go: no page belongs to two, and slots hold what was written to them."""
+    g = random.Random(page)
+    pool = ops.PagePool(5, 48, 5 * -(-48 // page), page, device="cpu")
+    lengths, content = [0] * 5, {}
+    memory = torch.full((pool.pages * page,), -1)
+    for step in range(60):
+        fresh = _random_step(g, pool, lengths)
+        T = sum(max(f, 0) for f in fresh)
+        plan = ops.page_plan(pool, torch.tensor(fresh, dtype=torch.int32), T + 2)
+        pool.check()
+        at = 0
+        for r, f in enumerate(fresh):
+            assert int(plan.starts[r]) == at
+            for i in range(max(f, 0)):
+                assert int(plan.positions[at + i]) == lengths[r] + i
+                memory[int(plan.slots[at + i])] = 1000 * step + at + i
+                content[r, lengths[r] + i] = 1000 * step + at + i
+            at += max(f, 0)
+            lengths[r] = 0 if f < 0 else lengths[r] + f
+        assert plan.slots[T:].tolist() == [-1, -1] and int(plan.starts[-1]) == T and pool.lengths.tolist() == lengths
+        used = [int(pool.tables[r, j]) for r in range(5) for j in range(pool.pages_for(lengths[r]))]
+        free = pool.free[:int(pool.state[0])].tolist()
+        assert sorted(used + free) == list(range(pool.pages))
+        for r, n in enumerate(lengths):
+            assert [int(memory[int(pool.tables[r, i // page]) * page + i % page]) for i in range(n)] == [content[r, i] for i in range(n)]
+
+
+def test_plan_refuses_a_step_as_a_whole():
+    pool = ops.PagePool(3, 32, 5, 8, device="cpu")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    ops.page_plan(pool, i32(17, 8, 0), 25)
+    before = (pool.tables.clone(), pool.lengths.clone(), pool.free.clone(), int(pool.state[0]))
+    for fresh, tokens, why in ((i32(8, 1, 1), 10, "free pages"), (i32(16, 0, 0), 16, "table"), (i32(1, 1, 0), 1, "packed batch"), (i32(-2, 0, 0), 4, "table")):
+        plan = ops.page_plan(pool, fresh, tokens, commit=False)
+        with pytest.raises(RuntimeError, match=why):
+            plan.check()
+        assert plan.slots.tolist() == [-1] * tokens and plan.starts.tolist() == [0] * 4 and torch.equal(plan.lengths, before[1])
+        ops.page_plan(pool, fresh, tokens)
+        with pytest.raises(RuntimeError, match=why):
+            pool.check()
+        assert torch.equal(pool.tables, before[0]) and torch.equal(pool.lengths, before[1]) and torch.equal(pool.free, before[2]) and int(pool.state[0]) == before[3]
+    ops.page_plan(pool, i32(-1, 1, 8), 9)   # a row closed in the same step gives its pages back first
+    pool.check()
+    assert pool.lengths.tolist() == [0, 9, 8] and int(pool.state[0]) == 2
+
+
+def test_plan_without_commit_can_be_repeated():
+    pool = ops.PagePool(2, 32, 8, 4, device="cpu")
+    fresh = torch.tensor([5, 2], dtype=torch.int32)
+    a = ops.page_plan(pool, fresh, 7, commit=False)
+    b = ops.page_plan(pool, fresh, 7, commit=False)
+    assert torch.equal(a.slots, b.slots) and a.lengths.tolist() == [5, 2] and pool.lengths.tolist() == [0, 0] and int(a.count) == 5 and int(pool.state[0]) == 8
+
+
+def test_append_and_attention_definitions():
+    old, new, page, n_q, n_kv, d = [0, 5, 3, 7], [4, 1, 0, 6], 4, 6, 2, 16
+    plan, pages = make_plan(old, new, page, "cpu", tail=2)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(pages, page, n_kv, d, generator=g) for _ in range(2))
+    T = plan.slots.numel()
+    qkv = torch.randn(T, (n_q + 2 * n_kv) * d, generator=g)
+    cos, sin = ops.rope_tables(32, d, 10000.0)
+    q = ops.paged_append(qkv, cos, sin, plan, k, v, n_q, n_kv, d)
+    want = ops.rope_reference(qkv[:, :(n_q + n_kv) * d].view(T, 1, n_q + n_kv, d), cos, sin, plan.positions.long()[:, None])[:, 0]
+    assert torch.allclose(q, want[:, :n_q], atol=1e-6)
+    for i in range(T - 2):
+        s = int(plan.slots[i])
+        assert torch.allclose(k.view(-1, n_kv, d)[s], want[i, n_q:], atol=1e-6) and torch.equal(v.view(-1, n_kv, d)[s], qkv[i, (n_q + n_kv) * d:].view(n_kv, d))
+    out = ops.paged_attention(q, k, v, plan)
+    ref, mass = attend64(q, k, v, plan, 1 / math.sqrt(d))
+    assert ((out.double() - ref).abs() <= 1e-5 * mass + 1e-7).all() and (out[T - 2:] == 0).all()
+    # and the dense attention of the framework over the same tokens
+    for r, (a, b) in enumerate(zip(plan.starts.tolist(), plan.starts.tolist()[1:])):
+        if b > a:
+            dense = ops.attention(q[None, a:b], rows_of_pages(k, plan, r)[None], rows_of_pages(v, plan, r)[None], causal=True, q_offset=old[r])
+            assert torch.allclose(out[a:b], dense[0], atol=1e-5)
+
+
+def test_refusals():
+    plan, pages = make_plan([3], [2], 4, "cpu")
+    k = torch.zeros(pages, 4, 2, 16)
+    q = torch.zeros(2, 4, 16)
+    with pytest.raises(ValueError, match="power of two"):
+        ops.PagePool(2, 16, 4, 12, device="cpu")
+    with pytest.raises(ValueError, match="rows"):
+        ops.PagePool(5000, 16, 4, 16, device="cpu")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.PagePool(2, 16, 1 << 26, 64, device="cpu")
+    pool = ops.PagePool(2, 16, 4, 4, device="cpu")
+    with pytest.raises(ValueError, match="fresh"):
+        ops.page_plan(pool, torch.zeros(3, dtype=torch.int32), 4)
+    with pytest.raises(ValueError, match="fresh"):
+        ops.page_plan(pool, torch.zeros(2, dtype=torch.int64), 4)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.page_plan(pool, torch.zeros(2, dtype=torch.int32), (1 << 18) + 1)
+    with pytest.raises(ValueError, match="page size"):
+        ops.paged_attention(q, k.view(pages * 2, 2, 2, 16), k.view(pages * 2, 2, 2, 16), plan)
+    with pytest.raises(ValueError, match="one type"):
+        ops.paged_attention(q.bfloat16(), k, k, plan)
+    with pytest.raises(ValueError, match="query heads"):
+        ops.paged_attention(q[:, :3], k, k, plan)
+    with pytest.raises(ValueError, match="plan.slots"):
+        ops.paged_attention(q[:1], k, k, plan)
+    with pytest.raises(ValueError, match="scale"):
+        ops.paged_attention(q, k, k, plan, scale=0.0)
+    with pytest.raises(ValueError, match="out"):
+        ops.paged_attention(q, k, k, plan, out=torch.zeros(2, 4, 16, dtype=torch.float64))
+    with pytest.raises(ValueError, match="qkv"):
+        ops.paged_append(torch.zeros(2, 100), None, None, plan, k, k, 4, 2, 16)
+    with pytest.raises(ValueError, match="rotary tables"):
+        ops.paged_append(torch.zeros(2, 128), *ops.rope_tables(4, 16, 10000.0), plan, k, k, 4, 2, 16)
+    with pytest.raises(ValueError, match="uniform"):
+        ops.sample_rows(torch.zeros(2, 8), torch.zeros(3))
+    with pytest.raises(ValueError, match="top_k"):
+        ops.sample_rows(torch.zeros(2, 8), torch.zeros(2), top_k=torch.ones(3))
+    with pytest.raises(ValueError, match="history"):
+        ops.sample_rows(torch.zeros(2, 8), torch.zeros(2), history=torch.zeros(2, 3, dtype=torch.int32))
+
+
+def test_sample_rows_definition():
+    g = torch.Generator().manual_seed(3)
+    B, V = 40, 57
+    logits = (3 * torch.randn(B, V, generator=g)).bfloat16().float().round()     # many ties
+    logits[5, 3:9], logits[6], logits[7, 11], logits[8, 4] = float("nan"), float("-inf"), float("inf"), float("-inf")
+    u = torch.rand(B, generator=g)
+    u[:4] = torch.tensor([0.0, 1.0, 1.5, 0.999999])
+    t = torch.tensor([0.7, 1.0, 2.5, 0.0])[torch.arange(B) % 4]
+    k = torch.tensor([0, 1, 5, 57, 100])[torch.arange(B) % 5].int()
+    p = torch.tensor([1.0, 0.9, 0.5, 0.0, 0.99, 1.0, 0.3])[torch.arange(B) % 7]
+    low = torch.tensor([0.0, 0.1, 1.0])[torch.arange(B) % 3]
+    pen = torch.tensor([1.0, 1.3])[torch.arange(B) % 2]
+    hist = torch.randint(-1, V + 3, (B, 9), generator=g)
+    got = ops.sample_rows(logits, u, t, k, p, low, pen, hist)
+    assert torch.equal(got, sample64(logits, u, t, k, p, low, pen, hist))
