@@ -31,9 +31,23 @@ MAX_ROWS, MAX_TOKENS = 4096, 1 << 18
 _REFUSED = {1: "a row gets more tokens than its table or the packed batch holds", 2: "not enough free pages", 3: "the stack of free pages is inconsistent"}
 
 
-def _fn(name: str, argtypes):
-    f = getattr(_lib.cuda_lib(), name)
-    f.restype, f.argtypes = _ci, argtypes
+_SIGNATURES = {
+    "ats_page_plan": [_vp] * 10 + [_ci] * 6 + [_vp],
+    "ats_paged_append": [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp],
+    "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp],
+    "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _cf, _ci, _vp, _vp, _vp, _vp],
+    "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
+    "ats_sample_rows": [_vp, _ci, _cll, _ci, _ci, _vp, _vp, _cf, _vp, _ci, _vp, _cf, _vp, _cf, _vp, _cf, _vp, _ci, _cll, _vp, _vp],
+}
+_fns = {}
+
+
+def _fn(name: str):
+    f = _fns.get(name)
+    if f is None:
+        f = getattr(_lib.cuda_lib(), name)
+        f.restype, f.argtypes = _cll if name.endswith("_scratch") else _ci, _SIGNATURES[name]
+        _fns[name] = f
     return f
 
 
@@ -41,11 +55,12 @@ def _p(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_here = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Launches go to the tensors' device, whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _here if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -54,8 +69,8 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _ints(t: torch.Tensor, name: str, shape, device) -> None:
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous() and t.device == device,
-          f"{name}: a contiguous int32 tensor {list(shape)} on {device} is needed")
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == shape and t.is_contiguous() and t.device == device):
+        raise ValueError(f"{name}: a contiguous int32 tensor {list(shape)} on {device} is needed")
 
 
 class PagePool:
@@ -128,7 +143,8 @@ def page_plan(pool: PagePool, fresh: torch.Tensor, tokens: int, commit: bool = T
     the same launch; without, its tables hold the step's pages but lengths and free pages stay, so the step can be planned again (or another
     one instead).  A step that does not fit is refused as a whole: no row has tokens in it, nothing changes, and :meth:`PagePlan.check`
     (without ``commit``) or :meth:`PagePool.check` raises."""
-    _need(0 <= tokens <= MAX_TOKENS, f"{tokens} tokens in a step: at most {MAX_TOKENS}")
+    if not 0 <= tokens <= MAX_TOKENS:
+        raise ValueError(f"{tokens} tokens in a step: at most {MAX_TOKENS}")
     _ints(fresh, "fresh", (pool.rows,), pool.device)
     i32 = dict(dtype=torch.int32, device=pool.device)
     R = pool.rows
@@ -141,9 +157,8 @@ def page_plan(pool: PagePool, fresh: torch.Tensor, tokens: int, commit: bool = T
     if not pool.device.type == "cuda":
         _page_plan_reference(pool, fresh, plan, commit)
         return plan
-    f = _fn("ats_page_plan", [_vp] * 10 + [_ci] * 6 + [_vp])
     with _on(pool.device):
-        _lib.check(f(_p(pool.lengths), _p(fresh), _p(pool.tables), _p(pool.free), _p(pool.state), _p(starts), _p(slots), _p(positions), _p(lengths), _p(info), R,
+        _lib.check(_fn("ats_page_plan")(_p(pool.lengths), _p(fresh), _p(pool.tables), _p(pool.free), _p(pool.state), _p(starts), _p(slots), _p(positions), _p(lengths), _p(info), R,
                      pool.width, pool.pages, pool.page_size, tokens, int(commit), _lib.stream_ptr(pool.device)), "ats_page_plan")
     return plan
 
@@ -207,9 +222,11 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, l
     return pages, ps, n_kv, d
 
 
-def _kernel_type(t: torch.Tensor) -> None:
+def _kernel_type(t: torch.Tensor, d: int) -> None:
     if t.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"{t.dtype}: the paged kernels take bfloat16 and float32")
+    if not 8 <= d <= 256 or d % 8:
+        raise ValueError(f"heads of {d}: multiples of 8 up to 256")
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -227,25 +244,27 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
     tables ``cos`` / ``sin`` [max position, d / 2] fp32 (halves of a head, d a multiple of 16); with ``cos`` = ``None`` they are rotated already and the
     queries are a view of ``qkv``."""
     T = qkv.shape[0]
-    _need(qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * d, f"qkv: [tokens, {(n_q + 2 * n_kv) * d}] is needed")
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * d:
+        raise ValueError(f"qkv: [tokens, {(n_q + 2 * n_kv) * d}] is needed")
     pages, ps, hk, dk = _check_pages(k_pages, v_pages, plan, qkv)
-    _need((hk, dk) == (n_kv, d), f"pages hold {hk} heads of {dk}, the projection {n_kv} of {d}")
+    if (hk, dk) != (n_kv, d):
+        raise ValueError(f"pages hold {hk} heads of {dk}, the projection {n_kv} of {d}")
     if cos is not None:
         _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d // 2 and cos.dtype == sin.dtype == torch.float32
               and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == qkv.device and d % 16 == 0,
               "cos, sin: contiguous float32 tables [positions, d / 2] on the projection's device, d a multiple of 16")
     if not qkv.is_cuda:
         return _paged_append_reference(qkv, cos, sin, plan, k_pages, v_pages, n_q, n_kv, d)
-    _kernel_type(qkv)
-    _need(8 <= d <= 256 and d % 8 == 0, f"heads of {d}: multiples of 8 up to 256")
+    _kernel_type(qkv, d)
     src = _rows_of(qkv)
     q = torch.empty(T, n_q, d, dtype=qkv.dtype, device=qkv.device) if cos is not None else src[:, :n_q * d].unflatten(1, (n_q, d))
     if T == 0:
         return q
-    f = _fn("ats_paged_append", [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp])
     with _on(qkv.device):
-        _lib.check(f(_p(src), src.stride(0) if T > 1 else src.shape[1], _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _p(plan.positions), _p(plan.slots), _p(q), _p(k_pages), _p(v_pages), T, n_q, n_kv, d,
-                     pages * ps, int(qkv.dtype == torch.float32), _p(_lib.status_tensor(qkv.device)), _lib.stream_ptr(qkv.device)), "ats_paged_append")
+        _lib.check(_fn("ats_paged_append")(
+            _p(src), src.stride(0) if T > 1 else src.shape[1], _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _p(plan.positions), _p(plan.slots), _p(q), _p(k_pages),
+            _p(v_pages), T, n_q, n_kv, d, pages * ps, int(qkv.dtype == torch.float32), _p(_lib.status_tensor(qkv.device)), _lib.stream_ptr(qkv.device)),
+            "ats_paged_append")
     return q
 
 
@@ -277,7 +296,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _need(q.dim() == 3, "q: [tokens, heads, d] is needed")
     pages, ps, n_kv, d = _check_pages(k_pages, v_pages, plan, q)
     T, n_q = q.shape[:2]
-    _need(q.shape[2] == d and n_q >= n_kv and n_q % n_kv == 0, f"{n_q} query heads of {q.shape[2]} over {n_kv} key heads of {d}")
+    if q.shape[2] != d or n_q < n_kv or n_q % n_kv:
+        raise ValueError(f"{n_q} query heads of {q.shape[2]} over {n_kv} key heads of {d}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _need(scale > 0 and math.isfinite(scale), "scale: a positive number")
     if out is not None:
@@ -285,8 +305,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
               "out: like q, rows of contiguous heads that start at multiples of 16 bytes")
     if not q.is_cuda:
         return _paged_attention_reference(q, k_pages, v_pages, plan, scale, out)
-    _kernel_type(q)
-    _need(8 <= d <= 256 and d % 8 == 0, f"heads of {d}: multiples of 8 up to 256")
+    _kernel_type(q, d)
     keep_tail = out is not None
     if out is None:
         out = torch.empty(T, n_q, d, dtype=q.dtype, device=q.device)
@@ -294,11 +313,18 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         return out
     q = _rows_of(q)
     ldq, ldo = (t.stride(0) if T > 1 else n_q * d for t in (q, out))
-    f = _fn("ats_paged_attn_any", [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp])
+    R, width = plan.tables.shape
+    rep, new, keys = n_q // n_kv, min(plan.max_new or T, T), min(plan.max_len or width * ps, width * ps)
+    status, stream = _p(_lib.status_tensor(q.device)), _lib.stream_ptr(q.device)
+    head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
     with _on(q.device):
-        _lib.check(f(_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, plan.tables.shape[0], n_q, n_kv, d,
-                     plan.tables.shape[1], pages, ps, scale, int(keep_tail), int(q.dtype == torch.float32), _p(_lib.status_tensor(q.device)),
-                     _lib.stream_ptr(q.device)), "ats_paged_attn_any")
+        if q.dtype == torch.bfloat16 and d in (64, 128) and ps >= 8 and new * rep <= 16:
+            limit = 8 if new * rep <= 8 else 16
+            n = _fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit)
+            part = torch.empty(n + 2 * n // d, dtype=torch.float32, device=q.device)
+            _lib.check(_fn("ats_paged_decode")(*head, keys, limit, scale, int(not keep_tail), _p(part), _p(part) + 4 * n, status, stream), "ats_paged_decode")
+        else:
+            _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
     return out
 
 

@@ -7,7 +7,6 @@ top-k, top-p, draw: reference ``Chat.py:391-425``) with min-p behind top-p.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Union
 
 import torch
@@ -15,7 +14,6 @@ import torch
 from . import _lib
 from .paged import _fn, _need, _on, _p
 
-_vp, _ci, _cll, _cf = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 MAX_VOCAB = 1 << 20
 PerRow = Union[int, float, torch.Tensor]
 
@@ -44,7 +42,8 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: PerRow
         _need(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.int64 and history.device == logits.device,
               "history: int64 [rows, n] on the logits' device")
     for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p), ("repetition_penalty", repetition_penalty)):
-        _need(not isinstance(v, torch.Tensor) or (v.shape == (B,) and v.device == logits.device), f"{name}: a number, or one per row on the logits' device")
+        if isinstance(v, torch.Tensor) and (v.shape != (B,) or v.device != logits.device):
+            raise ValueError(f"{name}: a number, or one per row on the logits' device")
     if not logits.is_cuda:
         return sample_rows_reference(logits, uniform, temperature, top_k, top_p, min_p, repetition_penalty, history)
     if logits.dtype not in (torch.bfloat16, torch.float32):
@@ -63,9 +62,8 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: PerRow
     rp, rp1 = _numbers(repetition_penalty, torch.float32)
     u = uniform.float().contiguous()
     n = 0 if history is None else history.shape[1]
-    f = _fn("ats_sample_rows", [_vp, _ci, _cll, _ci, _ci, _vp, _vp, _cf, _vp, _ci, _vp, _cf, _vp, _cf, _vp, _cf, _vp, _ci, _cll, _vp, _vp])
     with _on(logits.device):
-        _lib.check(f(_p(logits), int(logits.dtype == torch.float32), logits.stride(0), B, V, _p(u), _p(t), t1, _p(k), k1, _p(tp), tp1, _p(mp), mp1, _p(rp), rp1,
+        _lib.check(_fn("ats_sample_rows")(_p(logits), int(logits.dtype == torch.float32), logits.stride(0), B, V, _p(u), _p(t), t1, _p(k), k1, _p(tp), tp1, _p(mp), mp1, _p(rp), rp1,
                      _p(history) if n else 0, n, history.stride(0) if n else 0, _p(out), _lib.stream_ptr(logits.device)), "ats_sample_rows")
     return out
 

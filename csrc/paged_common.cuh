@@ -1,0 +1,37 @@
+// What the tensor-core kernels over paged caches share.
+#pragma once
+#include "common.cuh"
+
+namespace ats {
+
+// Pages [rows, n_kv, d] of bf16 (rows = pages * page) as 64-column pieces of one head, 128-byte swizzle; the box is `box_rows` tokens of a page.
+inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, uint64_t n_kv, uint64_t d, uint32_t box_rows) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return 1000;
+  if (reinterpret_cast<uintptr_t>(base) & 15) return 1001;
+  cuuint64_t dims[3] = {d, n_kv, rows};
+  cuuint64_t strides[2] = {d * 2, n_kv * d * 2};
+  cuuint32_t box[3] = {64, 1, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1100 + int(r);
+}
+
+struct PagedRows {
+  const int* starts;    // [R + 1] packed starts of the rows' new tokens
+  const int* lengths;   // [R] tokens of a row, the new ones among them
+  const int* tables;    // [R, width]
+  int R, width, pages, page_log, tokens;   // tokens: rows of the packed batch
+};
+// New tokens and keys of row r, as far as the batch and the table hold them: no index that follows from these leaves its buffer, whatever the plan says.
+__device__ __forceinline__ void paged_row(const PagedRows& p, int r, int* first, int* fresh, int* keys) {
+  const int a = min(max(p.starts[r], 0), p.tokens), b = min(max(p.starts[r + 1], a), p.tokens);
+  const long long room = (long long)p.width << p.page_log;
+  const int len = (int)min((long long)max(p.lengths[r], 0), room);
+  *first = a;
+  *fresh = b - a;
+  *keys = len;
+}
+
+}  // namespace ats
