@@ -9,9 +9,9 @@
 //   and keeps a running softmax; the fragments come out of the swizzled units as in the decode kernel over contiguous rows (inference.cu).
 //   The page of a unit comes from the row's table, which the lanes read 32 entries at a time.
 // * Rows of a batch are of any length, so the work is dealt out by units, not by rows: the units of all rows and key heads form one line, and
-//   every CTA takes an equal stretch of it.  A stretch's pairs (row, key head) that lie in it as a whole are finished there; what it holds of the
-//   first and the last goes to a scratch slot, and a second launch joins the slots of each such pair, in the order of the line: results do
-//   not depend on timing.
+//   every warp takes an equal stretch of it, its ring running on from one pair (row, key head) to the next.  Pairs that lie in a stretch as a
+//   whole are finished there; what it holds of the first and the last goes to a scratch slot, and a second launch joins the slots of each
+//   such pair, in the order of the line: results do not depend on timing.
 #include "paged_common.cuh"
 
 namespace ats {
@@ -27,11 +27,12 @@ struct PagedDecodeArgs {
   __nv_bfloat16* out;       // [tokens, ldo]
   long long ldo;
   int n_kv, rep, limit;     // rows with at most `limit` MMA rows are taken
-  int grid;                 // CTAs of the main launch
+  int warps;                // of the main launch
   int zero_tail;            // tokens behind the last row get zeros
   float scale_log2;
-  float* part_o;            // [grid, 2, rows of the MMA, D]
-  float* part_ml;           // [grid, 2, rows of the MMA, 2]
+  long long* line;          // [R + 1]: where a row's units begin, per key head; the end of the line
+  float* part_o;            // [warps, 2, rows of the MMA, D]
+  float* part_ml;           // [warps, 2, rows of the MMA, 2]
   int* status;
 };
 
@@ -60,46 +61,19 @@ __device__ __forceinline__ int pd_units(const PagedDecodeArgs& p, int r) {
   return fresh > 0 && (long long)fresh * p.rep <= p.limit ? (max(keys, 1) + UNIT - 1) / UNIT : 0;
 }
 
-// Sum of the units of all rows, and for every thread that of the rows in front of its own share [*r0, *r1).
-template <int UNIT, int THREADS>
-__device__ __forceinline__ long long pd_scan(const PagedDecodeArgs& p, int* r0, int* r1, long long* before, long long* s_sum) {
-  const int share = (p.rows.R + THREADS - 1) / THREADS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  *r0 = min(tid * share, p.rows.R);
-  *r1 = min(*r0 + share, p.rows.R);
-  long long mine = 0;
-  for (int r = *r0; r < *r1; ++r) mine += pd_units<UNIT>(p, r);
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
-  long long total = 0;
-  *before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) *before += s_sum[w];
-    total += s_sum[w];
-  }
-  return total;
-}
-
-// CTAs that share a line of `total` units: at least a unit for each of their warps, as long as there are that many.
-__device__ __forceinline__ int pd_ctas(const PagedDecodeArgs& p, long long total) { return int(min((long long)p.grid, (total + PD_WARPS - 1) / PD_WARPS)); }
+// Warps that share a line of `total` units.
+__device__ __forceinline__ long long pd_shares(const PagedDecodeArgs& p, long long total) { return min((long long)p.warps, total); }
 
 template <int D, int NR>  // NR: sets of eight MMA rows (1 or 2)
 __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                      const PagedDecodeArgs p) {
   constexpr int UNIT = 2048 / D, NT = UNIT / 8, KB = UNIT / 16, JD = D / 32, RD = D / 64, ROWS = 8 * NR;
-  static_assert(ROWS * D * 4 <= PD_STAGES * PD_UNIT_BYTES, "a warp's result fits its ring");
   extern __shared__ uint8_t pd_smem[];
   __shared__ uint64_t s_full[PD_WARPS][PD_STAGES];
-  __shared__ float s_m[PD_WARPS][ROWS], s_l[PD_WARPS][ROWS];
-  __shared__ long long s_sum[PD_WARPS], s_at;
-  __shared__ int s_row, s_abort;
-  pdl_prologue();
+  __shared__ long long s_sum[PD_WARPS], s_at[PD_WARPS];
+  __shared__ int s_row[PD_WARPS], s_abort;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const PagedRows& rows = p.rows;
   uint8_t* base_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_smem) + 1023) & ~uintptr_t(1023));
@@ -109,82 +83,122 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
     for (int i = 0; i < PD_STAGES; ++i) mbar_init(&full[i], 1);
     mbar_fence_init();
   }
-  if (tid == 0) s_abort = 0, s_row = rows.R, s_at = 0;
+  if (tid == 0) s_abort = 0;
+  // where the rows begin on the line: every thread sums up a share of the rows
+  const int share = (rows.R + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * share, rows.R), r1 = min(r0 + share, rows.R);
+  long long mine = 0;
+  for (int r = r0; r < r1; ++r) mine += pd_units<UNIT>(p, r);
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  __syncthreads();
+  long long total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < PD_WARPS; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  total *= p.n_kv;
+  const long long shares = pd_shares(p, total), me0 = (long long)blockIdx.x * PD_WARPS;
+  for (int r = r0; r < r1; ++r) {
+    const long long n = pd_units<UNIT>(p, r), at = before * p.n_kv;
+    if (blockIdx.x == 0) p.line[r] = before;
+    for (int w = 0; w < PD_WARPS && me0 + w < shares; ++w) {
+      const long long x = (me0 + w) * total / shares;
+      if (at <= x && x < at + n * p.n_kv) s_row[w] = r, s_at[w] = at;
+    }
+    before += n;
+  }
+  if (blockIdx.x == 0 && tid == 0) p.line[rows.R] = total / p.n_kv;
+  __syncthreads();
   if (p.zero_tail) {
     const int tail = min(max(rows.starts[rows.R], 0), rows.tokens), vecs = p.n_kv * p.rep * (D / 8);
     for (long long i = (long long)blockIdx.x * PD_THREADS + tid; i < (long long)(rows.tokens - tail) * vecs; i += (long long)gridDim.x * PD_THREADS)
       *reinterpret_cast<uint4*>(p.out + (tail + i / vecs) * p.ldo + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
   }
-  // this CTA's stretch of the line
-  int r0, r1;
-  long long before;
-  const long long total = pd_scan<UNIT, PD_THREADS>(p, &r0, &r1, &before, s_sum) * p.n_kv;
-  const int ctas = pd_ctas(p, total);
-  if (int(blockIdx.x) >= ctas) return;
-  const long long lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1) * total / ctas;   // (not empty)
-  long long at = before * p.n_kv;   // where the row's units begin
-  for (int r = r0; r < r1; ++r) {
-    const long long n = (long long)pd_units<UNIT>(p, r) * p.n_kv;
-    if (n > 0 && at <= lo && lo < at + n) s_row = r, s_at = at;
-    at += n;
+  const long long me = me0 + warp;
+  if (me >= shares) return;
+  const long long lo = me * total / shares;
+  const int n_mine = int((me + 1) * total / shares - lo);
+
+  // ---- requests run ahead of the units that are worked on, into the pairs that follow
+  const int page = 1 << rows.page_log, box = min(UNIT, page), per = UNIT / box;   // tokens and number of the copies of a unit's 64-column piece
+  const int batch = 32 / per;   // units whose coordinates the lanes hold, copy lane % per of unit lane / per
+  int q_row = s_row[warp], q_hk, q_unit, q_units = pd_units<UNIT>(p, q_row), q_pages, q_base = 0, here = 0, asked = 0;
+  {
+    const long long in_row = lo - s_at[warp];
+    q_hk = int(in_row / q_units);
+    q_unit = int(in_row - (long long)q_hk * q_units);
   }
-  __syncthreads();
-  int row = s_row;
-  at = s_at;
-  const int box = min(UNIT, 1 << rows.page_log), per = UNIT / box;   // tokens and number of the copies of a unit's 64-column piece
-  uint32_t stage = 0, parity = 0;
-  bool ok = true;
-  int first_seg = 1;
-  long long cur = lo;
-  while (cur < hi && row < rows.R) {
+  const int w_row = q_row, w_hk = q_hk, w_unit = q_unit;   // the first unit to work on
+  auto pages_of = [&](int r) {
     int first, fresh, keys;
-    paged_row(rows, row, &first, &fresh, &keys);
+    paged_row(rows, r, &first, &fresh, &keys);
+    return (keys + page - 1) >> rows.page_log;
+  };
+  auto look_up = [&](int from) {   // coordinates of units from .. from + batch - 1 of the pair
+    q_base = from;
+    const int k0 = (from + lane / per) * UNIT + (lane % per) * box, j = k0 >> rows.page_log;
+    here = rows.pages << rows.page_log;    // behind the pages: reads as zero
+    if (j < q_pages) {
+      const int id = rows.tables[(long long)q_row * rows.width + j];
+      if (id >= 0 && id < rows.pages) here = (id << rows.page_log) + (k0 & (page - 1));
+      else atomicCAS(p.status, 0, int(kBadArgument));
+    }
+  };
+  q_pages = pages_of(q_row);
+  look_up(q_unit);
+  auto request = [&]() {   // whole warp: the next unit of the stretch
+    if (q_unit == q_units) {
+      q_unit = 0;
+      if (++q_hk == p.n_kv) {
+        q_hk = 0;
+        do q_units = pd_units<UNIT>(p, ++q_row);   // (a unit is still to come, so a row is)
+        while (q_units == 0);
+        q_pages = pages_of(q_row);
+      }
+      look_up(0);
+    } else if (q_unit - q_base == batch) {
+      look_up(q_unit);
+    }
+    const uint32_t st = asked % PD_STAGES;
+    uint8_t* dst = ring + st * PD_UNIT_BYTES;
+    if (lane == 0) mbar_expect_tx(&full[st], PD_UNIT_BYTES);
+    for (int s = 0; s < per; ++s) {
+      const int c = __shfl_sync(0xffffffffu, here, (q_unit - q_base) * per + s);
+      if (lane == 0) {
+#pragma unroll
+        for (int rd = 0; rd < RD; ++rd) {
+          tma_load_3d(dst + (rd * UNIT + s * box) * 128, &map_k, &full[st], 64 * rd, q_hk, c);
+          tma_load_3d(dst + PD_UNIT_BYTES / 2 + (rd * UNIT + s * box) * 128, &map_v, &full[st], 64 * rd, q_hk, c);
+        }
+      }
+    }
+    ++q_unit;
+    ++asked;
+  };
+  while (asked < min(n_mine, PD_STAGES)) request();
+
+  const uint32_t k_at = smem_u32(ring) + g * 128, v_at = smem_u32(ring) + PD_UNIT_BYTES / 2 + 2 * t * 128;
+  // the pieces of key 8 nt + g and of the values' keys 2 t, 2 t + 1 (+ 8), swizzled by their rows modulo eight
+  const uint32_t piece[2] = {uint32_t((t ^ g) << 4), uint32_t(((4 + t) ^ g) << 4)};
+  const uint32_t vpiece[2] = {uint32_t((g ^ (2 * t)) << 4), uint32_t((g ^ (2 * t + 1)) << 4) + 128};
+  int row = w_row, hk = w_hk, u0 = w_unit, done = 0;
+#pragma unroll 1
+  while (done < n_mine) {
     const int units = pd_units<UNIT>(p, row);
-    if (units == 0 || cur >= at + (long long)units * p.n_kv) {   // (the same for all threads)
-      at += (long long)units * p.n_kv;
+    if (units == 0) {
       ++row;
       continue;
     }
-    const int hk = int((cur - at) / units), u0 = int((cur - at) - (long long)hk * units), u1 = int(min((long long)units, u0 + (hi - cur)));
-    const bool whole = u0 == 0 && u1 == units;
+    int first, fresh, keys;
+    paged_row(rows, row, &first, &fresh, &keys);
+    const int count = min(units - u0, n_mine - done);
     const int n_rows = fresh * p.rep, open = keys - fresh + 1;   // keys below `open` are seen by all new tokens
-    const int* table = rows.tables + (long long)row * rows.width;
-    const int n_pages = (keys + (1 << rows.page_log) - 1) >> rows.page_log;
-    const int count = u1 - u0 > warp ? (u1 - u0 - warp + PD_WARPS - 1) / PD_WARPS : 0;   // units of this warp: u0 + warp, + 4, ..
-    // coordinates of the warp's copies, one per lane, `batch` units at a time
-    const int batch = 32 / per;
-    auto coordinate = [&](int first_unit) {   // of copy `lane % per` of the warp's unit first_unit + lane / per
-      const int i = first_unit + lane / per;
-      const int k0 = (u0 + warp + i * PD_WARPS) * UNIT + (lane % per) * box;
-      int c = rows.pages << rows.page_log;    // behind the pages: reads as zero
-      if (i < count && (k0 >> rows.page_log) < n_pages) {
-        const int id = table[k0 >> rows.page_log];
-        if (id >= 0 && id < rows.pages) c = (id << rows.page_log) + (k0 & ((1 << rows.page_log) - 1));
-        else atomicCAS(p.status, 0, int(kBadArgument));
-      }
-      return c;
-    };
-    int here = coordinate(0), next = count > batch ? coordinate(batch) : 0, base_unit = 0;
-    auto request = [&](int i, uint32_t st) {   // whole warp; units in order
-      if (i - base_unit >= batch) {
-        base_unit += batch;
-        here = next;
-        if (base_unit + batch < count) next = coordinate(base_unit + batch);
-      }
-      uint8_t* dst = ring + st * PD_UNIT_BYTES;
-      if (lane == 0) mbar_expect_tx(&full[st], PD_UNIT_BYTES);
-      for (int s = 0; s < per; ++s) {
-        const int c = __shfl_sync(0xffffffffu, here, (i - base_unit) * per + s);
-        if (lane == 0) {
-#pragma unroll
-          for (int rd = 0; rd < RD; ++rd) {
-            tma_load_3d(dst + (rd * UNIT + s * box) * 128, &map_k, &full[st], 64 * rd, hk, c);
-            tma_load_3d(dst + PD_UNIT_BYTES / 2 + (rd * UNIT + s * box) * 128, &map_v, &full[st], 64 * rd, hk, c);
-          }
-        }
-      }
-    };
-    for (int i = 0; i < min(count, PD_STAGES); ++i) request(i, (stage + i) % PD_STAGES);
     // queries of MMA rows g and g + 8, [virtual k-step][pieces of a row]
     uint32_t qa[NR][D / 16][2];
     int last[NR];   // keys up to this one are seen by the row
@@ -210,15 +224,16 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
         for (int e = 0; e < 4; ++e) oe[rd][i][e] = oo[rd][i][e] = 0.f;
 #pragma unroll
     for (int x = 0; x < NR; ++x) m[x] = -INFINITY, l[x] = 0.f;
-    const uint32_t k_at = smem_u32(ring) + g * 128, v_at = smem_u32(ring) + PD_UNIT_BYTES / 2 + 2 * t * 128;
-    // the pieces of key 8 nt + g and of the values' keys 2 t, 2 t + 1 (+ 8), swizzled by their rows modulo eight
-    const uint32_t piece[2] = {uint32_t((t ^ g) << 4), uint32_t(((4 + t) ^ g) << 4)};
-    const uint32_t vpiece[2] = {uint32_t((g ^ (2 * t)) << 4), uint32_t((g ^ (2 * t + 1)) << 4) + 128};
 #pragma unroll 1
-    for (int u = 0; u < count; ++u) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], parity, &s_abort, p.status, kTimeoutFull));
-      if (!ok) break;
-      const int k0 = (u0 + warp + u * PD_WARPS) * UNIT;
+    for (int u = 0; u < count; ++u, ++done) {
+      const uint32_t stage = done % PD_STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], (done / PD_STAGES) & 1, &s_abort, p.status, kTimeoutFull))) {
+        const uint64_t t0 = globaltimer_ns();   // copies that were issued land before the warp gives its shared memory back
+        while (globaltimer_ns() - t0 < 10000000ull) {
+        }
+        return;
+      }
+      const int k0 = (u0 + u) * UNIT;
       const uint32_t ks = k_at + stage * PD_UNIT_BYTES, vs = v_at + stage * PD_UNIT_BYTES;
       const bool edge = k0 + UNIT > open;   // the unit holds keys that some row does not see
       uint4 vv[KB][RD][4];
@@ -309,141 +324,129 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
         }
       }
       __syncwarp();   // the stage has been read
-      if (u + PD_STAGES < count) request(u + PD_STAGES, stage);
-      if (++stage == PD_STAGES) stage = 0, parity ^= 1;
-    }
-    if (!ok) {   // copies that were issued land before the CTA gives its shared memory back
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 10000000ull) {
-      }
+      if (asked < n_mine) request();
     }
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    }
-    // the warps' results lie in their rings, which are empty
-    auto red = [&](int w, int i, int d) { return reinterpret_cast<float*>(base_smem + w * (PD_STAGES * PD_UNIT_BYTES)) + i * D + d; };
-    // lane (g, t): accumulator column 2t is dim 64 rd + 16 t + 2 i (+ 1 for the odd tile), column 2t + 1 eight dims further
-#pragma unroll
-    for (int x = 0; x < NR; ++x) {
       const int i = g + 8 * x;
-      if (t == 0) s_m[warp][i] = m[x], s_l[warp][i] = l[x];
-#pragma unroll
-      for (int rd = 0; rd < RD; ++rd) {
-        float* dst = red(warp, i, 64 * rd + 16 * t);
-        *reinterpret_cast<float4*>(dst) = make_float4(oe[rd][0][2 * x], oo[rd][0][2 * x], oe[rd][1][2 * x], oo[rd][1][2 * x]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(oe[rd][2][2 * x], oo[rd][2][2 * x], oe[rd][3][2 * x], oo[rd][3][2 * x]);
-        *reinterpret_cast<float4*>(dst + 8) = make_float4(oe[rd][0][2 * x + 1], oo[rd][0][2 * x + 1], oe[rd][1][2 * x + 1], oo[rd][1][2 * x + 1]);
-        *reinterpret_cast<float4*>(dst + 12) = make_float4(oe[rd][2][2 * x + 1], oo[rd][2][2 * x + 1], oe[rd][3][2 * x + 1], oo[rd][3][2 * x + 1]);
-      }
-    }
-    __syncthreads();
-    const long long slot = (long long)blockIdx.x * 2 + (first_seg ? 0 : 1);
-    for (int e = tid; e < n_rows * D; e += PD_THREADS) {
-      const int i = e / D, d = e - i * D;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, s_m[w][i]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float acc = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < PD_WARPS; ++w) {
-        const float f = pd_from(s_m[w][i], ref);
-        acc += *red(w, i, d) * f;
-        sum += s_l[w][i] * f;
-      }
-      if (whole) {
+      if (i >= n_rows) continue;
+      // lane (g, t): accumulator column 2t is dim 64 rd + 16 t + 2 i (+ 1 for the odd tile), column 2t + 1 eight dims further
+      if (count == units) {
         const int tok = i / p.rep, head = i - tok * p.rep;
-        p.out[(long long)(first + tok) * p.ldo + (long long)(hk * p.rep + head) * D + d] = __float2bfloat16(sum > 0.f ? acc / sum : acc);
+        const float inv = l[x] > 0.f ? 1.f / l[x] : 1.f;
+        __nv_bfloat16* dst = p.out + (long long)(first + tok) * p.ldo + (long long)(hk * p.rep + head) * D + 16 * t;
+#pragma unroll
+        for (int rd = 0; rd < RD; ++rd)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<uint4*>(dst + 64 * rd + 8 * e) =
+                make_uint4(pack_bf16x2(oe[rd][0][2 * x + e] * inv, oo[rd][0][2 * x + e] * inv), pack_bf16x2(oe[rd][1][2 * x + e] * inv, oo[rd][1][2 * x + e] * inv),
+                           pack_bf16x2(oe[rd][2][2 * x + e] * inv, oo[rd][2][2 * x + e] * inv), pack_bf16x2(oe[rd][3][2 * x + e] * inv, oo[rd][3][2 * x + e] * inv));
       } else {
-        p.part_o[(slot * ROWS + i) * D + d] = acc;
-        if (d == 0) p.part_ml[(slot * ROWS + i) * 2] = top, p.part_ml[(slot * ROWS + i) * 2 + 1] = sum;
+        const long long slot = (me * 2 + (done == count ? 0 : 1)) * ROWS + i;   // the stretch's first piece, or its last
+        if (t == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(m[x], l[x]);
+        float* dst = p.part_o + slot * D + 16 * t;
+#pragma unroll
+        for (int rd = 0; rd < RD; ++rd)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            *reinterpret_cast<float4*>(dst + 64 * rd + 8 * e) = make_float4(oe[rd][0][2 * x + e], oo[rd][0][2 * x + e], oe[rd][1][2 * x + e], oo[rd][1][2 * x + e]);
+            *reinterpret_cast<float4*>(dst + 64 * rd + 8 * e + 4) = make_float4(oe[rd][2][2 * x + e], oo[rd][2][2 * x + e], oe[rd][3][2 * x + e], oo[rd][3][2 * x + e]);
+          }
       }
     }
-    fence_proxy_async_smem();   // plain accesses to the rings come before the next copies into them
-    __syncthreads();
-    if (s_abort) return;
-    first_seg = 0;
-    cur += u1 - u0;
+    u0 = 0;
+    if (++hk == p.n_kv) hk = 0, ++row;
   }
 }
 
-// One CTA per (key head, row): the scratch slots of a pair that several CTAs shared, joined in the order of the line.
-constexpr int PJ_THREADS = 128;
+// One CTA per (key head, row, MMA row): the scratch slots of a pair that several warps shared.  D / 4 lanes hold a row's columns; sixteen such
+// groups take the slots in turn, and their sums are joined in order.
+constexpr int PJ_GROUPS = 16;
 template <int D, int NR>
-__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedDecodeArgs p) {
-  constexpr int UNIT = 2048 / D, ROWS = 8 * NR;
-  __shared__ long long s_sum[PJ_THREADS / 32], s_at;
+__global__ void __launch_bounds__(PJ_GROUPS * D / 4) paged_join_kernel(const PagedDecodeArgs p) {
+  constexpr int UNIT = 2048 / D, ROWS = 8 * NR, LANES = D / 4;
+  __shared__ float4 s_acc[PJ_GROUPS][LANES];
+  __shared__ float s_m[PJ_GROUPS], s_l[PJ_GROUPS];
+  const int i = blockIdx.x, hk = blockIdx.y, row = blockIdx.z, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   pdl_prologue();
-  const int hk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
-  const int units = pd_units<UNIT>(p, row);
-  if (units == 0) return;
-  int r0, r1;
-  long long before;
-  const long long total = pd_scan<UNIT, PJ_THREADS>(p, &r0, &r1, &before, s_sum) * p.n_kv;
-  if (r0 <= row && row < r1) {
-    for (int r = r0; r < row; ++r) before += pd_units<UNIT>(p, r);
-    s_at = before;
-  }
-  __syncthreads();
-  const long long a = s_at * p.n_kv + (long long)hk * units, b = a + units;
-  const int ctas = pd_ctas(p, total);
-  auto owner = [&](long long x) { return ((x + 1) * ctas - 1) / total; };   // the CTA whose stretch holds x: the largest c with c total / ctas <= x
-  const long long c0 = owner(a), c1 = owner(b - 1);
-  if (c0 == c1) return;   // finished by that CTA
-  const long long s0 = 2 * c0 + (c0 * total / ctas >= a ? 0 : 1);   // the first CTA's slot: its first piece unless its stretch began before the pair
   int first, fresh, keys;
   paged_row(p.rows, row, &first, &fresh, &keys);
-  for (int e = tid; e < fresh * p.rep * D; e += PJ_THREADS) {
-    const int i = e / D, d = e - i * D;
-    float top = p.part_ml[(s0 * ROWS + i) * 2];
-    for (long long c = c0 + 1; c <= c1; ++c) top = fmaxf(top, p.part_ml[(2 * c * ROWS + i) * 2]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
+  const int units = pd_units<UNIT>(p, row);
+  if (i >= fresh * p.rep || units == 0) return;
+  const long long total = p.line[p.rows.R] * p.n_kv, a = p.line[row] * p.n_kv + (long long)hk * units;
+  const long long shares = pd_shares(p, total);
+  auto owner = [&](long long x) { return ((x + 1) * shares - 1) / total; };   // whose stretch holds x: the largest w with w total / shares <= x
+  const long long w0 = owner(a), w1 = owner(a + units - 1);
+  if (w0 == w1) return;   // finished by that warp
+  const long long s0 = 2 * w0 + (w0 * total / shares >= a ? 0 : 1);   // the first one's slot: its first piece unless its stretch began before the pair
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (long long c = c0; c <= c1; ++c) {
-      const long long at = (c == c0 ? s0 : 2 * c) * ROWS + i;
-      const float f = pd_from(p.part_ml[at * 2], ref);
-      acc += p.part_o[at * D + d] * f;
-      sum += p.part_ml[at * 2 + 1] * f;
-    }
-    const int tok = i / p.rep, head = i - tok * p.rep;
-    p.out[(long long)(first + tok) * p.ldo + (long long)(hk * p.rep + head) * D + d] = __float2bfloat16(sum > 0.f ? acc / sum : acc);
+  for (long long w = w0 + group; w <= w1; w += PJ_GROUPS) {
+    const long long at = (w == w0 ? s0 : 2 * w) * ROWS + i;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
+    const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top, keep = pd_from(m, ref), f = pd_from(ml.x, ref);
+    m = top;
+    l = l * keep + ml.y * f;
+    acc = make_float4(acc.x * keep + v.x * f, acc.y * keep + v.y * f, acc.z * keep + v.z * f, acc.w * keep + v.w * f);
   }
+  s_acc[group][lane] = acc;
+  if (lane == 0) s_m[group] = m, s_l[group] = l;
+  __syncthreads();
+  if (group > 0) return;
+  float top = m;
+#pragma unroll
+  for (int x = 1; x < PJ_GROUPS; ++x) top = fmaxf(top, s_m[x]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int x = 0; x < PJ_GROUPS; ++x) {
+    const float f = pd_from(s_m[x], ref);
+    const float4 v = s_acc[x][lane];
+    sum += s_l[x] * f;
+    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 1.f;
+  const int tok = i / p.rep, head = i - tok * p.rep;
+  *reinterpret_cast<uint2*>(p.out + (long long)(first + tok) * p.ldo + (long long)(hk * p.rep + head) * D + 4 * lane) =
+      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
   cudaError_t ce = cudaFuncSetAttribute(paged_decode_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_SMEM);
-  if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3(p.grid), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
-  if (ce == cudaSuccess) ce = launch_pdl(paged_join_kernel<D, NR>, dim3(p.n_kv, p.rows.R), dim3(PJ_THREADS), 0, s, p);
+  if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
+  if (ce == cudaSuccess) ce = launch_pdl(paged_join_kernel<D, NR>, dim3(p.limit, p.n_kv, p.rows.R), dim3(PJ_GROUPS * D / 4), 0, s, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }
 
-// CTAs of the main launch for up to `keys` keys in each of R rows: three an SM, but no more than have a unit for each of their warps.
-static int paged_decode_grid(int R, int n_kv, int D, long long keys) {
+// Warps of the main launch for up to `keys` keys in each of R rows: three CTAs an SM, but no more warps than there are units.
+static int paged_decode_warps(int R, int n_kv, int D, long long keys) {
   const long long units = (keys + 2048 / D - 1) / (2048 / D) * R * n_kv;
-  const long long n = (units + PD_WARPS - 1) / PD_WARPS;
-  return int(n < 1 ? 1 : n > 444 ? 444 : n);
+  return int(units < 1 ? 1 : units > 444 * PD_WARPS ? 444 * PD_WARPS : units);
 }
 
 }  // namespace ats
 
 using namespace ats;
 
-// Floats of scratch that `ats_paged_decode` needs: part_o this many, part_ml 2 / D as many.
+// Bytes of scratch that `ats_paged_decode` needs (16-byte aligned).
 ATS_API long long ats_paged_decode_scratch(int R, int n_kv, int D, long long max_keys, int limit) {
-  return 2ll * paged_decode_grid(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * D;
+  return ((R + 2ll) / 2 * 2) * 8 + 2ll * paged_decode_warps(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
 }
 
 // Rows whose new tokens times n_q / n_kv are at most `limit` (8 or 16).  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens
 // (a power of two) or more; max_keys: no row has more.  zero_tail: tokens behind the last row get zeros.
 ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
                              void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, long long max_keys, int limit,
-                             float scale, int zero_tail, float* part_o, float* part_ml, int* status, void* stream) {
-  if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
+                             float scale, int zero_tail, void* scratch, int* status, void* stream) {
+  if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_kv > 65535 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
       (limit != 8 && limit != 16) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
     return 1003;
   static thread_local bool ctx_bound = false;
@@ -459,8 +462,11 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.grid = paged_decode_grid(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
-  p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part_o; p.part_ml = part_ml; p.status = status;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  p.line = static_cast<long long*>(scratch);
+  p.part_o = reinterpret_cast<float*>(p.line + (R + 2) / 2 * 2);
+  p.part_ml = p.part_o + 2ll * p.warps * (limit > 8 ? 16 : 8) * D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (limit > 8) return D == 64 ? launch_paged_decode<64, 2>(mk, mv, p, s) : launch_paged_decode<128, 2>(mk, mv, p, s);
   return D == 64 ? launch_paged_decode<64, 1>(mk, mv, p, s) : launch_paged_decode<128, 1>(mk, mv, p, s);
