@@ -35,7 +35,7 @@ _SIGNATURES = {
     "ats_page_plan": [_vp] * 10 + [_ci] * 6 + [_vp],
     "ats_paged_append": [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp],
     "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp],
-    "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _cf, _ci, _vp, _vp, _vp],
+    "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _vp, _vp, _vp],
     "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
     "ats_sample_rows": [_vp, _ci, _cll, _ci, _ci, _vp, _vp, _cf, _vp, _ci, _vp, _cf, _vp, _cf, _vp, _cf, _vp, _ci, _cll, _vp, _vp],
 }
@@ -318,11 +318,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status, stream = _p(_lib.status_tensor(q.device)), _lib.stream_ptr(q.device)
     head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
     with _on(q.device):
-        if q.dtype == torch.bfloat16 and d in (64, 128) and ps >= 8 and new * rep <= 16:
+        if q.dtype == torch.bfloat16 and d in (64, 128) and ps >= 8 and new * rep <= 16 and (keys // 16 + 1) * R * n_kv < 1 << 31:
             limit = 8 if new * rep <= 8 else 16
             n = _fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit)
             scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
-            _lib.check(_fn("ats_paged_decode")(*head, keys, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_decode")
+            _lib.check(_fn("ats_paged_decode")(*head, keys, new, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_decode")
         else:
             _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
     return out

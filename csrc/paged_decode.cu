@@ -28,9 +28,10 @@ struct PagedDecodeArgs {
   long long ldo;
   int n_kv, rep, limit;     // rows with at most `limit` MMA rows are taken
   int warps;                // of the main launch
+  int rows_most;            // MMA rows of any row
   int zero_tail;            // tokens behind the last row get zeros
   float scale_log2;
-  long long* line;          // [R + 1]: where a row's units begin, per key head; the end of the line
+  uint32_t* line;           // [R + 1]: where a row's units begin, per key head; the end of the line
   float* part_o;            // [warps, 2, rows of the MMA, D]
   float* part_ml;           // [warps, 2, rows of the MMA, 2]
   int* status;
@@ -61,8 +62,20 @@ __device__ __forceinline__ int pd_units(const PagedDecodeArgs& p, int r) {
   return fresh > 0 && (long long)fresh * p.rep <= p.limit ? (max(keys, 1) + UNIT - 1) / UNIT : 0;
 }
 
-// Warps that share a line of `total` units.
-__device__ __forceinline__ long long pd_shares(const PagedDecodeArgs& p, long long total) { return min((long long)p.warps, total); }
+// A line of `total` units (below 2^31) shared out over as many warps as there are, one more unit to each of the first `extra`.
+struct PdShares {
+  uint32_t n, each, extra;
+  __device__ __forceinline__ PdShares(const PagedDecodeArgs& p, uint32_t total) {
+    n = min(uint32_t(p.warps), total);
+    each = n ? total / n : 0;
+    extra = total - each * n;
+  }
+  __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * each + min(w, extra); }
+  __device__ __forceinline__ uint32_t owner(uint32_t x) const {   // the warp whose stretch holds unit x
+    const uint32_t longer = extra * (each + 1);
+    return x < longer ? x / (each + 1) : extra + (x - longer) / each;
+  }
+};
 
 template <int D, int NR>  // NR: sets of eight MMA rows (1 or 2)
 __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -70,7 +83,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   constexpr int UNIT = 2048 / D, NT = UNIT / 8, KB = UNIT / 16, JD = D / 32, RD = D / 64, ROWS = 8 * NR;
   extern __shared__ uint8_t pd_smem[];
   __shared__ uint64_t s_full[PD_WARPS][PD_STAGES];
-  __shared__ long long s_sum[PD_WARPS], s_at[PD_WARPS];
+  __shared__ uint32_t s_sum[PD_WARPS], s_at[PD_WARPS];
   __shared__ int s_row[PD_WARPS], s_abort;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -86,29 +99,31 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   if (tid == 0) s_abort = 0;
   // where the rows begin on the line: every thread sums up a share of the rows
   const int share = (rows.R + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * share, rows.R), r1 = min(r0 + share, rows.R);
-  long long mine = 0;
+  uint32_t mine = 0;
   for (int r = r0; r < r1; ++r) mine += pd_units<UNIT>(p, r);
-  long long incl = mine;
+  uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  long long total = 0, before = incl - mine;
+  uint32_t total = 0, before = incl - mine;
 #pragma unroll
   for (int w = 0; w < PD_WARPS; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
   total *= p.n_kv;
-  const long long shares = pd_shares(p, total), me0 = (long long)blockIdx.x * PD_WARPS;
+  const PdShares shares(p, total);
+  const uint32_t me0 = blockIdx.x * PD_WARPS;
   for (int r = r0; r < r1; ++r) {
-    const long long n = pd_units<UNIT>(p, r), at = before * p.n_kv;
+    const uint32_t n = pd_units<UNIT>(p, r), at = before * p.n_kv;
     if (blockIdx.x == 0) p.line[r] = before;
-    for (int w = 0; w < PD_WARPS && me0 + w < shares; ++w) {
-      const long long x = (me0 + w) * total / shares;
+#pragma unroll
+    for (int w = 0; w < PD_WARPS; ++w) {
+      const uint32_t x = shares.begin(me0 + w);
       if (at <= x && x < at + n * p.n_kv) s_row[w] = r, s_at[w] = at;
     }
     before += n;
@@ -120,19 +135,19 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
     for (long long i = (long long)blockIdx.x * PD_THREADS + tid; i < (long long)(rows.tokens - tail) * vecs; i += (long long)gridDim.x * PD_THREADS)
       *reinterpret_cast<uint4*>(p.out + (tail + i / vecs) * p.ldo + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
   }
-  const long long me = me0 + warp;
-  if (me >= shares) return;
-  const long long lo = me * total / shares;
-  const int n_mine = int((me + 1) * total / shares - lo);
+  const uint32_t me = me0 + warp;
+  if (me >= shares.n) return;
+  const uint32_t lo = shares.begin(me);
+  const int n_mine = int(shares.begin(me + 1) - lo);
 
   // ---- requests run ahead of the units that are worked on, into the pairs that follow
   const int page = 1 << rows.page_log, box = min(UNIT, page), per = UNIT / box;   // tokens and number of the copies of a unit's 64-column piece
   const int batch = 32 / per;   // units whose coordinates the lanes hold, copy lane % per of unit lane / per
   int q_row = s_row[warp], q_hk, q_unit, q_units = pd_units<UNIT>(p, q_row), q_pages, q_base = 0, here = 0, asked = 0;
   {
-    const long long in_row = lo - s_at[warp];
-    q_hk = int(in_row / q_units);
-    q_unit = int(in_row - (long long)q_hk * q_units);
+    const uint32_t in_row = lo - s_at[warp];
+    q_hk = int(in_row / uint32_t(q_units));
+    q_unit = int(in_row) - q_hk * q_units;
   }
   const int w_row = q_row, w_hk = q_hk, w_unit = q_unit;   // the first unit to work on
   auto pages_of = [&](int r) {
@@ -345,7 +360,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
                 make_uint4(pack_bf16x2(oe[rd][0][2 * x + e] * inv, oo[rd][0][2 * x + e] * inv), pack_bf16x2(oe[rd][1][2 * x + e] * inv, oo[rd][1][2 * x + e] * inv),
                            pack_bf16x2(oe[rd][2][2 * x + e] * inv, oo[rd][2][2 * x + e] * inv), pack_bf16x2(oe[rd][3][2 * x + e] * inv, oo[rd][3][2 * x + e] * inv));
       } else {
-        const long long slot = (me * 2 + (done == count ? 0 : 1)) * ROWS + i;   // the stretch's first piece, or its last
+        const long long slot = ((long long)me * 2 + (done == count ? 0 : 1)) * ROWS + i;   // the stretch's first piece, or its last
         if (t == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(m[x], l[x]);
         float* dst = p.part_o + slot * D + 16 * t;
 #pragma unroll
@@ -362,66 +377,83 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   }
 }
 
-// One CTA per (key head, row, MMA row): the scratch slots of a pair that several warps shared.  D / 4 lanes hold a row's columns; sixteen such
-// groups take the slots in turn, and their sums are joined in order.
-constexpr int PJ_GROUPS = 16;
-template <int D, int NR>
-__global__ void __launch_bounds__(PJ_GROUPS * D / 4) paged_join_kernel(const PagedDecodeArgs p) {
-  constexpr int UNIT = 2048 / D, ROWS = 8 * NR, LANES = D / 4;
-  __shared__ float4 s_acc[PJ_GROUPS][LANES];
-  __shared__ float s_m[PJ_GROUPS], s_l[PJ_GROUPS];
-  const int i = blockIdx.x, hk = blockIdx.y, row = blockIdx.z, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+// The scratch slots of a pair (row, key head) that several warps shared.  D / 4 lanes hold an MMA row's columns; G such groups take the row's slots
+// in turn and are joined in order.  A CTA serves 256 / (G D / 4) MMA rows: many slots (few pairs) want many groups, few slots one or two.
+constexpr int PJ_THREADS = 256;
+template <int D, int NR, int G>
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const PagedDecodeArgs p) {
+  constexpr int ROWS = 8 * NR, LANES = D / 4, AT_ONCE = PJ_THREADS / (G * LANES), UNIT = 2048 / D;
+  __shared__ float4 s_acc[AT_ONCE][G][LANES];
+  __shared__ float s_m[AT_ONCE][G], s_l[AT_ONCE][G];
   pdl_prologue();
+  const int hk = blockIdx.y, row = blockIdx.z, lane = threadIdx.x % LANES, group = threadIdx.x / LANES % G, sub = threadIdx.x / (LANES * G);
+  const int i = blockIdx.x * AT_ONCE + sub;
   int first, fresh, keys;
   paged_row(p.rows, row, &first, &fresh, &keys);
-  const int units = pd_units<UNIT>(p, row);
-  if (i >= fresh * p.rep || units == 0) return;
-  const long long total = p.line[p.rows.R] * p.n_kv, a = p.line[row] * p.n_kv + (long long)hk * units;
-  const long long shares = pd_shares(p, total);
-  auto owner = [&](long long x) { return ((x + 1) * shares - 1) / total; };   // whose stretch holds x: the largest w with w total / shares <= x
-  const long long w0 = owner(a), w1 = owner(a + units - 1);
+  const uint32_t units = pd_units<UNIT>(p, row);
+  const uint32_t total = p.line[p.rows.R] * p.n_kv, a = p.line[row] * p.n_kv + hk * units;
+  if (units == 0) return;
+  const PdShares shares(p, total);
+  const uint32_t w0 = shares.owner(a), w1 = shares.owner(a + units - 1);
   if (w0 == w1) return;   // finished by that warp
-  const long long s0 = 2 * w0 + (w0 * total / shares >= a ? 0 : 1);   // the first one's slot: its first piece unless its stretch began before the pair
+  const bool live = i < fresh * p.rep;
+  const uint32_t s0 = 2 * w0 + (shares.begin(w0) >= a ? 0 : 1);   // the first one's slot: its first piece unless its stretch began before the pair
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
 #pragma unroll 4
-  for (long long w = w0 + group; w <= w1; w += PJ_GROUPS) {
-    const long long at = (w == w0 ? s0 : 2 * w) * ROWS + i;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
-    const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top, keep = pd_from(m, ref), f = pd_from(ml.x, ref);
-    m = top;
-    l = l * keep + ml.y * f;
-    acc = make_float4(acc.x * keep + v.x * f, acc.y * keep + v.y * f, acc.z * keep + v.z * f, acc.w * keep + v.w * f);
+    for (uint32_t w = w0 + group; w <= w1; w += G) {
+      const long long at = (long long)(w == w0 ? s0 : 2 * w) * ROWS + i;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+      const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
+      const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top, keep = pd_from(m, ref), f = pd_from(ml.x, ref);
+      m = top;
+      l = l * keep + ml.y * f;
+      acc = make_float4(acc.x * keep + v.x * f, acc.y * keep + v.y * f, acc.z * keep + v.z * f, acc.w * keep + v.w * f);
+    }
   }
-  s_acc[group][lane] = acc;
-  if (lane == 0) s_m[group] = m, s_l[group] = l;
-  __syncthreads();
-  if (group > 0) return;
-  float top = m;
+  float sum = l;
+  float4 o = acc;
+  if (G > 1) {
+    s_acc[sub][group][lane] = acc;
+    if (lane == 0) s_m[sub][group] = m, s_l[sub][group] = l;
+    __syncthreads();
+    if (group > 0) return;
+    float top = m;
 #pragma unroll
-  for (int x = 1; x < PJ_GROUPS; ++x) top = fmaxf(top, s_m[x]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 1; x < G; ++x) top = fmaxf(top, s_m[sub][x]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int x = 0; x < PJ_GROUPS; ++x) {
-    const float f = pd_from(s_m[x], ref);
-    const float4 v = s_acc[x][lane];
-    sum += s_l[x] * f;
-    o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+    for (int x = 0; x < G; ++x) {
+      const float f = pd_from(s_m[sub][x], ref);
+      const float4 v = s_acc[sub][x][lane];
+      sum += s_l[sub][x] * f;
+      o = make_float4(o.x + v.x * f, o.y + v.y * f, o.z + v.z * f, o.w + v.w * f);
+    }
   }
+  if (!live) return;
   const float inv = sum > 0.f ? 1.f / sum : 1.f;
   const int tok = i / p.rep, head = i - tok * p.rep;
   *reinterpret_cast<uint2*>(p.out + (long long)(first + tok) * p.ldo + (long long)(hk * p.rep + head) * D + 4 * lane) =
       make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
+template <int D, int NR, int G>
+static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
+  constexpr int AT_ONCE = PJ_THREADS / (G * D / 4);
+  const int n = min(p.limit, p.rows_most);
+  return launch_pdl(paged_join_kernel<D, NR, G>, dim3((n + AT_ONCE - 1) / AT_ONCE, p.n_kv, p.rows.R), dim3(PJ_THREADS), 0, s, p);
+}
+
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
   cudaError_t ce = cudaFuncSetAttribute(paged_decode_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_SMEM);
   if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
-  if (ce == cudaSuccess) ce = launch_pdl(paged_join_kernel<D, NR>, dim3(p.limit, p.n_kv, p.rows.R), dim3(PJ_GROUPS * D / 4), 0, s, p);
+  // slots of a pair, if the rows are about as long as each other
+  const int slots = p.warps / (p.rows.R * p.n_kv);
+  if (ce == cudaSuccess) ce = slots >= 8 ? launch_paged_join<D, NR, 8>(p, s) : launch_paged_join<D, NR, 2>(p, s);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }
@@ -438,16 +470,16 @@ using namespace ats;
 
 // Bytes of scratch that `ats_paged_decode` needs (16-byte aligned).
 ATS_API long long ats_paged_decode_scratch(int R, int n_kv, int D, long long max_keys, int limit) {
-  return ((R + 2ll) / 2 * 2) * 8 + 2ll * paged_decode_warps(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
+  return (R + 4ll) / 4 * 16 + 2ll * paged_decode_warps(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
 }
 
 // Rows whose new tokens times n_q / n_kv are at most `limit` (8 or 16).  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens
 // (a power of two) or more; max_keys: no row has more.  zero_tail: tokens behind the last row get zeros.
 ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
-                             void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, long long max_keys, int limit,
+                             void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, long long max_keys, int max_new, int limit,
                              float scale, int zero_tail, void* scratch, int* status, void* stream) {
   if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_kv > 65535 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
-      (limit != 8 && limit != 16) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
+      (limit != 8 && limit != 16) || max_new < 1 || (max_keys / 16 + 1) * R * n_kv >= (1ll << 31) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
     return 1003;
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
@@ -462,10 +494,10 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
-  p.line = static_cast<long long*>(scratch);
-  p.part_o = reinterpret_cast<float*>(p.line + (R + 2) / 2 * 2);
+  p.line = static_cast<uint32_t*>(scratch);
+  p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);
   p.part_ml = p.part_o + 2ll * p.warps * (limit > 8 ? 16 : 8) * D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (limit > 8) return D == 64 ? launch_paged_decode<64, 2>(mk, mv, p, s) : launch_paged_decode<128, 2>(mk, mv, p, s);
