@@ -27,7 +27,7 @@ import torch
 from . import _lib
 
 _vp, _ci, _cll, _cf = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-MAX_ROWS, MAX_TOKENS = 4096, 1 << 18
+MAX_ROWS, MAX_TOKENS, MAX_SLOTS = 4096, 1 << 18, (1 << 31) - 257
 _REFUSED = {1: "a row gets more tokens than its table or the packed batch holds", 2: "not enough free pages", 3: "the stack of free pages is inconsistent"}
 
 
@@ -37,6 +37,8 @@ _SIGNATURES = {
     "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp],
     "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _vp, _vp, _vp],
     "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
+    "ats_paged_portion": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 9 + [_cf, _ci, _vp, _vp, _vp],
+    "ats_paged_portion_scratch": [_ci, _ci],
     "ats_sample_rows": [_vp, _ci, _cll, _ci, _ci, _vp, _vp, _cf, _vp, _ci, _vp, _cf, _vp, _cf, _vp, _cf, _vp, _ci, _cll, _vp, _vp],
 }
 _fns = {}
@@ -82,8 +84,8 @@ class PagePool:
         _need(page_size >= 1 and page_size & (page_size - 1) == 0, f"page_size {page_size}: a power of two is needed")
         _need(1 <= rows <= MAX_ROWS, f"{rows} rows: 1 to {MAX_ROWS} are possible")
         width = -(-max_len // page_size)
-        _need(max_len >= 1 and pages >= 1 and pages * page_size < 1 << 31 and rows * width < 1 << 31 and width * page_size < 1 << 31,
-              "pages and rows: at least one page and one token, and slots below 2^31")
+        _need(max_len >= 1 and pages >= 1 and pages * page_size <= MAX_SLOTS and rows * width < 1 << 31 and width * page_size <= MAX_SLOTS,
+              "pages and rows: at least one page and one token, and slots below 2^31 - 256")
         self.rows, self.pages, self.page_size, self.width = rows, pages, page_size, width
         self.max_len = max_len
         device = torch.device(device)
@@ -212,8 +214,8 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, l
           "k_pages, v_pages: contiguous [pages, page_size, n_kv, d] tensors of the plan's page size are needed")
     _need(k_pages.dtype == v_pages.dtype == like.dtype and k_pages.device == v_pages.device == like.device, "pages and tokens: one type, one device")
     pages, ps, n_kv, d = k_pages.shape
-    _need(pages * ps < 1 << 31, "slots have to stay below 2^31")
     R, T = plan.tables.shape[0], like.shape[0]
+    _need(pages * ps <= MAX_SLOTS and plan.tables.shape[1] * ps <= MAX_SLOTS and R <= MAX_ROWS, "slots have to stay below 2^31 - 256, rows at 4096")
     _ints(plan.tables, "plan.tables", plan.tables.shape, like.device)
     _ints(plan.lengths, "plan.lengths", (R,), like.device)
     _ints(plan.starts, "plan.starts", (R + 1,), like.device)
@@ -318,13 +320,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status, stream = _p(_lib.status_tensor(q.device)), _lib.stream_ptr(q.device)
     head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
     with _on(q.device):
-        if q.dtype == torch.bfloat16 and d in (64, 128) and ps >= 8 and new * rep <= 16 and (keys // 16 + 1) * R * n_kv < 1 << 31:
-            limit = 8 if new * rep <= 8 else 16
-            n = _fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit)
-            scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
-            _lib.check(_fn("ats_paged_decode")(*head, keys, new, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_decode")
-        else:
+        if q.dtype != torch.bfloat16 or d not in (64, 128) or ps < 8 or rep > 128 or (keys // 16 + 1) * R * n_kv >= 1 << 31:
             _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
+            return out
+        # Rows of a few query rows (new tokens times heads of a group) are a stream of the cache, longer portions a matter of the tensor cores.  A batch may
+        # hold both, and which is which the kernels find in the plan; the host only knows when there can be none of one kind.
+        limit = 0 if rep > 16 else 8 if new * rep <= 8 or rep <= 8 < 16 < new * rep else 16
+        portions = new * rep > limit
+        if portions:
+            scratch = torch.empty(_fn("ats_paged_portion_scratch")(R, d), dtype=torch.uint8, device=q.device)
+            _lib.check(_fn("ats_paged_portion")(*head, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_portion")
+        if limit:
+            scratch = torch.empty(_fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit), dtype=torch.uint8, device=q.device)
+            _lib.check(_fn("ats_paged_decode")(*head, keys, T if portions else new, limit, scale, int(not keep_tail and not portions), _p(scratch), status, stream), "ats_paged_decode")
     return out
 
 

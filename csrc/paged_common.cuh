@@ -4,18 +4,24 @@
 
 namespace ats {
 
-// Pages [rows, n_kv, d] of bf16 (rows = pages * page) as 64-column pieces of one head, 128-byte swizzle; the box is `box_rows` tokens of a page.
-inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, uint64_t n_kv, uint64_t d, uint32_t box_rows) {
+// bf16 [rows, heads, d], rows `ld` elements apart, as boxes of 64 columns x `box_heads` heads x `box_rows` rows, 128-byte swizzle; rows behind the last
+// read as zero.
+inline int make_tmap_tokens(CUtensorMap* out, const void* base, uint64_t rows, uint64_t heads, uint64_t d, uint64_t ld, uint32_t box_heads, uint32_t box_rows) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return 1000;
-  if (reinterpret_cast<uintptr_t>(base) & 15) return 1001;
-  cuuint64_t dims[3] = {d, n_kv, rows};
-  cuuint64_t strides[2] = {d * 2, n_kv * d * 2};
-  cuuint32_t box[3] = {64, 1, box_rows};
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (ld & 7) || (d & 7)) return 1001;
+  cuuint64_t dims[3] = {d, heads, rows};
+  cuuint64_t strides[2] = {d * 2, ld * 2};
+  cuuint32_t box[3] = {64, box_heads, box_rows};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 1100 + int(r);
+}
+
+// Pages [rows, n_kv, d] (rows = pages * page): `box_rows` tokens of one head.
+inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, uint64_t n_kv, uint64_t d, uint32_t box_rows) {
+  return make_tmap_tokens(out, base, rows, n_kv, d, n_kv * d, 1, box_rows);
 }
 
 struct PagedRows {

@@ -28,7 +28,8 @@ struct PagedDecodeArgs {
   long long ldo;
   int n_kv, rep, limit;     // rows with at most `limit` MMA rows are taken
   int warps;                // of the main launch
-  int rows_most;            // MMA rows of any row
+  int max_new;              // no row has more new tokens
+  int rows_most;            // MMA rows of any row that is taken
   int zero_tail;            // tokens behind the last row get zeros
   float scale_log2;
   uint32_t* line;           // [R + 1]: where a row's units begin, per key head; the end of the line
@@ -120,7 +121,10 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   const uint32_t me0 = blockIdx.x * PD_WARPS;
   for (int r = r0; r < r1; ++r) {
     const uint32_t n = pd_units<UNIT>(p, r), at = before * p.n_kv;
-    if (blockIdx.x == 0) p.line[r] = before;
+    if (blockIdx.x == 0) {
+      p.line[r] = before;
+      if (rows.starts[r + 1] - rows.starts[r] > p.max_new) atomicCAS(p.status, 0, int(kBadArgument));   // more than the caller promised: nobody serves the row
+    }
 #pragma unroll
     for (int w = 0; w < PD_WARPS; ++w) {
       const uint32_t x = shares.begin(me0 + w);
@@ -479,7 +483,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
                              void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, long long max_keys, int max_new, int limit,
                              float scale, int zero_tail, void* scratch, int* status, void* stream) {
   if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_kv > 65535 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
-      (limit != 8 && limit != 16) || max_new < 1 || (max_keys / 16 + 1) * R * n_kv >= (1ll << 31) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
+      (limit != 8 && limit != 16) || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) || max_new < 1 || (max_keys / 16 + 1) * R * n_kv >= (1ll << 31) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
     return 1003;
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
@@ -494,7 +498,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.line = static_cast<uint32_t*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);
