@@ -11,18 +11,38 @@
 //   evaluation puts it: the rounding of all masses together moves a border by 2^-43 sqrt(V) of the largest mass or so.
 //   2^42 times 2^20 tokens stays below 2^63.
 // * NaN counts as -infinity (mass 0), -0 as 0.
+//
+// One cluster per row, a contiguous slice of the vocabulary per CTA, read once into shared memory where it fits.  No sort of the vocabulary:
+// tokens are counted by how far below the largest they lie (4,095 bins over the 30.5 T that have any mass, and one for the rest), which brackets a
+// cut between two bins; only the tokens of the bracket are collected, sorted and cut exactly.
+//   top-k           the largest of every eight tokens is counted: k of these above a bin mean k tokens above it, and the tokens from there up are a
+//                   little more than k.  They are all that is kept, so nothing but these few needs an exponential.
+//   top-p alone     one pass for the masses' sum and the counts; the counts bound the cumulative mass to a bin's width (0.75 %) from either side, the
+//                   bracket is what lies between; a second pass sums what is above it, and if the bracket holds too many tokens still, its own sum
+//                   is now uncertain by 0.75 % only: the next bracket is a hundredth of it.
+//   neither         one pass of masses.
+// Cuts whose brackets do not fit the list (thousands of equal scores, k above 1,024) are found by bisection over the 64-bit order.
+// The draw works on sums per 256 consecutive tokens and looks into one of them.
+// Bound by the 64-bit exponentials of rows without top-k (13 FP64 operations a token and pass), else by latency: three to five cluster barriers.
 #include "common.cuh"
 
 namespace ats {
 
-constexpr int SR_THREADS = 1024;
+constexpr int SR_THREADS = 512, SR_WARPS = SR_THREADS / 32;
 constexpr int SR_MASS_BITS = 42;
 constexpr int SR_MAX_VOCAB = 1 << 20;
+constexpr int SR_BINS = 4096;          // the last one: no mass
+constexpr float SR_RANGE = 30.5f;      // in units of T: exp(-30.49) 2^42 rounds to nothing
+constexpr int SR_LIST = 2048;
+constexpr int SR_MAX_K = 1024;
+constexpr int SR_CHUNK = 256;
+constexpr int SR_MAX_CLUSTER = 8;
 
 struct SampleRowsArgs {
   const void* logits;   // [B, ld] bf16 or fp32
   long long ld;
-  int fp32, V;
+  int V, slice;         // tokens of a CTA (a multiple of SR_CHUNK)
+  int cached;           // the slice is kept in shared memory
   const float* uniform;       // [B]
   const float* temperature;   // [B], or null: the number beside it
   const int* top_k;
@@ -37,33 +57,72 @@ struct SampleRowsArgs {
   long long* out;             // [B]
 };
 
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* red) {
+template <typename T>
+struct SampleRowsSmem {   // byte offsets of the dynamic shared memory
+  int hist, list, chunks, seen, raw, total;
+  __host__ __device__ SampleRowsSmem(int slice, bool cached) {
+    hist = 0;                            // u32 [SR_BINS]; later u64 [SR_LIST]: this CTA's tokens of the bracket, or masses of the list
+    list = hist + SR_BINS * 4;           // u64 [SR_LIST]: the cluster's tokens of the bracket (rank 0); before that the cluster's counts
+    chunks = list + SR_LIST * 8;         // u64 [slice / SR_CHUNK]
+    seen = chunks + slice / SR_CHUNK * 8;        // one bit per token of the slice
+    raw = (seen + slice / 8 + 15) / 16 * 16;     // the slice
+    total = raw + (cached ? slice * int(sizeof(T)) : 0);
+  }
+};
+
+__device__ __forceinline__ uint64_t sr_ld_u64(const void* local, uint32_t rank) {   // the same place in another CTA of the cluster
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(local), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t sr_ld_u32(const void* local, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(local), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sr_st_u64(void* local, uint32_t rank, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(local), rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void sr_st_u32(void* local, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(local), rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint64_t sr_warp_sum(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  return v;
+}
+// Sum over the block (valid in all threads); two barriers, so `red` [SR_WARPS] may be used again at once.
+__device__ __forceinline__ uint64_t sr_block_sum(uint64_t v, uint64_t* red) {
+  v = sr_warp_sum(v);
   __syncthreads();
-  if (l == 0) red[w] = v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   uint64_t t = 0;
 #pragma unroll
-  for (int i = 0; i < SR_THREADS / 32; ++i) t += red[i];
+  for (int i = 0; i < SR_WARPS; ++i) t += red[i];
   return t;
 }
-
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* red) {
+// Exclusive prefix over the block's threads; *total: the sum.
+template <typename N>
+__device__ __forceinline__ N sr_block_scan(N v, N* red, N* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  N incl = v;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
+  for (int o = 1; o < 32; o <<= 1) {
+    const N u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
   }
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   __syncthreads();
-  if (l == 0) red[w] = v;
+  if (lane == 31) red[warp] = incl;
   __syncthreads();
-  uint64_t t = 0;
+  N before = incl - v, all = 0;
 #pragma unroll
-  for (int i = 0; i < SR_THREADS / 32; ++i) t = red[i] > t ? red[i] : t;
-  return t;
+  for (int w = 0; w < SR_WARPS; ++w) {
+    if (w < warp) before += red[w];
+    all += red[w];
+  }
+  *total = all;
+  return before;
 }
 
 // order-preserving image of a float without NaN
@@ -73,121 +132,560 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-__global__ void __launch_bounds__(SR_THREADS) sample_rows_kernel(const SampleRowsArgs p) {
+// exp(-w) for w >= 0: w = n ln 2 / 32 - z, |z| <= ln 2 / 64; exp(z) by its Taylor series to the fifth power (the next term is below 2^-48), 2^-(n mod 32)/32
+// from a table.
+__device__ __forceinline__ double sr_exp_neg(double w, const double* table) {
+  constexpr double magic = 6755399441055744.0;   // 1.5 * 2^52
+  const double t = fma(w, 32 * 1.4426950408889634074, magic);
+  const int n = __double2loint(t);
+  const double z = fma(t - magic, 0.69314718055994530942 / 32, -w);
+  double r = fma(z, 1.0 / 120, 1.0 / 24);
+  r = fma(r, z, 1.0 / 6);
+  r = fma(r, z, 0.5);
+  r = fma(r, z, 1.0);
+  r = fma(r, z, 1.0) * table[n & 31];
+  return __hiloint2double(__double2hiint(r) - ((n >> 5) << 20), __double2loint(r));   // (n / 32 stays far from the smallest exponents)
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const SampleRowsArgs p) {
   pdl_prologue();
-  extern __shared__ uint32_t s_seen[];   // one bit per token of the history
-  __shared__ uint64_t red[SR_THREADS / 32];
-  __shared__ int s_pick;
-  const int b = blockIdx.x, tid = threadIdx.x, V = p.V;
+  extern __shared__ __align__(16) uint8_t sr_smem[];
+  __shared__ uint64_t red[SR_WARPS], s_top, s_sum[2], s_cut;
+  __shared__ double red_d[SR_WARPS], s_table[32];
+  __shared__ uint32_t red_u[SR_WARPS], s_count, s_found;   // tokens of the bracket: this CTA's, the cluster's (rank 0)
+  __shared__ int s_bracket[3];
+  constexpr int PER = 16 / sizeof(T);
+  const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, groups = p.slice / 8;
+  const SampleRowsSmem<T> at(p.slice, p.cached);
+  uint32_t* hist = reinterpret_cast<uint32_t*>(sr_smem + at.hist);
+  uint64_t* near = reinterpret_cast<uint64_t*>(sr_smem + at.hist);
+  uint64_t* masses = near;
+  uint64_t* list = reinterpret_cast<uint64_t*>(sr_smem + at.list);
+  uint32_t* counts = reinterpret_cast<uint32_t*>(sr_smem + at.list);
+  uint64_t* chunks = reinterpret_cast<uint64_t*>(sr_smem + at.chunks);
+  uint32_t* seen = reinterpret_cast<uint32_t*>(sr_smem + at.seen);
+  T* raw = reinterpret_cast<T*>(sr_smem + at.raw);
+  auto csync = [&]() {
+    if (C > 1) cluster_sync_all();
+    else __syncthreads();
+  };
   const float temp = p.temperature ? p.temperature[b] : p.temperature1;
   const int top_k = p.top_k ? p.top_k[b] : p.top_k1;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p1;
-  const float min_p = fminf(p.min_p ? p.min_p[b] : p.min_p1, 1.f);   // the first token always stays
+  const double low = double(fminf(p.min_p ? p.min_p[b] : p.min_p1, 1.f));   // the first token always stays
   const float pen = p.penalty ? p.penalty[b] : p.penalty1;
   const bool penalise = p.history != nullptr && pen != 1.f;
+  const T* row = static_cast<const T*>(p.logits) + (long long)b * p.ld;
+  // Slices are cut so that they begin at whole 16 bytes: token i0 + j is the slice's j-th; places before token 0 and behind the last hold -infinity.
+  const int i0 = rank * p.slice - int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+
+  // ---- the slice into shared memory, the history's bits
+  auto fetch = [&](int v) -> uint4 {   // 16 bytes of the row: tokens i0 + v * PER ..
+    const int i = i0 + v * PER;
+    if (i >= 0 && i + PER <= V) return *reinterpret_cast<const uint4*>(row + i);
+    uint4 out;
+    T* o = reinterpret_cast<T*>(&out);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = i + e >= 0 && i + e < V ? row[i + e] : T(-INFINITY);
+    return out;
+  };
+  if (p.cached) {
+#pragma unroll 4
+    for (int v = tid; v < p.slice / PER; v += SR_THREADS) reinterpret_cast<uint4*>(raw)[v] = fetch(v);
+  }
+  if (penalise)
+    for (int i = tid; i < p.slice / 32; i += SR_THREADS) seen[i] = 0;
+  for (int i = tid; i < SR_BINS; i += SR_THREADS) hist[i] = 0;
+  if (tid < 32) s_table[tid] = exp2(-double(tid) / 32);
+  if (tid == 0) s_count = 0, s_found = 0;
+  __syncthreads();
   if (penalise) {
-    for (int i = tid; i < (V + 31) / 32; i += SR_THREADS) s_seen[i] = 0;
-    __syncthreads();
     for (int j = tid; j < p.hist_len; j += SR_THREADS) {
-      const long long tok = p.history[b * p.hist_ld + j];
-      if (tok >= 0 && tok < V) atomicOr(&s_seen[tok >> 5], 1u << (tok & 31));
+      const long long id = p.history[b * p.hist_ld + j], tok = id - i0;
+      if (id >= 0 && id < V && tok >= 0 && tok < p.slice) atomicOr(&seen[tok >> 5], 1u << (tok & 31));
     }
     __syncthreads();
   }
-  auto key = [&](int i) -> uint64_t {
-    float x = p.fp32 ? static_cast<const float*>(p.logits)[b * p.ld + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[b * p.ld + i]);
-    if (penalise && (s_seen[i >> 5] >> (i & 31) & 1)) x = x > 0.f ? __fdiv_rn(x, pen) : __fmul_rn(x, pen);
-    if (x != x) x = -INFINITY;
-    x += 0.f;
-    return (uint64_t(order_key(x)) << 32) | (0xffffffffu - uint32_t(i));
+  auto load8 = [&](int g, float (&x)[8]) {   // the scores of the slice's tokens 8 g ..
+    uint4 w[8 / PER];
+#pragma unroll
+    for (int e = 0; e < 8 / PER; ++e) w[e] = p.cached ? reinterpret_cast<const uint4*>(raw)[g * (8 / PER) + e] : fetch(g * (8 / PER) + e);
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(u[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(u[e] << 16), x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+    }
+    if (penalise) {
+      const uint32_t bits = reinterpret_cast<const uint8_t*>(seen)[g];
+      if (bits) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (bits >> e & 1) x[e] = x[e] > 0.f ? __fdiv_rn(x[e], pen) : __fmul_rn(x[e], pen);
+      }
+    }
   };
+  auto key_of = [&](float x, int j) -> uint64_t { return (uint64_t(order_key(x + 0.f)) << 32) | (0xffffffffu - uint32_t(i0 + j)); };
+
+  // ---- the first token of the order
+  {
+    float best = -INFINITY;
+    int j_best = -1;
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (x[e] > best) best = x[e], j_best = 8 * g + e;
+    }
+    uint64_t k = j_best >= 0 ? key_of(best, j_best) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t u = __shfl_xor_sync(0xffffffffu, k, o);
+      k = u > k ? u : k;
+    }
+    if (lane == 0) red[warp] = k;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < SR_WARPS; ++w) k = red[w] > k ? red[w] : k;
+      s_top = k;
+    }
+  }
+  csync();
   uint64_t top = 0;
-  for (int i = tid; i < V; i += SR_THREADS) {
-    const uint64_t k = key(i);
+  for (int r = 0; r < C; ++r) {
+    const uint64_t k = sr_ld_u64(&s_top, r);
     top = k > top ? k : top;
   }
-  top = block_max_u64(top, red);
-  const int arg = int(0xffffffffu - uint32_t(top));
+  const int arg = top ? int(0xffffffffu - uint32_t(top)) : 0;   // (0: nothing above -infinity)
   const float x_max = key_value(uint32_t(top >> 32));
-  if (!(temp > 0.f) || x_max == -INFINITY) {
-    if (tid == 0) p.out[b] = arg;
+
+  const double inv_t = 1.0 / double(temp), x_top = double(x_max);
+  const float per_bin = float(SR_BINS - 1) / (SR_RANGE * temp);
+  auto bin_of = [&](float x) -> int {   // does not fall as x falls; fp32 rounding moves a border by less than a hundredth of a bin.  NaN: the last one
+    const float d = x == x_max ? 0.f : (x_max - x) * per_bin;
+    return int(fminf(d, float(SR_BINS - 1)));
+  };
+  // relative to the first token's; the last bin's (which has none) as that of its border
+  auto weight = [&](float x, int bin) -> double { return sr_exp_neg(x == x_max || bin == SR_BINS - 1 ? 0.0 : (x_top - double(x)) * inv_t, s_table); };
+  auto fixed = [&](double w) -> uint64_t {   // round(w * 2^42)
+    return uint64_t(__double_as_longlong(fma(w, double(1ll << SR_MASS_BITS), 4503599627370496.0))) & ((1ull << 52) - 1);
+  };
+  auto mass = [&](float x) -> uint64_t {
+    const int bin = bin_of(x);
+    return bin == SR_BINS - 1 ? 0 : fixed(weight(x, bin));
+  };
+  auto cluster_sum = [&](uint64_t v, int slot) -> uint64_t {   // (one barrier; the slots take turns)
+    const uint64_t mine = sr_block_sum(v, red);
+    if (tid == 0) s_sum[slot] = mine;
+    csync();
+    uint64_t t = 0;
+    for (int r = 0; r < C; ++r) t += sr_ld_u64(&s_sum[slot], r);
+    return t;
+  };
+  const double u = fmax(double(p.uniform[b]), 0.0);
+  auto target_of = [&](uint64_t total) -> uint64_t {
+    const double want = u * double(total);
+    return want < double(total) ? min(uint64_t(want), total - 1) : total - 1;
+  };
+  auto collect = [&](float x, int j, bool mine_too) {   // into rank 0's list, and this CTA's own
+    const uint64_t k = key_of(x, j);
+    uint32_t i;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(i) : "r"(mapa_shared(smem_u32(&s_found), 0)) : "memory");
+    if (i < SR_LIST) sr_st_u64(&list[i], 0, k);
+    if (mine_too) {
+      i = atomicAdd(&s_count, 1u);
+      if (i < SR_LIST) near[i] = k;
+    }
+  };
+  // what is kept, per SR_CHUNK consecutive tokens (one group a lane): `kept(x, bin, j)` says whether the token is, as far as its mass does not.  -> the mass
+  // of these before min-p, this thread's share
+  auto sum_chunks = [&](auto kept, bool add) -> uint64_t {   // (add: to the sums that are there)
+    uint64_t all = 0;
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
+      uint64_t v = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int bin = bin_of(x[e]);
+        const bool in = kept(x[e], bin, 8 * g + e);
+        const double w = weight(x[e], bin);
+        const uint64_t m = in ? fixed(w) : 0;
+        all += m;
+        v += w >= low ? m : 0;
+      }
+      v = sr_warp_sum(v);
+      if (lane == 0) chunks[g >> 5] = add ? chunks[g >> 5] + v : v;
+    }
+    __syncthreads();
+    return all;
+  };
+
+  const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.f;
+  if (!(temp > 0.f) || top == 0) {
+    if (rank == 0 && tid == 0) p.out[b] = arg;
+    if (C > 1) cluster_sync_all();   // nobody leaves while its shared memory is read
     return;
   }
-  const double inv_t = 1.0 / double(temp);
-  auto weight = [&](uint64_t k) -> double {   // relative to the first token's
-    const float x = key_value(uint32_t(k >> 32));
-    return x == x_max ? 1.0 : exp((double(x) - double(x_max)) * inv_t);
-  };
-  auto mass = [&](uint64_t k) -> uint64_t { return uint64_t(__double2ll_rn(weight(k) * double(1ll << SR_MASS_BITS))); };
-  uint64_t cut = 0;   // tokens with at least this key stay
-  if (top_k > 0 && top_k < V) {   // the k-th largest key, bit by bit
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t trial = cut | (1ull << bit);
-      uint64_t c = 0;
-      for (int i = tid; i < V; i += SR_THREADS) c += key(i) >= trial;
-      if (block_sum_u64(c, red) >= uint64_t(top_k)) cut = trial;
-    }
-  }
-  if (top_p < 1.f) {   // the smallest key with mass above it <= top_p Z
-    uint64_t z = 0;
-    for (int i = tid; i < V; i += SR_THREADS) {
-      const uint64_t k = key(i);
-      if (k >= cut) z += mass(k);
-    }
-    const double limit = double(fmaxf(top_p, 0.f)) * double(block_sum_u64(z, red));
-    uint64_t lo = cut, hi = top;
-    while (lo < hi) {
-      const uint64_t mid = lo + ((hi - lo) >> 1);
-      uint64_t above = 0;
-      for (int i = tid; i < V; i += SR_THREADS) {
-        const uint64_t k = key(i);
-        if (k > mid) above += mass(k);
-      }
-      if (double(block_sum_u64(above, red)) <= limit) hi = mid;
-      else lo = mid + 1;
-    }
-    cut = lo;
-  }
-  const double low = double(min_p);
-  auto kept_mass = [&](int i) -> uint64_t {
-    const uint64_t k = key(i);
-    if (k < cut) return 0;
-    const double w = weight(k);
-    return w >= low ? uint64_t(__double2ll_rn(w * double(1ll << SR_MASS_BITS))) : 0;
-  };
-  // in index order: a run of tokens per thread
-  const int seg = (V + SR_THREADS - 1) / SR_THREADS, i0 = min(tid * seg, V), i1 = min(i0 + seg, V);
-  uint64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += kept_mass(i);
-  const uint64_t total = block_sum_u64(mine, red);
-  uint64_t incl = mine;
-  const int lane = tid & 31, warp = tid >> 5;
+  bool bisect = by_k && top_k > SR_MAX_K, listed = false;   // listed: the answer is among the list's tokens
+  int b_lo = 0;
+  uint64_t cut = 0, z = 0, above = 0;   // tokens with at least the key `cut` are kept
+  // rank 0, with `found` tokens in the list, `above` the mass of what is in front of them: the cut, and the answer if nothing is in front of them
+  auto finish_list = [&](uint32_t found) {
+    auto sort = [&](uint32_t m) {   // the list's first m entries, largest first (bitonic, padded with zeros)
+      uint32_t size = 1;
+      while (size < m) size *= 2;
+      for (uint32_t i = m + tid; i < size; i += SR_THREADS) list[i] = 0;
+      __syncthreads();
+      for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+          for (uint32_t i = tid; i < size / 2; i += SR_THREADS) {
+            const uint32_t a = 2 * i - (i & (j - 1)), c = a + j;
+            const uint64_t va = list[a], vc = list[c];
+            if ((va < vc) == ((a & k) == 0)) list[a] = vc, list[c] = va;
+          }
+          __syncthreads();
+        }
+    };
+    sort(found);
+    // masses and their prefix: SR_LIST / SR_THREADS consecutive tokens a thread
+    constexpr int EACH = SR_LIST / SR_THREADS;
+    const uint32_t m = by_k ? min(found, uint32_t(top_k)) : found;
+    uint64_t v[EACH], own = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
-  }
-  __syncthreads();
-  if (lane == 31) red[warp] = incl;
-  if (tid == 0) s_pick = arg;
-  __syncthreads();
-  uint64_t before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += red[w];
-  const double u = fmax(double(p.uniform[b]), 0.0);
-  const double want = u * double(total);
-  const uint64_t target = want < double(total) ? min((uint64_t)want, total - 1) : total - 1;
-  if (mine > 0 && target >= before && target < before + mine) {
-    uint64_t run = before;
-    for (int i = i0; i < i1; ++i) {
-      run += kept_mass(i);
-      if (run > target) {
-        s_pick = i;
-        break;
+    for (int e = 0; e < EACH; ++e) {
+      const uint32_t i = tid * EACH + e;
+      v[e] = i < m ? mass(key_value(uint32_t(list[i] >> 32))) : 0;
+      own += v[e];
+    }
+    uint64_t all, run = sr_block_scan<uint64_t>(own, red, &all) + above;
+    const double limit = by_p ? double(fmaxf(top_p, 0.f)) * double(by_k ? all : z) : INFINITY;
+    uint32_t kept = 0, n_kept;
+    own = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const uint32_t i = tid * EACH + e;
+      if (i < m) {
+        // both rules keep a leading run; a token without mass is never the answer
+        const bool in = double(run) <= limit;
+        kept += in;
+        run += in ? v[e] : 0;
+        const float x = key_value(uint32_t(list[i] >> 32));
+        if (!in || !(weight(x, bin_of(x)) >= low)) v[e] = 0;
+        own += v[e];
+        if (listed) masses[i] = v[e];
+      }
+    }
+    sr_block_scan<uint32_t>(kept, red_u, &n_kept);
+    if (!listed) {
+      if (tid == 0) s_cut = n_kept > 0 ? list[n_kept - 1] : ~0ull;
+      return;
+    }
+    // all that is kept is here: in index order, the token whose mass covers the target
+    const uint64_t target = target_of(sr_block_sum(own, red));
+    for (uint32_t i = tid; i < n_kept; i += SR_THREADS) list[i] = (list[i] << 32) | i;   // (what was the low half falls as the index grows)
+    __syncthreads();
+    sort(n_kept);
+    own = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const uint32_t i = tid * EACH + e;
+      v[e] = i < n_kept ? masses[uint32_t(list[i])] : 0;
+      own += v[e];
+    }
+    run = sr_block_scan<uint64_t>(own, red, &all);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (run <= target && target < run + v[e]) p.out[b] = int(0xffffffffu - uint32_t(list[tid * EACH + e] >> 32));
+      run += v[e];
+    }
+  };
+
+  if (by_k && !bisect) {
+    // ---- counts of the largest of every eight tokens, eight bins in one
+    constexpr int WIDE = SR_BINS / SR_THREADS;
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
+      float m = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
+      const int bin = bin_of(m);
+      if (bin < SR_BINS - 1) atomicAdd(&hist[bin / WIDE], 1u);
+    }
+    csync();
+    uint32_t c = 0, all;
+    for (int r = 0; r < C; ++r) c += sr_ld_u32(&hist[tid], r);
+    const uint32_t before = sr_block_scan<uint32_t>(c, red_u, &all);
+    if (tid == 0) s_bracket[1] = SR_BINS - 2;   // fewer than k with any mass: all that have some
+    __syncthreads();
+    if (before < uint32_t(top_k) && before + c >= uint32_t(top_k)) s_bracket[1] = min((tid + 1) * WIDE - 1, SR_BINS - 2);
+    __syncthreads();
+    const int b_hi = s_bracket[1];
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e, false);
+    }
+    csync();
+    const uint32_t found = sr_ld_u32(&s_found, 0);
+    bisect = found > SR_LIST;
+    listed = !bisect;
+    if (listed && rank == 0) finish_list(found);
+  } else if (by_p && !bisect) {
+    // ---- counts of all tokens, and the masses' sum
+    uint64_t v = 0;
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int bin = bin_of(x[e]);
+        const uint64_t m = fixed(weight(x[e], bin));
+        if (bin < SR_BINS - 1) {
+          atomicAdd(&hist[bin], 1u);
+          v += m;
+        }
+      }
+    }
+    z = cluster_sum(v, 0);
+    // a share of the bins each, into rank 0's counts
+    for (int i = rank * (SR_BINS / C) + tid; i < (rank + 1) * (SR_BINS / C); i += SR_THREADS) {
+      uint32_t c = 0;
+      for (int r = 0; r < C; ++r) c += sr_ld_u32(&hist[i], r);
+      sr_st_u32(&counts[i], 0, c);
+    }
+    csync();
+    // ---- the bracket, in rounds: what is above it is summed exactly, which narrows the next one to a bin's width of what is left
+    int done = 0;        // bins that are summed
+    bool last = false;
+    for (int round = 0; !last; ++round) {
+      if (rank == 0) {
+        constexpr int EACH = SR_BINS / SR_THREADS;
+        if (tid == 0) s_bracket[0] = done, s_bracket[1] = SR_BINS - 2;
+        __syncthreads();
+        // bounds of the cumulative mass through each bin, in units of the largest mass: a bin's tokens lie within a hundredth of a bin of it, a
+        // mass is rounded by 2^-43, and the sums here by less than a part in 10^9
+        const double unit = 1.0 / double(1ll << SR_MASS_BITS), width = double(SR_RANGE) / (SR_BINS - 1), limit = double(fmaxf(top_p, 0.f)) * double(z) * unit;
+        auto most_of = [&](int i, double c) { return c * (sr_exp_neg(fmax(width * (i - 0.02), 0.0), s_table) * (1 + 2e-4 * (i == 0)) + unit); };
+        auto least_of = [&](int i, double c) { return c * fmax(sr_exp_neg(width * (i + 1.02), s_table) - unit, 0.0); };
+        double own_most = 0, own_least = 0;
+        uint32_t c[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int i = tid * EACH + e;
+          c[e] = i < SR_BINS - 1 ? counts[i] : 0;
+          own_most += i >= done ? most_of(i, c[e]) : 0;
+          own_least += i >= done ? least_of(i, c[e]) : 0;
+        }
+        double all;
+        double run_most = sr_block_scan<double>(own_most, red_d, &all) + double(above) * unit;
+        double run_least = sr_block_scan<double>(own_least, red_d, &all) + double(above) * unit;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int i = tid * EACH + e;
+          if (i < done) continue;
+          const double next_most = run_most + most_of(i, c[e]), next_least = run_least + least_of(i, c[e]);
+          if (run_most * (1 + 1e-9) <= limit && next_most * (1 + 1e-9) > limit) s_bracket[0] = i;
+          if (run_least * (1 - 1e-9) <= limit && next_least * (1 - 1e-9) > limit) s_bracket[1] = i;
+          run_most = next_most, run_least = next_least;
+        }
+        __syncthreads();
+        // does the bracket fit the list, or even all tokens down to its end?
+        const int from = s_bracket[0], to = s_bracket[1];
+        uint32_t upto = 0, in = 0, n_upto, n_in;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int i = tid * EACH + e;
+          upto += i <= to ? c[e] : 0;
+          in += i >= from && i <= to ? c[e] : 0;
+        }
+        sr_block_scan<uint32_t>(upto, red_u, &n_upto);
+        sr_block_scan<uint32_t>(in, red_u, &n_in);
+        if (tid == 0) {
+          if (done == 0 && n_upto <= SR_LIST) s_bracket[0] = 0;
+          s_bracket[2] = n_in <= SR_LIST || from == done || round == 4;   // (the last two: it gets no narrower)
+        }
+      }
+      csync();
+      b_lo = int(sr_ld_u32(&s_bracket[0], 0));
+      const int b_hi = int(sr_ld_u32(&s_bracket[1], 0));
+      last = b_lo == 0 || sr_ld_u32(&s_bracket[2], 0) != 0;
+      csync();   // the counts have been read: the last round's tokens take their place
+      // sum what is above the bracket, collect its tokens once it is the last
+      uint64_t more = 0;
+      if (b_lo > 0)
+        more = sum_chunks([&](float x, int bin, int j) -> bool {
+          if (last && bin >= b_lo && bin <= b_hi) collect(x, j, true);
+          return bin >= done && bin < b_lo;
+        }, done > 0);
+      else
+        for (int g = tid; g < groups; g += SR_THREADS) {
+          float x[8];
+          load8(g, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e, false);
+        }
+      above += cluster_sum(more, (round & 1) ^ 1);
+      done = b_lo;
+    }
+    const uint32_t found = sr_ld_u32(&s_found, 0);
+    bisect = found > SR_LIST;
+    listed = !bisect && b_lo == 0;
+    if (!bisect) {
+      if (rank == 0) finish_list(found);
+      if (!listed) {
+        csync();
+        cut = sr_ld_u64(&s_cut, 0);
+        for (uint32_t i = tid; i < s_count; i += SR_THREADS)   // the bracket's part of what is kept
+          if (near[i] >= cut) {
+            const float x = key_value(uint32_t(near[i] >> 32));
+            const double w = weight(x, bin_of(x));
+            if (w >= low) atomicAdd(reinterpret_cast<unsigned long long*>(&chunks[(int(0xffffffffu - uint32_t(near[i])) - i0) / SR_CHUNK]), (unsigned long long)fixed(w));
+          }
+        __syncthreads();
       }
     }
   }
-  __syncthreads();
-  if (tid == 0) p.out[b] = s_pick;
+  if (!listed) {
+    const bool chunked = !bisect && by_p;   // the chunks hold what is kept
+    int slot = 0;
+    if (bisect) {
+      csync();   // the sum last taken may still be read
+      auto total_of = [&](auto f) {
+        uint64_t v = 0;
+        for (int g = tid; g < groups; g += SR_THREADS) {
+          float x[8];
+          load8(g, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = x[e] == x[e] ? x[e] : -INFINITY;
+            const int i = i0 + 8 * g + e;
+            if (i >= 0 && i < V) v += f(y, 8 * g + e);
+          }
+        }
+        slot ^= 1;
+        return cluster_sum(v, slot);
+      };
+      cut = 0;
+      if (by_k) {   // the k-th largest key, bit by bit
+        for (int bit = 63; bit >= 0; --bit) {
+          const uint64_t trial = cut | (1ull << bit);
+          if (total_of([&](float x, int j) -> uint64_t { return key_of(x, j) >= trial; }) >= uint64_t(top_k)) cut = trial;
+        }
+      }
+      if (by_p) {   // the smallest key with mass above it <= top_p Z
+        const uint64_t zz = total_of([&](float x, int j) -> uint64_t { return key_of(x, j) >= cut ? mass(x) : 0; });
+        const double limit = double(fmaxf(top_p, 0.f)) * double(zz);
+        uint64_t lo = cut, hi = top;
+        while (lo < hi) {
+          const uint64_t mid = lo + ((hi - lo) >> 1);
+          if (double(total_of([&](float x, int j) -> uint64_t { return key_of(x, j) > mid ? mass(x) : 0; })) <= limit) hi = mid;
+          else lo = mid + 1;
+        }
+        cut = lo;
+      }
+    }
+    auto is_kept = [&](float x, int bin, int j) -> bool { return bin < SR_BINS - 1 && ((chunked && bin < b_lo) || key_of(x, j) >= cut); };
+    if (!chunked) sum_chunks(is_kept, false);
+    uint64_t mine = 0;
+    for (int c = tid; c < p.slice / SR_CHUNK; c += SR_THREADS) mine += chunks[c];
+    // (the sums of the CTAs one by one: where the target lies)
+    const uint64_t own = sr_block_sum(mine, red);
+    if (tid == 0) s_sum[slot ^ 1] = own;
+    csync();
+    uint64_t total = 0, before = 0;
+    for (int r = 0; r < C; ++r) {
+      const uint64_t v = sr_ld_u64(&s_sum[slot ^ 1], r);
+      if (r < rank) before += v;
+      total += v;
+    }
+    const uint64_t target = target_of(total);
+    if (own > 0 && target >= before && target < before + own && warp == 0) {
+      // one warp: the chunk, 32 at a time, then the group of eight, then the token
+      uint64_t run = before;
+      auto step = [&](uint64_t v, int* which) -> bool {   // the lane whose value covers the target, or go on behind all of them
+        uint64_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t w = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += w;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, run + incl > target);
+        const int from = hit ? __ffs(hit) - 1 : 31;
+        run += __shfl_sync(0xffffffffu, hit ? incl - v : incl, from);
+        *which = from;
+        return hit != 0;
+      };
+      const int n_chunks = p.slice / SR_CHUNK;
+      int w = 0, pick = arg;
+      bool found = false;
+      int c = 0;
+      for (; c < n_chunks && !found; c += 32) found = step(c + lane < n_chunks ? chunks[c + lane] : 0, &w);
+      if (found) {
+        const int chunk = c - 32 + w, g = chunk * 32 + lane;
+        float x[8];
+        load8(g, x);
+        uint64_t m[8], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int bin = bin_of(x[e]);
+          const double wt = weight(x[e], bin);
+          m[e] = is_kept(x[e], bin, 8 * g + e) && wt >= low ? fixed(wt) : 0;
+          sum += m[e];
+        }
+        if (step(sum, &w)) {
+          if (lane == w) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (run <= target && target < run + m[e]) pick = i0 + 8 * g + e;
+              run += m[e];
+            }
+          }
+          pick = __shfl_sync(0xffffffffu, pick, w);
+        }
+      }
+      if (lane == 0) p.out[b] = pick;
+    }
+  }
+  if (C > 1) cluster_sync_all();   // nobody leaves while its shared memory is read
+}
+
+template <typename T>
+static int launch_sample_rows(SampleRowsArgs& p, int B, cudaStream_t s) {
+  // As many CTAs a row as keep its slices in shared memory (64 KB each, so that an SM holds two), more while the rows leave SMs idle and a CTA
+  // keeps 2,048 tokens.
+  int C = 1;
+  while (C < SR_MAX_CLUSTER && (long long)p.V * sizeof(T) > C * 65536ll) C *= 2;
+  while (C < SR_MAX_CLUSTER && 2 * C * B <= 148 && p.V > C * 2048) C *= 2;
+  p.slice = (p.V + 7 + C * SR_CHUNK - 1) / (C * SR_CHUNK) * SR_CHUNK;   // (up to seven places in front of the first token)
+  p.cached = (long long)p.slice * sizeof(T) <= 131072 + SR_CHUNK * 8;
+  const SampleRowsSmem<T> at(p.slice, p.cached);
+  cudaError_t ce = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, at.total);
+  if (ce != cudaSuccess) return int(ce);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, B);
+  cfg.blockDim = dim3(SR_THREADS);
+  cfg.dynamicSmemBytes = at.total;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  ce = cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, p);
+  if (ce != cudaSuccess) return int(ce);
+  return int(cudaGetLastError());
 }
 
 }  // namespace ats
@@ -198,16 +696,12 @@ using namespace ats;
 ATS_API int ats_sample_rows(const void* logits, int fp32, long long ld, int B, int V, const float* uniform, const float* temperature, float temperature1,
                             const int* top_k, int top_k1, const float* top_p, float top_p1, const float* min_p, float min_p1, const float* penalty, float penalty1,
                             const long long* history, int hist_len, long long hist_ld, long long* out, void* stream) {
-  if (B < 1 || V < 1 || V > SR_MAX_VOCAB || hist_len < 0) return 1003;
+  if (B < 1 || B > 65535 || V < 1 || V > SR_MAX_VOCAB || hist_len < 0) return 1003;
   SampleRowsArgs p;
-  p.logits = logits; p.ld = ld; p.fp32 = fp32; p.V = V; p.uniform = uniform;
+  p.logits = logits; p.ld = ld; p.V = V; p.uniform = uniform;
   p.temperature = temperature; p.temperature1 = temperature1; p.top_k = top_k; p.top_k1 = top_k1; p.top_p = top_p; p.top_p1 = top_p1;
   p.min_p = min_p; p.min_p1 = min_p1; p.penalty = penalty; p.penalty1 = penalty1;
   p.history = hist_len > 0 ? history : nullptr; p.hist_len = hist_len; p.hist_ld = hist_ld; p.out = out;
-  const size_t smem = p.history ? size_t((V + 31) / 32) * 4 : 0;
-  cudaError_t ce = cudaSuccess;
-  if (smem > 40 * 1024) ce = cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (ce == cudaSuccess) ce = launch_pdl(sample_rows_kernel, dim3(B), dim3(SR_THREADS), smem, static_cast<cudaStream_t>(stream), p);
-  if (ce != cudaSuccess) return int(ce);
-  return int(cudaGetLastError());
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return fp32 ? launch_sample_rows<float>(p, B, s) : launch_sample_rows<__nv_bfloat16>(p, B, s);
 }
