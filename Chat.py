@@ -103,8 +103,9 @@ class ChatInterface:
         self.history += [{"role": "user", "content": user_text}, {"role": "assistant", "content": text}]
         return text
 
-    def respond_many(self, user_texts, max_batch: int = 16):
-        """Independent single-turn prompts served together: continuous batching over ``max_batch`` cache rows (GPU only)."""
+    def respond_many(self, user_texts, max_batch: int = 16, page_size=None):
+        """Independent single-turn prompts served together: continuous batching over ``max_batch`` cache rows (GPU only), with ``page_size`` in pages
+        of so many tokens that the rows share."""
         from adaptivetrainingsystem_b200.inference import ContinuousBatcher
         saved, self.history = self.history, []
         try:
@@ -112,7 +113,7 @@ class ChatInterface:
         finally:
             self.history = saved
         rows = max(len(p) for p in prompts) + self.params.max_new_tokens
-        batcher = ContinuousBatcher(self.engine, max_batch=min(max_batch, len(prompts)), max_len=rows, params=self.params)
+        batcher = ContinuousBatcher(self.engine, max_batch=min(max_batch, len(prompts)), max_len=rows, params=self.params, page_size=page_size)
         return [self.tokenizer.decode(t) for t in batcher.run(prompts)]
 
     def continue_ids(self, ids, new_tokens: int):
@@ -172,6 +173,7 @@ if __name__ == "__main__":
                     help="with --quantize int4: load the packed 4-bit copies from this file if it exists (the bf16 projections are freed), else write them there")
     ap.add_argument("--prompts-file", default=None, help="one prompt per line, answered together by continuous batching")
     ap.add_argument("--max-batch", type=int, default=16)
+    ap.add_argument("--page-size", type=int, default=None, help="with --prompts-file: key / value cache in pages of so many tokens (a power of two)")
     a = ap.parse_args()
     chat = ChatInterface(a.checkpoint, a.device, a.mode, a.quantize, a.quantized_file, a.model)
     if a.token_ids:
@@ -179,7 +181,7 @@ if __name__ == "__main__":
     elif a.prompts_file:
         with open(a.prompts_file) as f:
             lines = [l.strip() for l in f if l.strip()]
-        for q, ans in zip(lines, chat.respond_many(lines, a.max_batch)):
+        for q, ans in zip(lines, chat.respond_many(lines, a.max_batch, a.page_size)):
             print(f"> {q}\n{ans}\n")
     elif a.prompt:
         print(chat.respond(a.prompt))

@@ -43,6 +43,7 @@ class SamplingParams:
     max_new_tokens: int = 512
     stop_token_ids: Sequence[int] = field(default_factory=tuple)
     seed: Optional[int] = None
+    min_p: float = 0.0
 
     @classmethod
     def from_mode(cls, mode: str, **kw) -> "SamplingParams":
@@ -53,7 +54,13 @@ def sample_next(logits: torch.Tensor, params: SamplingParams, history: Optional[
                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
     """logits [B, V] -> token ids [B].  Order of operations as in the reference (``Chat.py:391-425``): repetition
     penalty over the last ``repetition_window`` tokens, temperature, top-k, top-p, multinomial; ``temperature <= 0``
-    is greedy.  On a GPU the whole chain is one kernel launch per step (bisection on the logit values instead of a sort)."""
+    is greedy.  On a GPU the whole chain is one kernel launch per step (bisection on the logit values instead of a sort).  ``min_p`` > 0 draws with
+    :func:`ops.sample_rows` (tokens below that share of the likeliest one's mass are dropped after top-p)."""
+    if params.min_p > 0:
+        from .. import ops
+        hist = history[:, -params.repetition_window:] if history is not None and history.numel() else None
+        return ops.sample_rows(logits, torch.rand(logits.shape[0], device=logits.device, generator=generator), params.temperature, params.top_k, params.top_p, params.min_p,
+                               params.repetition_penalty, hist)
     if logits.is_cuda and logits.dim() == 2:
         from ..ops import serving
         hist = history[:, -params.repetition_window:] if history is not None and history.numel() else None

@@ -10,6 +10,10 @@ The rows live in a :class:`SequencePool` (one cache of ``max_batch`` rows and on
    unchanged and their output is ignored), samples one token per row in one launch;
 3. retires rows that produced a stop token or their token budget and frees their slots.
 
+With ``page_size`` the rows live in a :class:`PagedPool` instead: a request takes pages for its own prompt and budget rather than a row of
+``max_len``, and the portions that a step admits run as one packed batch.  A request may bring sampling numbers of its own
+(:meth:`ContinuousBatcher.submit`); then the step's tokens are drawn by ``ops.sample_rows``, still in one launch.
+
 The reference's own generator serves one sequence at a time and re-runs the context for every token (``Chat.py:355-465``); its
 vendored serving engine keeps a slot table per batch (``colossalai/inference/kv_cache/kvcache_manager.py:11-106`` allocator,
 ``kv_cache/batch_infer_state.py:13-118`` per-batch lengths and start locations), which is the bookkeeping done here on rows.
@@ -17,12 +21,15 @@ vendored serving engine keeps a slot table per batch (``colossalai/inference/kv_
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .. import ops
 from .engine import GenerationEngine, SamplingParams, sample_next
-from .pool import SequencePool
+from .pool import PagedPool, SequencePool
+
+MAX_PACKED = 8192   # prompt tokens that run as one packed batch
 
 
 @dataclass
@@ -34,11 +41,13 @@ class Request:
     slot: int = -1
     prefilled: int = 0                        # prompt tokens the row already holds
     done: bool = False
+    params: Optional[SamplingParams] = None   # sampling numbers of its own
 
 
 class ContinuousBatcher:
     def __init__(self, engine: GenerationEngine, max_batch: int = 64, max_len: int = 2048, params: Optional[SamplingParams] = None,
-                 prefill_chunk: Optional[int] = None):
+                 prefill_chunk: Optional[int] = None, page_size: Optional[int] = None, pages: Optional[int] = None):
+        """``page_size``: rows share ``pages`` pages of so many tokens (by default as many as ``max_batch`` rows of ``max_len`` take)."""
         self.engine, self.model = engine, engine.model
         self.params = params or SamplingParams.from_mode("greedy")
         self.max_batch, self.max_len = max_batch, max_len
@@ -47,7 +56,8 @@ class ContinuousBatcher:
         if getattr(self.model, "_ep_comm", None) is not None:
             # admission prefills one request on one rank, which the expert-parallel exchange (a collective of all ranks) cannot serve
             raise RuntimeError("continuous batching runs on one GPU (or on replicas): the model must not be expert-parallel")
-        self.pool = SequencePool(self.model, max_batch, max_len)
+        self.paged = page_size is not None
+        self.pool = PagedPool(self.model, max_batch, max_len, pages, page_size) if self.paged else SequencePool(self.model, max_batch, max_len)
         self.cache, self.slots = self.pool.cache, self.pool.slots
         self.history = torch.zeros(max_batch, self.params.repetition_window, dtype=torch.long, device=self.device)
         self.by_slot: Dict[int, Request] = {}          # rows that decode
@@ -56,16 +66,22 @@ class ContinuousBatcher:
         self.finished: Dict[int, Request] = {}
         self._next_id = 0
         self._stop = set(int(t) for t in (self.params.stop_token_ids or ()))
+        self._own = 0                                  # requests under way that bring sampling numbers of their own
+        self._numbers: Optional[Dict[str, torch.Tensor]] = None   # per row, once such a request has come
         self.steps = 0
         self.generator = torch.Generator(device=self.device).manual_seed(self.params.seed) if self.params.seed is not None else None
 
     # -- requests --------------------------------------------------------------------------------------------------
-    def submit(self, prompt: Sequence[int], max_new_tokens: Optional[int] = None) -> int:
+    def submit(self, prompt: Sequence[int], max_new_tokens: Optional[int] = None, params: Optional[SamplingParams] = None) -> int:
+        """``params``: sampling numbers, stop tokens and token budget of this request (its ``repetition_window`` is the batcher's, as are the random
+        numbers)."""
         ids = torch.as_tensor(prompt, dtype=torch.long).flatten()
-        budget = int(max_new_tokens if max_new_tokens is not None else self.params.max_new_tokens)
+        budget = int(max_new_tokens if max_new_tokens is not None else (params or self.params).max_new_tokens)
+        if self.paged and self.pool.cache.pool.pages_for(ids.numel() + budget) > self.pool.pages:
+            raise ValueError(f"prompt of {ids.numel()} tokens + {budget} new tokens does not fit {self.pool.pages} pages")
         if ids.numel() < 1 or ids.numel() + budget > self.max_len:
             raise ValueError(f"prompt of {ids.numel()} tokens + {budget} new tokens does not fit rows of {self.max_len}")
-        r = Request(self._next_id, ids, budget)
+        r = Request(self._next_id, ids, budget, params=params)
         self._next_id += 1
         self.waiting.append(r)
         return r.rid
@@ -74,11 +90,36 @@ class ContinuousBatcher:
     def pending(self) -> int:
         return len(self.waiting) + len(self.prefilling) + len(self.by_slot)
 
+    # -- sampling ----------------------------------------------------------------------------------------------------
+    _FIELDS: Tuple[Tuple[str, torch.dtype], ...] = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32),
+                                                    ("repetition_penalty", torch.float32))
+
+    def _set_numbers(self, slot: int, params: SamplingParams) -> None:
+        if self._numbers is None:
+            self._numbers = {n: torch.full((self.max_batch,), getattr(self.params, n), dtype=t, device=self.device) for n, t in self._FIELDS}
+        for n, _ in self._FIELDS:
+            self._numbers[n][slot] = getattr(params, n)
+
+    def _sample(self, logits: torch.Tensor, slot: Optional[int] = None) -> torch.Tensor:
+        """Tokens of all rows, or of row ``slot`` alone."""
+        history = self.history if slot is None else self.history[slot:slot + 1]
+        if not self._own:
+            return sample_next(logits, self.params, history, self.generator)
+        n = {k: v if slot is None else v[slot:slot + 1] for k, v in self._numbers.items()}
+        uniform = torch.rand(logits.shape[0], device=self.device, generator=self.generator)
+        return ops.sample_rows(logits, uniform, n["temperature"], n["top_k"], n["top_p"], n["min_p"], n["repetition_penalty"], history)
+
     # -- one scheduling step ---------------------------------------------------------------------------------------
     @torch.no_grad()
     def _admit(self) -> None:
         budget = self.prefill_chunk or (1 << 62)       # prompt tokens this step may still run
         while budget > 0:
+            if self.paged:
+                used = self._admit_packed(min(budget, MAX_PACKED))
+                if not used:
+                    return
+                budget -= used
+                continue
             if not self.prefilling:
                 if not (self.waiting and self.pool.available):
                     return
@@ -96,12 +137,41 @@ class ContinuousBatcher:
                 self.prefilling.pop(0)
                 self._first_token(r, logits)
 
+    def _admit_packed(self, room: int) -> int:
+        """The next portions of prompts, oldest first, up to ``room`` tokens in one packed batch -> tokens that were run."""
+        taken: List[Tuple[Request, torch.Tensor]] = []
+        left = room
+        while left > 0:
+            r = self.prefilling[len(taken)] if len(taken) < len(self.prefilling) else None
+            if r is None:
+                # (requests wait for their turn: a later one that is shorter does not overtake)
+                if not (self.waiting and self.pool.fits(self.waiting[0].prompt.numel() + self.waiting[0].max_new_tokens)):
+                    break
+                r = self.waiting.pop(0)
+                r.slot = self.pool.open(r.prompt.numel() + r.max_new_tokens)
+                self.prefilling.append(r)
+            n = min(left, r.prompt.numel() - r.prefilled)
+            taken.append((r, r.prompt[r.prefilled:r.prefilled + n]))
+            r.prefilled += n
+            left -= n
+        if not taken:
+            return 0
+        logits = self.pool.extend_many([(r.slot, part) for r, part in taken])
+        for i, (r, _) in enumerate(taken):
+            if r.prefilled == r.prompt.numel():
+                self.prefilling.remove(r)
+                self._first_token(r, logits[i:i + 1])
+        return room - left
+
     def _first_token(self, r: Request, logits: torch.Tensor) -> None:
         slot, ids, w = r.slot, r.prompt.to(self.device), self.history.shape[1]
         n = ids.numel()
         self.history[slot].fill_(int(r.prompt[0]))     # left padding of a short prompt repeats its first token
         self.history[slot, -min(n, w):] = ids[-min(n, w):]
-        first = sample_next(logits, self.params, self.history[slot:slot + 1], self.generator)
+        self._own += r.params is not None
+        if r.params is not None or self._numbers is not None:
+            self._set_numbers(slot, r.params or self.params)
+        first = self._sample(logits, slot)
         self.pool.last[slot:slot + 1] = first
         self.history[slot] = torch.roll(self.history[slot], -1)
         self.history[slot, -1:] = first
@@ -112,12 +182,14 @@ class ContinuousBatcher:
         """Host-side bookkeeping of one generated token (the device-side state was updated for all rows at once)."""
         r = self.by_slot[slot]
         r.tokens.append(token)
-        if token in self._stop or len(r.tokens) >= r.max_new_tokens:
+        stop = self._stop if r.params is None else r.params.stop_token_ids
+        if token in stop or len(r.tokens) >= r.max_new_tokens:
             self._retire(slot)
 
     def _retire(self, slot: int) -> None:
         r = self.by_slot.pop(slot)
         r.done = True
+        self._own -= r.params is not None
         self.finished[r.rid] = r
         self.pool.close(slot)
 
@@ -129,7 +201,7 @@ class ContinuousBatcher:
         if not live:
             return 0
         logits = self.pool.decode(live)
-        nxt_dev = sample_next(logits, self.params, self.history, self.generator)
+        nxt_dev = self._sample(logits)
         self.pool.last.copy_(nxt_dev)
         self.history = torch.roll(self.history, -1, dims=1)
         self.history[:, -1] = nxt_dev

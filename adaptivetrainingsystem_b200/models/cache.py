@@ -2,7 +2,8 @@
 
 :class:`SequenceCache` is the part every model shares: the fill level, its device-side copy for decode steps that are replayed from a
 CUDA graph, and row views for schedulers that admit sequences one by one into a pool.  ``KVCache`` (``transformer.py``) holds keys and
-values of every position; :class:`LayerStateCache` holds whatever its layers declare -- rings of the last tokens, recurrent states,
+values of every position in a row per sequence, :class:`PagedKVCache` the same in pages that rows share out among themselves;
+:class:`LayerStateCache` holds whatever its layers declare -- rings of the last tokens, recurrent states,
 convolution inputs -- one entry per layer *run*, so a layer that is run several times per token has a state for each run.
 """
 from __future__ import annotations
@@ -10,6 +11,8 @@ from __future__ import annotations
 from typing import Dict, List, Optional
 
 import torch
+
+from .. import ops
 
 
 class SequenceCache:
@@ -65,3 +68,38 @@ class LayerStateCache(SequenceCache):
 
     def row(self, i: int) -> "LayerStateCache":
         return LayerStateCache(1, self.max_len, self.device, [{k: t[i:i + 1] for k, t in s.items()} for s in self.states])
+
+
+class PagedKVCache(SequenceCache):
+    """Keys and values of ``batch`` rows in ``pages`` pages of ``page_size`` tokens, per layer ``[pages, page_size, Hkv, D]`` (``ops.PagePool``).  A row
+    takes pages as it grows, so memory follows the tokens that rows hold, not the longest that they might.
+
+    A step of the model is planned first (:meth:`plan`): it runs the new tokens of all rows packed one row after the other, portions of prompts
+    ``[1, T]`` or, with ``single``, at most one token per row ``[rows, 1]`` (the form that is captured in a CUDA graph)."""
+
+    def __init__(self, num_layers: int, batch: int, max_len: int, pages: int, page_size: int, n_kv: int, head_dim: int, dtype, device):
+        super().__init__(batch, max_len, device)
+        self.pool = ops.PagePool(batch, max_len, pages, page_size, device)
+        self.k = [torch.zeros(pages, page_size, n_kv, head_dim, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.v = [torch.zeros(pages, page_size, n_kv, head_dim, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.step: Optional[ops.PagePlan] = None
+
+    def plan(self, fresh: torch.Tensor, tokens: int, max_new: Optional[int] = None, max_len: Optional[int] = None, single: bool = False) -> "ops.PagePlan":
+        """``fresh`` int32 [batch]: new tokens of every row (-1: the row is closed), ``tokens`` of them in all at most."""
+        self.step = ops.page_plan(self.pool, fresh, tokens, max_new=1 if single else max_new, max_len=max_len)
+        # a step of single tokens reads positions from the device, like a replayed step over contiguous rows
+        self.device_lengths, self.device_positions = (self.step.lengths, self.step.positions) if single else (None, None)
+        return self.step
+
+    def advance(self, n: int) -> None:
+        pass   # the plan moves the rows on
+
+    def device_advance(self) -> None:
+        pass
+
+    def attend(self, layer: int, qkv: torch.Tensor, n_q: int, n_kv: int, d: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor]) -> torch.Tensor:
+        """qkv [..., (n_q + 2 n_kv) d], the step's packed projection, rotated already where ``cos`` is ``None`` -> [..., n_q * d]."""
+        if cos is not None and qkv.is_cuda and d % 16:   # (heads that the kernel does not rotate)
+            qkv, cos, sin = ops.rope_packed(qkv, cos, sin, n_q, n_kv, d, positions=self.step.positions.view(qkv.shape[:-1])), None, None
+        q = ops.paged_append(qkv.reshape(-1, qkv.shape[-1]), cos, sin, self.step, self.k[layer], self.v[layer], n_q, n_kv, d)
+        return ops.paged_attention(q, self.k[layer], self.v[layer], self.step).reshape(*qkv.shape[:-1], n_q * d)

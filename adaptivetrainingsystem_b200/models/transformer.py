@@ -31,7 +31,7 @@ from ..config import ModelConfig
 from .. import ops
 from ..ops import moe as moe_ops
 from ..ops import mod as mod_ops
-from .cache import SequenceCache
+from .cache import PagedKVCache, SequenceCache
 
 
 class RMSNorm(nn.Module):
@@ -166,13 +166,22 @@ class GroupedQueryAttention(nn.Module):
             if qkv is None:
                 qkv = ops.linear(h, self.qkv_proj, reduce_group=self.tp_group)
                 qkv = ops.rope_packed(qkv, rope.cos, rope.sin, self.n_q, self.n_kv, self.d, positions=cache.device_positions.view(B, 1))
-            a = ops.decode_attention(qkv, cache.k[self.layer_idx], cache.v[self.layer_idx], cache.device_lengths, self.n_q, self.n_kv, self.d)
+            if isinstance(cache, PagedKVCache):
+                a = cache.attend(self.layer_idx, qkv, self.n_q, self.n_kv, self.d, None, None)
+            else:
+                a = ops.decode_attention(qkv, cache.k[self.layer_idx], cache.v[self.layer_idx], cache.device_lengths, self.n_q, self.n_kv, self.d)
             if post_norm is not None and self.tp_group is None:  # the fold of the output projection adds the residual and normalises
                 fused = ops.serving.out_proj_norm(a.reshape(B, -1), self.o_proj, residual.reshape(B, -1), post_norm.weight, post_norm.eps, scaled)
                 if fused is not None:
                     return fused[0].view(residual.shape), fused[1].view(residual.shape)
             x = self._project_out(a, residual)
             return (x, None) if post_norm is not None else x
+        if isinstance(cache, PagedKVCache):
+            if attention_mask is not None or positions is not None:
+                raise ValueError("a step over a paged cache takes its positions and what a token sees from the cache's plan")
+            rope.ensure(cache.max_len, h.device)
+            a = cache.attend(self.layer_idx, ops.linear(h, self.qkv_proj, reduce_group=self.tp_group), self.n_q, self.n_kv, self.d, rope.cos, rope.sin)
+            return self._project_out(a, residual)
         rope.ensure(offset + L if positions is None else int(self.cfg.seq_length), h.device)
         qkv = ops.linear(h, self.qkv_proj, reduce_group=self.tp_group)
         nq, nk = self.n_q * self.d, self.n_kv * self.d
@@ -656,6 +665,14 @@ class DeepSeekTransformer(nn.Module):
         p = self.embed_tokens.weight
         n_kv = self.layers[0].self_attn.n_kv if len(self.layers) else self.config.num_kv_heads  # this rank's KV heads (tensor parallelism)
         return KVCache(self.config.num_layers, batch, max_len, n_kv, self.config.head_dim, dtype or p.dtype, device or p.device)
+
+    def make_paged_cache(self, rows: int, max_len: int, pages: int, page_size: int = 64) -> PagedKVCache:
+        """A cache of ``rows`` rows of up to ``max_len`` tokens that share ``pages`` pages."""
+        if self.get_mod_layers():
+            raise ValueError("a step over a paged cache packs tokens of many sequences; Mixture-of-Depths layers choose tokens per sequence")
+        p = self.embed_tokens.weight
+        n_kv = self.layers[0].self_attn.n_kv if len(self.layers) else self.config.num_kv_heads
+        return PagedKVCache(self.config.num_layers, rows, max_len, pages, page_size, n_kv, self.config.head_dim, p.dtype, p.device)
 
 
 # ----------------------------------------------------------------------------------------------------------

@@ -253,7 +253,7 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
         raise ValueError(f"pages hold {hk} heads of {dk}, the projection {n_kv} of {d}")
     if cos is not None:
         _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d // 2 and cos.dtype == sin.dtype == torch.float32
-              and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == qkv.device and d % 16 == 0,
+              and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == qkv.device and (d % 16 == 0 or not qkv.is_cuda and d % 2 == 0),
               "cos, sin: contiguous float32 tables [positions, d / 2] on the projection's device, d a multiple of 16")
     if not qkv.is_cuda:
         return _paged_append_reference(qkv, cos, sin, plan, k_pages, v_pages, n_q, n_kv, d)

@@ -1,0 +1,120 @@
+"""Rows over a paged cache: the pool and the batcher on it (CPU; on a GPU in test_gpu_paged_pool.py)."""
+import pytest
+import torch
+
+from adaptivetrainingsystem_b200.config import ModelConfig
+from adaptivetrainingsystem_b200.inference import ContinuousBatcher, GenerationEngine, PagedPool, SamplingParams, sample_next
+from adaptivetrainingsystem_b200.models import DeepSeekTransformer
+
+
+def _model(moe=False, **kw):
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=97, hidden_size=32, num_layers=2, num_heads=4, num_kv_heads=2, intermediate_size=64, seq_length=64, use_moe=moe, num_experts=4,
+                      moe_top_k=2, capacity_factor=4.0, routing_noise_std=0.0, **kw)
+    model = DeepSeekTransformer(cfg).eval()
+    with torch.no_grad():
+        model.lm_head.mul_(8.0)
+    return model
+
+
+@pytest.mark.parametrize("moe", [False, True])
+@torch.no_grad()
+def test_rows_equal_sequences_of_their_own(moe):
+    """Portions packed with other rows' and single tokens beside other rows give the logits of the whole sequence on its own."""
+    model = _model(moe)
+    pool = PagedPool(model, 4, 40, pages=14, page_size=8, use_graph=False)
+    g = torch.Generator().manual_seed(1)
+    seqs = [torch.randint(0, 97, (n,), generator=g) for n in (20, 33, 9)]
+    rows = [pool.open(n) for n in (20, 33, 9)]
+    fed = [7, 16, 1]
+    logits = pool.extend_many([(rows[i], seqs[i][:fed[i]]) for i in (2, 0, 1)])      # in any order
+    got = {i: logits[j] for j, i in enumerate((2, 0, 1))}
+    for step in range(12):
+        for i, s in enumerate(seqs):
+            want = model(s[None, :fed[i]], return_aux_loss=False)[0, -1]
+            assert torch.allclose(got[i], want, atol=2e-4), (step, i)
+        live = [i for i in range(3) if fed[i] < seqs[i].numel() and (i + step) % 3]
+        if step == 5:                                                             # a portion in the middle
+            live = []
+            if fed[1] + 6 <= 33:
+                got[1] = pool.extend(rows[1], seqs[1][fed[1]:fed[1] + 6])[0]
+                fed[1] += 6
+        if not live:
+            continue
+        for i in live:
+            pool.last[rows[i]] = seqs[i][fed[i]]
+            fed[i] += 1
+        out = pool.decode(sorted(rows[i] for i in live))
+        for i in live:
+            got[i] = out[rows[i]]
+    pool.cache.pool.check()
+    for r in rows:
+        pool.close(r)
+    assert pool.pages_left == 14 and int(pool.cache.pool.state[0]) == 14 and pool.available == 4
+
+
+def test_pool_refusals():
+    model = _model()
+    pool = PagedPool(model, 2, 32, pages=5, page_size=8, use_graph=False)
+    a = pool.open(17)
+    assert pool.pages_left == 2 and pool.fits(16) and not pool.fits(17)
+    with pytest.raises(RuntimeError, match="pages are free"):
+        pool.open(17)
+    with pytest.raises(RuntimeError, match="no room"):
+        pool.extend(a, torch.zeros(25, dtype=torch.long))
+    with pytest.raises(ValueError, match="different rows"):
+        pool.extend_many([(a, [1]), (a, [2])])
+    with pytest.raises(ValueError, match="at least one token"):
+        pool.extend_many([(a, [])])
+    with pytest.raises(ValueError, match="power of two"):
+        PagedPool(model, 2, 32, page_size=12)
+    with pytest.raises(ValueError, match="Mixture-of-Depths"):
+        PagedPool(_model(use_mod=True), 2, 32)
+    with pytest.raises(ValueError, match="plan"):
+        model(torch.zeros(1, 2, dtype=torch.long), attention_mask=torch.ones(1, 2), cache=pool.cache)
+
+
+@pytest.mark.parametrize("chunk", [None, 5])
+def test_batcher_serves_more_rows_than_whole_rows_would_fit(chunk, monkeypatch):
+    """Greedy requests over pages against each one on its own; pages for a third of the rows at full length."""
+    model = _model()
+    eng = GenerationEngine(model)
+    monkeypatch.setattr(PagedPool, "_capture", lambda self: setattr(self, "use_graph", False))
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(0, 97, (n,), generator=g).tolist() for n in (5, 17, 3, 11, 8, 2, 14)]
+    budgets = [6, 4, 9, 5, 7, 3, 6]
+    batcher = ContinuousBatcher(eng, max_batch=6, max_len=40, params=SamplingParams.from_mode("greedy"), prefill_chunk=chunk, page_size=4, pages=20)
+    rids = [batcher.submit(p, b) for p, b in zip(prompts, budgets)]
+    peak = 0
+    while batcher.pending:
+        peak = max(peak, batcher.step())
+    for p, b, r in zip(prompts, budgets, rids):
+        want = eng.generate(torch.tensor([p]), SamplingParams.from_mode("greedy", max_new_tokens=b), use_graph=False)["tokens"][0].tolist()
+        assert batcher.finished[r].tokens == want
+    assert peak >= 3 and batcher.pool.pages_left == 20 and int(batcher.cache.pool.state[0]) == 20
+    with pytest.raises(ValueError, match="pages"):
+        ContinuousBatcher(eng, max_batch=2, max_len=40, page_size=4, pages=5).submit([1] * 20, 8)
+
+
+def test_requests_with_sampling_numbers_of_their_own():
+    model = _model()
+    eng = GenerationEngine(model)
+    batcher = ContinuousBatcher(eng, max_batch=4, max_len=40, params=SamplingParams.from_mode("greedy", seed=3), page_size=8)
+    batcher.pool.use_graph = False
+    greedy = batcher.submit([1, 2, 3], 8)
+    sure = batcher.submit([1, 2, 3], params=SamplingParams(temperature=2.0, top_k=1, repetition_penalty=1.0, max_new_tokens=8))
+    tiny = batcher.submit([1, 2, 3], params=SamplingParams(temperature=2.0, top_k=0, top_p=1.0, min_p=1.0, repetition_penalty=1.0, max_new_tokens=8))
+    wild = batcher.submit([1, 2, 3], params=SamplingParams(temperature=50.0, top_k=0, top_p=1.0, repetition_penalty=1.0, max_new_tokens=8))
+    first = eng.generate(torch.tensor([[1, 2, 3]]), SamplingParams.from_mode("greedy", max_new_tokens=8), use_graph=False)["tokens"][0].tolist()
+    stops = batcher.submit([1, 2, 3], params=SamplingParams.from_mode("greedy", stop_token_ids=(first[2],), max_new_tokens=8))
+    while batcher.pending:
+        batcher.step()
+    done = {n: batcher.finished[r].tokens for n, r in (("greedy", greedy), ("sure", sure), ("tiny", tiny), ("wild", wild), ("stops", stops))}
+    assert done["greedy"] == done["sure"] == done["tiny"] == first and done["wild"] != first and done["stops"] == first[:first.index(first[2]) + 1]
+    assert batcher._own == 0
+
+
+def test_min_p_in_sampling_params():
+    x = torch.tensor([[0.0, 5.0, 4.0, -3.0]]).expand(200, -1)
+    kept = sample_next(x, SamplingParams(temperature=1.0, top_k=0, top_p=1.0, repetition_penalty=1.0, min_p=0.2)).unique().tolist()
+    assert kept == [1, 2]
