@@ -38,7 +38,7 @@ _SIGNATURES = {
     "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _vp, _vp, _vp],
     "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
     "ats_paged_portion": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 9 + [_cf, _ci, _vp, _vp, _vp],
-    "ats_paged_portion_scratch": [_ci, _ci],
+    "ats_paged_portion_scratch": [_ci],
     "ats_sample_rows": [_vp, _ci, _cll, _ci, _ci, _vp, _vp, _cf, _vp, _ci, _vp, _cf, _vp, _cf, _vp, _cf, _vp, _ci, _cll, _vp, _vp],
 }
 _fns = {}
@@ -328,7 +328,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         limit = 0 if rep > 16 else 8 if new * rep <= 8 or rep <= 8 < 16 < new * rep else 16
         portions = new * rep > limit
         if portions:
-            scratch = torch.empty(_fn("ats_paged_portion_scratch")(R, d), dtype=torch.uint8, device=q.device)
+            scratch = torch.empty(_fn("ats_paged_portion_scratch")(d), dtype=torch.uint8, device=q.device)
             _lib.check(_fn("ats_paged_portion")(*head, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_portion")
         if limit:
             scratch = torch.empty(_fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit), dtype=torch.uint8, device=q.device)

@@ -9,7 +9,7 @@
 // Bound by the tensor cores and the exponentials (per block of 128 keys and tile 2 x 128 x 128 x D products, 16,384 exponentials).
 //
 // Rows, portions and caches are of any length, so work is dealt out in key blocks: all (row, key head, pair of tiles), each as long as the keys
-// that its last token sees, form one line, and each of 148 CTAs takes an equal stretch of it.  The roles of a CTA run through the pieces of
+// that its last token sees and PC_PIECE more for its beginning and end, form one line, and each of 148 CTAs takes an equal stretch of it.  The roles of a CTA run through the pieces of
 // the stretch independently, so the loads and the first scores of the next piece overlap the end of this one.  A pair of tiles that CTAs share
 // leaves fp32 sums in scratch slots, joined by a second launch in the order of the line: results do not depend on timing.
 // Every wait is bounded (status word + clean unwind); no load uses cluster multicast.
@@ -17,6 +17,8 @@
 
 namespace ats {
 
+constexpr int PC_CTAS = 148;
+constexpr int PC_PIECE = 192;    // keys that take as long as the first loads and scores and the outputs of a pair of tiles (4 us, a block of 128 keys 2.4 us)
 constexpr int PC_THREADS = 320;  // soft-max A (warps 0-3), soft-max B (4-7), TMA (8), MMA (9)
 
 struct PagedPortionArgs {
@@ -27,11 +29,20 @@ struct PagedPortionArgs {
   int tile;                 // tokens of a tile: 128 / rep
   int ctas;
   int zero_tail;            // tokens behind the last row get zeros
+  int wide;                 // output rows begin at multiples of 32 bytes
   float scale_log2;
-  unsigned long long* line; // [R + 1]: where a row's work begins (all key heads); the end of the line
+  unsigned long long* total;   // the length of the line
+  struct PcPlace* begins;      // [ctas]: where the CTAs' stretches begin
   float* part_o;            // [ctas, 2, 256, D]
   float* part_ml;           // [ctas, 2, 256, 2]
   int* status;
+};
+
+// A place on the line: pair `k` of tiles of (row, key head), which begins at `base`.
+struct PcPlace {
+  int row, hk, k, pad;
+  unsigned long long base, pad2;
+  __device__ __forceinline__ void find(const PagedPortionArgs& p, int r, unsigned long long row_base, unsigned long long x);   // x within row r
 };
 
 template <int D>
@@ -45,8 +56,8 @@ struct PagedPortionSmem {
   static constexpr int TOTAL = BAR_OFF + 512 + 1024;
 };
 
-// The keys that the pairs of tiles 0 .. k - 1 of a row see, each up to its last token (`at` tokens before the portion, `pair` tokens a pair).
-__device__ __forceinline__ unsigned long long pc_before(unsigned long long k, unsigned at, unsigned pair) { return k * at + pair * (k * (k + 1) / 2); }
+// The length of pairs of tiles 0 .. k - 1 of a row, each seeing the keys up to its last token (`at` tokens before the portion, `pair` tokens a pair).
+__device__ __forceinline__ unsigned long long pc_before(unsigned long long k, unsigned at, unsigned pair) { return k * (at + PC_PIECE) + pair * (k * (k + 1) / 2); }
 
 struct PcRow {
   int first, fresh, keys, at, pairs;
@@ -56,11 +67,11 @@ struct PcRow {
     at = max(keys - fresh, 0);
     const int pair = 2 * p.tile;
     pairs = (long long)fresh * p.rep > p.limit ? (fresh + pair - 1) / pair : 0;
-    cost = pairs ? pc_before(pairs - 1, at, pair) + at + fresh : 0;
+    cost = pairs ? pc_before(pairs - 1, at, pair) + PC_PIECE + at + fresh : 0;
   }
 };
 
-// The line shared out: one key more to each of the first `extra` CTAs.  No CTA has less than 256 keys of a pair of tiles to itself.
+// The line shared out: one key more to each of the first `extra` CTAs, and no CTA for less than two blocks.
 struct PcShares {
   unsigned long long n, each, extra;
   __device__ __forceinline__ PcShares(const PagedPortionArgs& p, unsigned long long total) {
@@ -69,31 +80,27 @@ struct PcShares {
     extra = total - each * n;
   }
   __device__ __forceinline__ unsigned long long begin(unsigned long long c) const { return c * each + min(c, extra); }
-  __device__ __forceinline__ unsigned long long owner(unsigned long long x) const {
-    const unsigned long long longer = extra * (each + 1);
-    return x < longer ? x / (each + 1) : extra + (x - longer) / each;
-  }
 };
 
-// A place on the line: pair `k` of tiles of (row, key head), which begins at `base`.
-struct PcPlace {
-  int row, hk, k;
-  unsigned long long base;
-  __device__ __forceinline__ void find(const PagedPortionArgs& p, int r, unsigned long long row_base, unsigned long long x) {   // x within row r
-    const PcRow w(p, r);
-    row = r;
-    hk = int((x - row_base) / w.cost);
-    base = row_base + hk * w.cost;
-    int lo = 0, hi = w.pairs;   // the last pair that begins at or before x
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pc_before(mid, w.at, 2 * p.tile) <= x - base) lo = mid;
-      else hi = mid;
-    }
-    k = lo;
-    base += pc_before(lo, w.at, 2 * p.tile);
+__device__ __forceinline__ void PcPlace::find(const PagedPortionArgs& p, int r, unsigned long long row_base, unsigned long long x) {
+  const PcRow w(p, r);
+  row = r;
+  hk = int((x - row_base) / w.cost);
+  base = row_base + hk * w.cost;
+  int lo = 0, hi = w.pairs;   // the last pair that begins at or before x
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pc_before(mid, w.at, 2 * p.tile) <= x - base) lo = mid;
+    else hi = mid;
   }
-};
+  k = lo;
+  base += pc_before(lo, w.at, 2 * p.tile);
+}
+// The first key block of a pair that begins at `base` behind place x of the line; `blocks` of them from its end on.
+__device__ __forceinline__ int pc_block(unsigned long long base, unsigned long long x, int seen, int blocks) {
+  if (x >= base + PC_PIECE + seen) return blocks;
+  return x > base + PC_PIECE ? int((x - base - PC_PIECE) >> 7) : 0;
+}
 
 // A piece: key blocks [j0, j1) of a pair of tiles.
 struct PcPiece {
@@ -121,11 +128,11 @@ struct PcWalk {
       s.row = at.row; s.hk = at.hk; s.first = w.first; s.fresh = w.fresh; s.keys = w.keys; s.tok0 = at.k * pair;
       s.blocks = (seen + 127) >> 7;
       s.opens = at.base <= lo;
-      s.j0 = at.base < lo ? int((lo - at.base) >> 7) : 0;
-      s.j1 = at.base + seen <= hi ? s.blocks : int((hi - at.base) >> 7);
+      s.j0 = pc_block(at.base, lo, seen, s.blocks);
+      s.j1 = pc_block(at.base, hi, seen, s.blocks);
       s.n[0] = (w.at + min(s.tok0 + p.tile, w.fresh) + 127) >> 7;
       s.n[1] = s.tok0 + p.tile < w.fresh ? s.blocks : 0;
-      at.base += seen;
+      at.base += PC_PIECE + seen;
       if (++at.k == w.pairs) {
         at.k = 0;
         if (++at.hk == p.n_kv) at.hk = 0, ++at.row;
@@ -216,11 +223,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   const unsigned long long lo = shares.begin(blockIdx.x), hi = blockIdx.x < shares.n ? shares.begin(blockIdx.x + 1) : lo;
   for (int r = r0; r < r1; ++r) {
     const unsigned long long n = PcRow(p, r).cost * p.n_kv;
-    if (blockIdx.x == 0) p.line[r] = before;
     if (before <= lo && lo < before + n) s_row = r, s_base = before;
     before += n;
   }
-  if (blockIdx.x == 0 && tid == 0) p.line[rows.R] = total;
+  if (blockIdx.x == 0 && tid == 0) *p.total = total;
   if (p.zero_tail) {
     const int tail = min(max(rows.starts[rows.R], 0), rows.tokens), vecs = p.n_kv * p.rep * (D / 8);
     for (long long i = (long long)blockIdx.x * PC_THREADS + tid; i < (long long)(rows.tokens - tail) * vecs; i += (long long)gridDim.x * PC_THREADS)
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   PcPlace start = {};
   if (lo < hi) start.find(p, s_row, s_base, lo);
   else start.base = hi;
+  if (tid == 0) p.begins[blockIdx.x] = start;
   PcWalk walk(p, start, lo, hi);
   PcPiece s;
   // columns: S_A [0,128)  S_B [128,256)  O_A [256, 256 + D)  O_B [256 + D, 256 + 2 D)
@@ -254,16 +261,6 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         return row;
       };
       int where = look_up(s.j0);
-      if (!(ok = mbar_wait_warp(q_empty, (n_pieces & 1) ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
-      ++n_pieces;
-      if (lane == 0) {
-        const bool a = s.end(0) > s.j0, b = s.end(1) > s.j0;
-        mbar_expect_tx(q_full, (int(a) + int(b)) * p.tile * p.rep * D * 2);
-        for (int x = 0; x < 2; ++x)
-          if (x ? b : a)
-#pragma unroll
-            for (int i = 0; i < DC; ++i) tma_load_3d(sQ + x * T + i * 16384, &map_q, q_full, 64 * i, s.hk * p.rep, s.first + s.tok0 + x * p.tile);
-      }
       for (int j = s.j0; j < s.j1; ++j, ++n_blocks) {
         const int here = where, st = n_blocks % ST;
         const uint32_t ph = (n_blocks / ST) & 1;
@@ -272,6 +269,18 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         if (lane == 0) mbar_expect_tx(&k_full[st], T);
         __syncwarp();
         if (lane < copies) tma_load_3d(sK + st * T + c * 16384 + at * 128, &map_k, &k_full[st], 64 * c, s.hk, here);
+        if (j == s.j0) {   // the queries, once the last piece's scores are done
+          if (!(ok = mbar_wait_warp(q_empty, (n_pieces & 1) ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
+          ++n_pieces;
+          if (lane == 0) {
+            const bool a = s.end(0) > s.j0, b = s.end(1) > s.j0;
+            mbar_expect_tx(q_full, (int(a) + int(b)) * p.tile * p.rep * D * 2);
+            for (int x = 0; x < 2; ++x)
+              if (x ? b : a)
+#pragma unroll
+                for (int i = 0; i < DC; ++i) tma_load_3d(sQ + x * T + i * 16384, &map_q, q_full, 64 * i, s.hk * p.rep, s.first + s.tok0 + x * p.tile);
+          }
+        }
         if (!(ok = mbar_wait_warp(&v_empty[st], ph ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
         const int live = s.keys - j * 128;   // values behind these are whatever earlier generations left in the page
         uint64_t* bar = live < 128 ? v_raw : &v_full[st];
@@ -404,7 +413,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         const float mnew = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2);
         if (j == s.j0) {
           m = mnew;
-        } else if (__any_sync(0xffffffffu, mnew > m + 8.f)) {
+        } else if (__any_sync(0xffffffffu, live && mnew > m + 8.f)) {   // (what lies behind the portion in the tile has no say)
           const float alpha = exp2f(m - mnew);  // the previous P V of this tile has completed: S(j) was computed after it
           m = mnew;
           l *= alpha;
@@ -461,13 +470,20 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
           tmem_ld_wait();
           if (!live) continue;
           if (whole) {
+            uint4 w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float f[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[8 * e + i]) * inv;
-              *reinterpret_cast<uint4*>(orow + c * 32 + e * 8) =
-                  make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+              w[e] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+            }
+            if (p.wide) {   // whole sectors
+              st_global_32B(orow + c * 32, w[0], w[1]);
+              st_global_32B(orow + c * 32 + 16, w[2], w[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(orow + c * 32 + e * 8) = w[e];
             }
           } else {
 #pragma unroll
@@ -488,45 +504,53 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   }
 }
 
-// CTA (c, part): the pair of tiles across the border between stretches c and c + 1, if no earlier border lies in it; 32 of its 256 query rows.
-constexpr int PCJ_THREADS = 256;
+// CTA (c, part): the pair of tiles across the border between stretches c and c + 1, if no earlier border lies in it; 16 of its 256 query rows.
+constexpr int PCJ_THREADS = 256, PCJ_ROWS = 16;
 template <int D>
 __global__ void __launch_bounds__(PCJ_THREADS) paged_portion_join_kernel(const PagedPortionArgs p) {
+  __shared__ int s_slots[PC_CTAS], s_n;
   pdl_prologue();
-  const unsigned long long total = p.line[p.rows.R];
-  const PcShares shares(p, total);
+  const PcShares shares(p, *p.total);
   const unsigned c = blockIdx.x;
   if (c + 1 >= shares.n) return;
-  const unsigned long long x = shares.begin(c + 1);
-  int lo = 0, hi = p.rows.R;   // the last row that begins at or before x (rows without work begin where the next one does)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.line[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  PcPlace at;
-  at.find(p, lo, p.line[lo], x);
-  if (at.base == x || shares.owner(at.base) != c) return;
+  const PcPlace at = p.begins[c + 1];
+  if (at.base == shares.begin(c + 1) || at.base < shares.begin(c)) return;   // no pair across this border, or an earlier one lies in it too
   const PcRow w(p, at.row);
   const int pair = 2 * p.tile, tok0 = at.k * pair, seen = w.at + min(tok0 + pair, w.fresh), blocks = (seen + 127) >> 7;
-  const unsigned long long w1 = shares.owner(at.base + seen - 1);
-  auto from = [&](unsigned long long s) { return shares.begin(s) <= at.base ? 0 : int((shares.begin(s) - at.base) >> 7); };
-  auto to = [&](unsigned long long s) { return shares.begin(s + 1) >= at.base + seen ? blocks : int((shares.begin(s + 1) - at.base) >> 7); };
-  for (unsigned long long s = c; s <= w1; ++s)
-    if (from(s) == 0 && to(s) == blocks) return;   // one of them had all of it
+  if (threadIdx.x < 32) {   // the slots of its pieces, in order
+    int n = 0;
+    for (unsigned s0 = c; s0 < shares.n; s0 += 32) {
+      const unsigned s = s0 + threadIdx.x;
+      const bool in = s < shares.n && shares.begin(s) < at.base + PC_PIECE + seen;
+      int from = 0, to = 0;
+      if (in) {
+        from = pc_block(at.base, shares.begin(s), seen, blocks);
+        to = pc_block(at.base, shares.begin(s + 1), seen, blocks);
+      }
+      const bool piece = from < to, whole = from == 0 && to == blocks;   // (whole: a CTA has finished the pair)
+      const unsigned mask = __ballot_sync(0xffffffffu, piece);
+      if (piece) s_slots[n + __popc(mask & ((1u << threadIdx.x) - 1))] = 2 * int(s) + (at.base <= shares.begin(s) ? 0 : 1);
+      n = __any_sync(0xffffffffu, whole) ? -1 : n + __popc(mask);
+      if (n < 0 || !__all_sync(0xffffffffu, in)) break;
+    }
+    if (threadIdx.x == 0) s_n = n;
+  }
+  __syncthreads();
+  const int n = s_n;
   constexpr int LANES = D / 4;
-  for (int i = threadIdx.x; i < 32 * LANES; i += PCJ_THREADS) {
-    const int q = blockIdx.y * 32 + i / LANES, lane = i % LANES, tile = q >> 7, r = q & 127;
+#pragma unroll
+  for (int i = threadIdx.x; i < PCJ_ROWS * LANES; i += PCJ_THREADS) {
+    const int q = blockIdx.y * PCJ_ROWS + i / LANES, lane = i % LANES, tile = q >> 7, r = q & 127;
     const int my_tok = r / p.rep, head = r - my_tok * p.rep, tok = tok0 + tile * p.tile + my_tok;
-    if (my_tok >= p.tile || tok >= w.fresh) continue;
+    if (n < 1 || my_tok >= p.tile || tok >= w.fresh) continue;
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (unsigned long long s = c; s <= w1; ++s) {
-      if (from(s) >= to(s)) continue;
-      const long long slot = (long long)(2 * s + (at.base <= shares.begin(s) ? 0 : 1)) * 256 + q;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const long long slot = (long long)s_slots[x] * 256 + q;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-      if (ml.x == -INFINITY) continue;   // the tile saw no keys of that piece
       const float4 v = reinterpret_cast<const float4*>(p.part_o + slot * D)[lane];
+      if (ml.x == -INFINITY) continue;   // the tile saw no keys of that piece: its sums were not written
       const float top = fmaxf(m, ml.x), keep = exp2f(m - top), f = exp2f(ml.x - top);
       m = top;
       l = l * keep + ml.y * f;
@@ -544,19 +568,17 @@ static int launch_paged_portion(const CUtensorMap& mq, const CUtensorMap& mk, co
   static_assert(SM::TOTAL <= 227 * 1024, "does not fit an SM");
   cudaError_t ce = cudaFuncSetAttribute(paged_portion_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
   if (ce == cudaSuccess) ce = launch_pdl(paged_portion_kernel<D>, dim3(p.ctas), dim3(PC_THREADS), SM::TOTAL, s, mq, mk, mv, p);
-  if (ce == cudaSuccess && p.ctas > 1) ce = launch_pdl(paged_portion_join_kernel<D>, dim3(p.ctas - 1, 8), dim3(PCJ_THREADS), 0, s, p);
+  if (ce == cudaSuccess && p.ctas > 1) ce = launch_pdl(paged_portion_join_kernel<D>, dim3(p.ctas - 1, 256 / PCJ_ROWS), dim3(PCJ_THREADS), 0, s, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }
-
-constexpr int PC_CTAS = 148;
 
 }  // namespace ats
 
 using namespace ats;
 
 // Bytes of scratch that `ats_paged_portion` needs (32-byte aligned).
-ATS_API long long ats_paged_portion_scratch(int R, int D) { return (R + 4ll) / 4 * 32 + 2ll * PC_CTAS * 256 * (D + 2) * 4; }
+ATS_API long long ats_paged_portion_scratch(int D) { return 32 + PC_CTAS * (long long)sizeof(PcPlace) + 2ll * PC_CTAS * 256 * (D + 2) * 4; }
 
 // Rows whose new tokens times n_q / n_kv are more than `limit`.  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens (a power of
 // two) or more, up to 128 query heads a group.  zero_tail: tokens behind the last row get zeros.
@@ -574,10 +596,12 @@ ATS_API int ats_paged_portion(const void* q, long long ldq, const void* k_pages,
   PagedPortionArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.tile = 128 / p.rep; p.ctas = PC_CTAS; p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.tile = 128 / p.rep; p.ctas = PC_CTAS; p.zero_tail = zero_tail; p.wide = !(reinterpret_cast<uintptr_t>(out) & 31) && !(ldo & 15);
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
-  p.line = static_cast<unsigned long long*>(scratch);
-  p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);   // 32-byte stores
+  static_assert(sizeof(PcPlace) % 32 == 0, "the sums are written 32 bytes at a time");
+  p.total = static_cast<unsigned long long*>(scratch);
+  p.begins = reinterpret_cast<PcPlace*>(p.total + 4);
+  p.part_o = reinterpret_cast<float*>(p.begins + PC_CTAS);
   p.part_ml = p.part_o + 2ll * PC_CTAS * 256 * D;
   CUtensorMap mq, mk, mv;
   int e;
