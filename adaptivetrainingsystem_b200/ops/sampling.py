@@ -90,7 +90,7 @@ def sample_rows_reference(logits: torch.Tensor, uniform: torch.Tensor, temperatu
     greedy = ~(t > 0) | torch.isinf(top) & (top < 0)
     order = x.argsort(dim=-1, descending=True, stable=True)
     gap = torch.where(x.double() == top, 0.0, x.double() - top)
-    w = (gap / torch.where(greedy, 1.0, t.double())).exp().gather(1, order)
+    w = torch.where(torch.isinf(gap), gap, gap / torch.where(greedy, 1.0, t.double())).exp().gather(1, order)
     k = column(top_k, torch.int64)
     w = torch.where(torch.arange(V, device=x.device)[None] < torch.where(k > 0, k, V), w, 0.0)
     before = w.cumsum(-1) - w

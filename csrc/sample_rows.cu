@@ -35,6 +35,7 @@ constexpr int SR_BINS = 4096;          // the last one: no mass
 constexpr float SR_RANGE = 30.5f;      // in units of T: exp(-30.49) 2^42 rounds to nothing
 constexpr int SR_LIST = 2048;
 constexpr int SR_MAX_K = 1024;
+constexpr int SR_FEW = SR_THREADS / 2;
 constexpr int SR_CHUNK = 256;
 constexpr int SR_MAX_CLUSTER = 8;
 
@@ -61,7 +62,7 @@ template <typename T>
 struct SampleRowsSmem {   // byte offsets of the dynamic shared memory
   int hist, list, chunks, seen, raw, total;
   __host__ __device__ SampleRowsSmem(int slice, bool cached) {
-    hist = 0;                            // u32 [SR_BINS]; later u64 [SR_LIST]: this CTA's tokens of the bracket, or masses of the list
+    hist = 0;                            // u32 [SR_BINS]; later u64 [SR_LIST]: this CTA's tokens of the bracket
     list = hist + SR_BINS * 4;           // u64 [SR_LIST]: the cluster's tokens of the bracket (rank 0); before that the cluster's counts
     chunks = list + SR_LIST * 8;         // u64 [slice / SR_CHUNK]
     seen = chunks + slice / SR_CHUNK * 8;        // one bit per token of the slice
@@ -132,10 +133,11 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-// exp(-w) for w >= 0: w = n ln 2 / 32 - z, |z| <= ln 2 / 64; exp(z) by its Taylor series to the fifth power (the next term is below 2^-48), 2^-(n mod 32)/32
+// exp(-w) for w >= 0 (from 44 on, and for NaN, exp(-44): no mass): w = n ln 2 / 32 - z, |z| <= ln 2 / 64; exp(z) by its Taylor series to the fifth power (the next term is below 2^-48), 2^-(n mod 32)/32
 // from a table.
 __device__ __forceinline__ double sr_exp_neg(double w, const double* table) {
   constexpr double magic = 6755399441055744.0;   // 1.5 * 2^52
+  w = __hiloint2double(int(min(uint32_t(__double2hiint(w)), 0x40460000u)), __double2loint(w));   // (the upper half of 44.0)
   const double t = fma(w, 32 * 1.4426950408889634074, magic);
   const int n = __double2loint(t);
   const double z = fma(t - magic, 0.69314718055994530942 / 32, -w);
@@ -153,14 +155,13 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   extern __shared__ __align__(16) uint8_t sr_smem[];
   __shared__ uint64_t red[SR_WARPS], s_top, s_sum[2], s_cut;
   __shared__ double red_d[SR_WARPS], s_table[32];
-  __shared__ uint32_t red_u[SR_WARPS], s_count, s_found;   // tokens of the bracket: this CTA's, the cluster's (rank 0)
+  __shared__ uint32_t red_u[SR_WARPS], s_count, s_found, s_base;   // tokens of the bracket: this CTA's, the cluster's (rank 0), in front of this CTA's
   __shared__ int s_bracket[3];
   constexpr int PER = 16 / sizeof(T);
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, groups = p.slice / 8;
   const SampleRowsSmem<T> at(p.slice, p.cached);
   uint32_t* hist = reinterpret_cast<uint32_t*>(sr_smem + at.hist);
   uint64_t* near = reinterpret_cast<uint64_t*>(sr_smem + at.hist);
-  uint64_t* masses = near;
   uint64_t* list = reinterpret_cast<uint64_t*>(sr_smem + at.list);
   uint32_t* counts = reinterpret_cast<uint32_t*>(sr_smem + at.list);
   uint64_t* chunks = reinterpret_cast<uint64_t*>(sr_smem + at.chunks);
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     }
     __syncthreads();
   }
+  bool infinite = false;   // the largest score is +infinity: such tokens count as 0, all others as -infinity
   auto load8 = [&](int g, float (&x)[8]) {   // the scores of the slice's tokens 8 g ..
     uint4 w[8 / PER];
 #pragma unroll
@@ -226,6 +228,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
         for (int e = 0; e < 8; ++e)
           if (bits >> e & 1) x[e] = x[e] > 0.f ? __fdiv_rn(x[e], pen) : __fmul_rn(x[e], pen);
       }
+    }
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
     }
   };
   auto key_of = [&](float x, int j) -> uint64_t { return (uint64_t(order_key(x + 0.f)) << 32) | (0xffffffffu - uint32_t(i0 + j)); };
@@ -261,7 +267,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     top = k > top ? k : top;
   }
   const int arg = top ? int(0xffffffffu - uint32_t(top)) : 0;   // (0: nothing above -infinity)
-  const float x_max = key_value(uint32_t(top >> 32));
+  float x_max = key_value(uint32_t(top >> 32));
+  if (x_max == INFINITY) infinite = true, x_max = 0.f, top = (uint64_t(order_key(0.f)) << 32) | uint32_t(top);
 
   const double inv_t = 1.0 / double(temp), x_top = double(x_max);
   const float per_bin = float(SR_BINS - 1) / (SR_RANGE * temp);
@@ -269,15 +276,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     const float d = x == x_max ? 0.f : (x_max - x) * per_bin;
     return int(fminf(d, float(SR_BINS - 1)));
   };
-  // relative to the first token's; the last bin's (which has none) as that of its border
-  auto weight = [&](float x, int bin) -> double { return sr_exp_neg(x == x_max || bin == SR_BINS - 1 ? 0.0 : (x_top - double(x)) * inv_t, s_table); };
+  auto weight = [&](float x) -> double { return sr_exp_neg((x_top - double(x)) * inv_t, s_table); };   // relative to the first token's
   auto fixed = [&](double w) -> uint64_t {   // round(w * 2^42)
     return uint64_t(__double_as_longlong(fma(w, double(1ll << SR_MASS_BITS), 4503599627370496.0))) & ((1ull << 52) - 1);
   };
-  auto mass = [&](float x) -> uint64_t {
-    const int bin = bin_of(x);
-    return bin == SR_BINS - 1 ? 0 : fixed(weight(x, bin));
-  };
+  auto mass = [&](float x) -> uint64_t { return bin_of(x) == SR_BINS - 1 ? 0 : fixed(weight(x)); };
   auto cluster_sum = [&](uint64_t v, int slot) -> uint64_t {   // (one barrier; the slots take turns)
     const uint64_t mine = sr_block_sum(v, red);
     if (tid == 0) s_sum[slot] = mine;
@@ -291,17 +294,32 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     const double want = u * double(total);
     return want < double(total) ? min(uint64_t(want), total - 1) : total - 1;
   };
-  auto collect = [&](float x, int j, bool mine_too) {   // into rank 0's list, and this CTA's own
-    const uint64_t k = key_of(x, j);
-    uint32_t i;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(i) : "r"(mapa_shared(smem_u32(&s_found), 0)) : "memory");
-    if (i < SR_LIST) sr_st_u64(&list[i], 0, k);
-    if (mine_too) {
-      i = atomicAdd(&s_count, 1u);
-      if (i < SR_LIST) near[i] = k;
-    }
+  // The bracket's tokens: each CTA notes its own (`stage`, room for `room`), then hand_over() puts them into rank 0's list and returns how many there are
+  // in all (more than SR_LIST: some did not fit).
+  uint64_t* stage = near;
+  uint32_t room = SR_LIST;
+  auto collect = [&](float x, int j) {
+    const uint32_t i = atomicAdd(&s_count, 1u);
+    if (i < room) stage[i] = key_of(x, j);
   };
-  // what is kept, per SR_CHUNK consecutive tokens (one group a lane): `kept(x, bin, j)` says whether the token is, as far as its mass does not.  -> the mass
+  auto hand_over = [&]() -> uint32_t {
+    __syncthreads();
+    const uint32_t n = s_count;
+    if (tid == 0) {
+      uint32_t at;
+      asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(mapa_shared(smem_u32(&s_found), 0)), "r"(n > room ? SR_LIST + 1 : n) : "memory");
+      s_base = at;
+    }
+    __syncthreads();
+    const uint32_t base = s_base;
+    if (n <= room && base + n <= SR_LIST)
+      for (uint32_t i = tid; i < n; i += SR_THREADS) sr_st_u64(&list[base + i], 0, stage[i]);
+    csync();
+    const uint32_t found = sr_ld_u32(&s_found, 0);
+    csync();   // everybody has read: a list that holds all that is kept needs no other CTA any more
+    return found;
+  };
+  // what is kept, per SR_CHUNK consecutive tokens (one group a lane): `kept(x, j)` says whether the token is, as far as its mass does not.  -> the mass
   // of these before min-p, this thread's share
   auto sum_chunks = [&](auto kept, bool add) -> uint64_t {   // (add: to the sums that are there)
     uint64_t all = 0;
@@ -309,14 +327,21 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       float x[8];
       load8(g, x);
       uint64_t v = 0;
+      if (low > 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int bin = bin_of(x[e]);
-        const bool in = kept(x[e], bin, 8 * g + e);
-        const double w = weight(x[e], bin);
-        const uint64_t m = in ? fixed(w) : 0;
-        all += m;
-        v += w >= low ? m : 0;
+        for (int e = 0; e < 8; ++e) {
+          const double w = weight(x[e]);
+          const uint64_t m = kept(x[e], 8 * g + e) ? fixed(w) : 0;
+          all += m;
+          v += w >= low ? m : 0;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t m = fixed(weight(x[e]));
+          v += kept(x[e], 8 * g + e) ? m : 0;
+        }
+        all += v;
       }
       v = sr_warp_sum(v);
       if (lane == 0) chunks[g >> 5] = add ? chunks[g >> 5] + v : v;
@@ -336,72 +361,158 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   uint64_t cut = 0, z = 0, above = 0;   // tokens with at least the key `cut` are kept
   // rank 0, with `found` tokens in the list, `above` the mass of what is in front of them: the cut, and the answer if nothing is in front of them
   auto finish_list = [&](uint32_t found) {
-    auto sort = [&](uint32_t m) {   // the list's first m entries, largest first (bitonic, padded with zeros)
-      uint32_t size = 1;
-      while (size < m) size *= 2;
-      for (uint32_t i = m + tid; i < size; i += SR_THREADS) list[i] = 0;
+    if (found <= SR_FEW) {
+      // Few tokens: two threads compare one with all others, half of them each, twice: by score for the cuts, by index for the draw.
+      uint64_t* few = list + SR_FEW;   // masses of the list's tokens; behind them the other half's sums
+      const int i = tid % SR_FEW, half = tid / SR_FEW, mid = int(found + 1) / 2, from = half ? mid : 0, to = half ? int(found) : mid;
+      const bool mine = i < int(found);
+      const uint64_t k = mine ? list[i] : 0;
+      const float x = key_value(uint32_t(k >> 32));
+      uint64_t m = mine ? mass(x) : 0;
       __syncthreads();
-      for (uint32_t k = 2; k <= size; k *= 2)
-        for (uint32_t j = k / 2; j > 0; j /= 2) {
-          for (uint32_t i = tid; i < size / 2; i += SR_THREADS) {
-            const uint32_t a = 2 * i - (i & (j - 1)), c = a + j;
-            const uint64_t va = list[a], vc = list[c];
-            if ((va < vc) == ((a & k) == 0)) list[a] = vc, list[c] = va;
-          }
-          __syncthreads();
+      if (half == 0) few[i] = m;
+      __syncthreads();
+      uint64_t before = 0;
+      uint32_t rank_of = 0;
+      if (mine)
+        for (int j = from; j < to; ++j) {
+          const bool in_front = list[j] > k;
+          before += in_front ? few[j] : 0;
+          rank_of += in_front;
         }
-    };
-    sort(found);
-    // masses and their prefix: SR_LIST / SR_THREADS consecutive tokens a thread
-    constexpr int EACH = SR_LIST / SR_THREADS;
-    const uint32_t m = by_k ? min(found, uint32_t(top_k)) : found;
-    uint64_t v[EACH], own = 0;
+      if (half) few[SR_FEW + i] = before, few[2 * SR_FEW + i] = rank_of;
+      __syncthreads();
+      before += few[SR_FEW + i] + above;
+      rank_of += uint32_t(few[2 * SR_FEW + i]);
+      const bool first_k = half == 0 && mine && (!by_k || rank_of < uint32_t(top_k));
+      const uint64_t all = by_k ? sr_block_sum(first_k ? m : 0, red) : z;
+      const bool in = first_k && (!by_p || double(before) <= double(fmaxf(top_p, 0.f)) * double(all));   // (both rules keep a leading run)
+      if (!in || (low > 0 && !(weight(x) >= low))) m = 0;
+      if (!listed) {   // the smallest key that is kept
+        uint64_t last = in ? k : ~0ull;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const uint32_t i = tid * EACH + e;
-      v[e] = i < m ? mass(key_value(uint32_t(list[i] >> 32))) : 0;
-      own += v[e];
-    }
-    uint64_t all, run = sr_block_scan<uint64_t>(own, red, &all) + above;
-    const double limit = by_p ? double(fmaxf(top_p, 0.f)) * double(by_k ? all : z) : INFINITY;
-    uint32_t kept = 0, n_kept;
-    own = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const uint32_t i = tid * EACH + e;
-      if (i < m) {
-        // both rules keep a leading run; a token without mass is never the answer
-        const bool in = double(run) <= limit;
-        kept += in;
-        run += in ? v[e] : 0;
-        const float x = key_value(uint32_t(list[i] >> 32));
-        if (!in || !(weight(x, bin_of(x)) >= low)) v[e] = 0;
-        own += v[e];
-        if (listed) masses[i] = v[e];
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, last, o);
+          last = other < last ? other : last;
+        }
+        __syncthreads();
+        if (lane == 0) red[warp] = last;
+        __syncthreads();
+        if (tid == 0) {
+          for (int w = 1; w < SR_WARPS; ++w) last = red[w] < last ? red[w] : last;
+          s_cut = last;
+        }
+        return;
       }
-    }
-    sr_block_scan<uint32_t>(kept, red_u, &n_kept);
-    if (!listed) {
-      if (tid == 0) s_cut = n_kept > 0 ? list[n_kept - 1] : ~0ull;
+      const uint64_t target = target_of(sr_block_sum(half == 0 ? m : 0, red));
+      if (half == 0) few[i] = m;
+      __syncthreads();
+      before = 0;
+      if (mine)
+        for (int j = from; j < to; ++j) before += uint32_t(list[j]) > uint32_t(k) ? few[j] : 0;   // (the lower half falls as the index grows)
+      if (half) few[SR_FEW + i] = before;
+      __syncthreads();
+      before += few[SR_FEW + i];
+      if (half == 0 && before <= target && target < before + m) p.out[b] = int(0xffffffffu - uint32_t(k));
       return;
     }
-    // all that is kept is here: in index order, the token whose mass covers the target
-    const uint64_t target = target_of(sr_block_sum(own, red));
-    for (uint32_t i = tid; i < n_kept; i += SR_THREADS) list[i] = (list[i] << 32) | i;   // (what was the low half falls as the index grows)
-    __syncthreads();
-    sort(n_kept);
+    constexpr int EACH = SR_LIST / SR_THREADS;   // four consecutive entries a thread
+    uint64_t v[EACH];
+    auto scan = [&](uint64_t mine, uint64_t* all) -> uint64_t { return sr_block_scan<uint64_t>(mine, red, all); };
+    // The entries of all threads, largest first (bitonic; `m` of them are not zero): pairs that lie in a thread or in a warp are exchanged in registers.
+    auto sort = [&](uint32_t m) {
+      uint32_t size = 2;
+      while (size < m) size *= 2;
+      for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+          if (j >= 32 * EACH) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) list[tid * EACH + e] = v[e];
+            __syncthreads();
+          }
+          if (warp * 32 * EACH >= size) continue;   // (nothing but zeros)
+          if (j >= EACH) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+              const uint32_t i = tid * EACH + e;
+              const uint64_t o = j >= 32 * EACH ? list[i ^ j] : __shfl_xor_sync(0xffffffffu, v[e], j / EACH);
+              const bool larger = ((i & k) == 0) == ((i & j) == 0);   // this place keeps the larger one
+              v[e] = (v[e] > o) == larger ? v[e] : o;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+              const int f = e ^ int(j);
+              if (f > e) {
+                const bool desc = ((tid * EACH + e) & k) == 0;
+                const uint64_t x = v[e], y = j == 1 ? v[e ^ 1] : v[e ^ 2];
+                const bool swap = (x < y) == desc;
+                v[e] = swap ? y : x;
+                if (j == 1) v[e ^ 1] = swap ? x : y;
+                else v[e ^ 2] = swap ? x : y;
+              }
+            }
+          }
+        }
+    };
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) v[e] = tid * EACH + e < found ? list[tid * EACH + e] : 0;
+    sort(found);
+    const uint32_t m = by_k ? min(found, uint32_t(top_k)) : found;
+    uint64_t w[EACH], own = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      w[e] = tid * EACH + e < m ? mass(key_value(uint32_t(v[e] >> 32))) : 0;
+      own += w[e];
+    }
+    uint64_t all, run = scan(own, &all) + above;
+    const double limit = by_p ? double(fmaxf(top_p, 0.f)) * double(by_k ? all : z) : INFINITY;
+    uint64_t last = ~0ull;
     own = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const uint32_t i = tid * EACH + e;
-      v[e] = i < n_kept ? masses[uint32_t(list[i])] : 0;
-      own += v[e];
+      // both rules keep a leading run; a token without mass is never the answer
+      if (tid * EACH + e >= m) break;
+      const bool in = double(run) <= limit;
+      run += in ? w[e] : 0;
+      if (in) last = v[e];
+      if (!in || (low > 0 && !(weight(key_value(uint32_t(v[e] >> 32))) >= low))) w[e] = 0;
+      own += w[e];
     }
-    run = sr_block_scan<uint64_t>(own, red, &all);
+    if (!listed) {   // the smallest key that is kept
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t u2 = __shfl_xor_sync(0xffffffffu, last, o);
+        last = u2 < last ? u2 : last;
+      }
+      __syncthreads();
+      if (lane == 0) red[warp] = last;
+      __syncthreads();
+      if (tid == 0) {
+        for (int i = 1; i < SR_WARPS; ++i) last = red[i] < last ? red[i] : last;
+        s_cut = last;
+      }
+      return;
+    }
+    // all that is kept is here: in index order (the index in the upper bits, inverted, the mass in the lower 43), the token whose mass covers the target
+    uint64_t kept;
+    scan(own, &kept);
+    const uint64_t target = target_of(kept);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) v[e] = w[e] ? (uint64_t(uint32_t(v[e]) & (SR_MAX_VOCAB - 1)) << (SR_MASS_BITS + 1)) | w[e] : 0;
+    sort(m);
+    own = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      if (run <= target && target < run + v[e]) p.out[b] = int(0xffffffffu - uint32_t(list[tid * EACH + e] >> 32));
-      run += v[e];
+      w[e] = v[e] & ((2ull << SR_MASS_BITS) - 1);
+      own += w[e];
+    }
+    run = scan(own, &all);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (run <= target && target < run + w[e]) p.out[b] = (SR_MAX_VOCAB - 1) - int(v[e] >> (SR_MASS_BITS + 1));
+      run += w[e];
     }
   };
 
@@ -426,18 +537,27 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     if (before < uint32_t(top_k) && before + c >= uint32_t(top_k)) s_bracket[1] = min((tid + 1) * WIDE - 1, SR_BINS - 2);
     __syncthreads();
     const int b_hi = s_bracket[1];
+    stage = near + SR_THREADS / 2;   // (behind the counts, which the other CTAs may still read)
+    room = SR_LIST - SR_THREADS / 2;
     for (int g = tid; g < groups; g += SR_THREADS) {
       float x[8];
       load8(g, x);
+      float m = x[0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e, false);
+      for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
+      if (bin_of(m) <= b_hi) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e);
+      }
     }
-    csync();
-    const uint32_t found = sr_ld_u32(&s_found, 0);
+    const uint32_t found = hand_over();
     bisect = found > SR_LIST;
     listed = !bisect;
-    if (listed && rank == 0) finish_list(found);
+    if (listed) {
+      if (rank == 0) finish_list(found);
+      return;
+    }
   } else if (by_p && !bisect) {
     // ---- counts of all tokens, and the masses' sum
     uint64_t v = 0;
@@ -447,11 +567,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int bin = bin_of(x[e]);
-        const uint64_t m = fixed(weight(x[e], bin));
-        if (bin < SR_BINS - 1) {
-          atomicAdd(&hist[bin], 1u);
-          v += m;
-        }
+        v += fixed(weight(x[e]));   // (nothing in the last bin)
+        if (bin < SR_BINS - 1) atomicAdd(&hist[bin], 1u);
       }
     }
     z = cluster_sum(v, 0);
@@ -469,48 +586,48 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       if (rank == 0) {
         constexpr int EACH = SR_BINS / SR_THREADS;
         if (tid == 0) s_bracket[0] = done, s_bracket[1] = SR_BINS - 2;
-        __syncthreads();
         // bounds of the cumulative mass through each bin, in units of the largest mass: a bin's tokens lie within a hundredth of a bin of it, a
         // mass is rounded by 2^-43, and the sums here by less than a part in 10^9
-        const double unit = 1.0 / double(1ll << SR_MASS_BITS), width = double(SR_RANGE) / (SR_BINS - 1), limit = double(fmaxf(top_p, 0.f)) * double(z) * unit;
-        auto most_of = [&](int i, double c) { return c * (sr_exp_neg(fmax(width * (i - 0.02), 0.0), s_table) * (1 + 2e-4 * (i == 0)) + unit); };
-        auto least_of = [&](int i, double c) { return c * fmax(sr_exp_neg(width * (i + 1.02), s_table) - unit, 0.0); };
-        double own_most = 0, own_least = 0;
+        constexpr double width = double(SR_RANGE) / (SR_BINS - 1), unit = 1.0 / double(1ll << SR_MASS_BITS);
+        constexpr double down = 1.0 - width * (1.0 - width / 2 * (1.0 - width / 3 * (1.0 - width / 4)));   // exp(-width), to 2^-44
+        constexpr double wide = 1.0 + 0.021 * width, near_end = 1.0 - 1.021 * width;                       // beyond exp(0.02 width), exp(-1.02 width)
+        const double limit = double(fmaxf(top_p, 0.f)) * double(z) * unit;
+        double most[EACH], least[EACH], own_most = 0, own_least = 0, f = sr_exp_neg(width * (tid * EACH), s_table);
         uint32_t c[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           const int i = tid * EACH + e;
           c[e] = i < SR_BINS - 1 ? counts[i] : 0;
-          own_most += i >= done ? most_of(i, c[e]) : 0;
-          own_least += i >= done ? least_of(i, c[e]) : 0;
+          const double n = i >= done ? double(c[e]) : 0.0;
+          most[e] = n * (f * wide + unit);
+          least[e] = n * fmax(f * near_end - unit, 0.0);
+          own_most += most[e];
+          own_least += least[e];
+          f *= down;
         }
-        double all;
-        double run_most = sr_block_scan<double>(own_most, red_d, &all) + double(above) * unit;
+        double all, run_most = sr_block_scan<double>(own_most, red_d, &all) + double(above) * unit;
         double run_least = sr_block_scan<double>(own_least, red_d, &all) + double(above) * unit;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           const int i = tid * EACH + e;
-          if (i < done) continue;
-          const double next_most = run_most + most_of(i, c[e]), next_least = run_least + least_of(i, c[e]);
-          if (run_most * (1 + 1e-9) <= limit && next_most * (1 + 1e-9) > limit) s_bracket[0] = i;
-          if (run_least * (1 - 1e-9) <= limit && next_least * (1 - 1e-9) > limit) s_bracket[1] = i;
-          run_most = next_most, run_least = next_least;
+          if (run_most * (1 + 1e-9) <= limit && (run_most + most[e]) * (1 + 1e-9) > limit) s_bracket[0] = i;
+          if (run_least * (1 - 1e-9) <= limit && (run_least + least[e]) * (1 - 1e-9) > limit) s_bracket[1] = i;
+          run_most += most[e], run_least += least[e];
         }
         __syncthreads();
         // does the bracket fit the list, or even all tokens down to its end?
         const int from = s_bracket[0], to = s_bracket[1];
-        uint32_t upto = 0, in = 0, n_upto, n_in;
+        uint64_t both = 0;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           const int i = tid * EACH + e;
-          upto += i <= to ? c[e] : 0;
-          in += i >= from && i <= to ? c[e] : 0;
+          both += i <= to ? uint64_t(c[e]) << 32 | (i >= from ? c[e] : 0u) : 0;
         }
-        sr_block_scan<uint32_t>(upto, red_u, &n_upto);
-        sr_block_scan<uint32_t>(in, red_u, &n_in);
+        both = sr_block_sum(both, red);
+        const uint32_t n_upto = uint32_t(both >> 32), n_in = uint32_t(both);
         if (tid == 0) {
-          if (done == 0 && n_upto <= SR_LIST) s_bracket[0] = 0;
-          s_bracket[2] = n_in <= SR_LIST || from == done || round == 4;   // (the last two: it gets no narrower)
+          if (done == 0 && n_upto <= SR_LIST / 4) s_bracket[0] = 0;
+          s_bracket[2] = n_in <= SR_LIST / 2 || from == done || round == 4;   // (the last two: it gets no narrower)
         }
       }
       csync();
@@ -521,8 +638,9 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       // sum what is above the bracket, collect its tokens once it is the last
       uint64_t more = 0;
       if (b_lo > 0)
-        more = sum_chunks([&](float x, int bin, int j) -> bool {
-          if (last && bin >= b_lo && bin <= b_hi) collect(x, j, true);
+        more = sum_chunks([&](float x, int j) -> bool {
+          const int bin = bin_of(x);
+          if (last && bin >= b_lo && bin <= b_hi) collect(x, j);
           return bin >= done && bin < b_lo;
         }, done > 0);
       else
@@ -531,30 +649,32 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
           load8(g, x);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e, false);
+            if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e);
         }
       above += cluster_sum(more, (round & 1) ^ 1);
       done = b_lo;
     }
-    const uint32_t found = sr_ld_u32(&s_found, 0);
+    const uint32_t found = hand_over();
     bisect = found > SR_LIST;
     listed = !bisect && b_lo == 0;
+    if (listed) {
+      if (rank == 0) finish_list(found);
+      return;
+    }
     if (!bisect) {
       if (rank == 0) finish_list(found);
-      if (!listed) {
-        csync();
-        cut = sr_ld_u64(&s_cut, 0);
-        for (uint32_t i = tid; i < s_count; i += SR_THREADS)   // the bracket's part of what is kept
-          if (near[i] >= cut) {
-            const float x = key_value(uint32_t(near[i] >> 32));
-            const double w = weight(x, bin_of(x));
-            if (w >= low) atomicAdd(reinterpret_cast<unsigned long long*>(&chunks[(int(0xffffffffu - uint32_t(near[i])) - i0) / SR_CHUNK]), (unsigned long long)fixed(w));
-          }
-        __syncthreads();
-      }
+      csync();
+      cut = sr_ld_u64(&s_cut, 0);
+      for (uint32_t i = tid; i < s_count; i += SR_THREADS)   // the bracket's part of what is kept
+        if (near[i] >= cut) {
+          const float x = key_value(uint32_t(near[i] >> 32));
+          const double w = weight(x);
+          if (w >= low) atomicAdd(reinterpret_cast<unsigned long long*>(&chunks[(int(0xffffffffu - uint32_t(near[i])) - i0) / SR_CHUNK]), (unsigned long long)fixed(w));
+        }
+      __syncthreads();
     }
   }
-  if (!listed) {
+  {
     const bool chunked = !bisect && by_p;   // the chunks hold what is kept
     int slot = 0;
     if (bisect) {
@@ -593,8 +713,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
         cut = lo;
       }
     }
-    auto is_kept = [&](float x, int bin, int j) -> bool { return bin < SR_BINS - 1 && ((chunked && bin < b_lo) || key_of(x, j) >= cut); };
-    if (!chunked) sum_chunks(is_kept, false);
+    const bool cuts = bisect || chunked;
+    auto is_kept = [&](float x, int j) -> bool { return !cuts || (chunked && bin_of(x) < b_lo) || key_of(x, j) >= cut; };
+    if (!cuts) sum_chunks([](float, int) { return true; }, false);
+    else if (bisect) sum_chunks(is_kept, false);
     uint64_t mine = 0;
     for (int c = tid; c < p.slice / SR_CHUNK; c += SR_THREADS) mine += chunks[c];
     // (the sums of the CTAs one by one: where the target lies)
@@ -636,9 +758,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
         uint64_t m[8], sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int bin = bin_of(x[e]);
-          const double wt = weight(x[e], bin);
-          m[e] = is_kept(x[e], bin, 8 * g + e) && wt >= low ? fixed(wt) : 0;
+          const double wt = weight(x[e]);
+          m[e] = is_kept(x[e], 8 * g + e) && wt >= low ? fixed(wt) : 0;
           sum += m[e];
         }
         if (step(sum, &w)) {

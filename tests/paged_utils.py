@@ -69,7 +69,8 @@ def sample64(logits, u, temperature, top_k, top_p, min_p, penalty, history):
         value, token = torch.sort(x.double(), descending=True, stable=True)
         if top_k[r] > 0:
             value, token = value[:int(top_k[r])], token[:int(top_k[r])]
-        mass = torch.where(value == value[0], 0.0, (value - value[0]) / float(temperature[r])).exp()
+        gap = torch.where(value == value[0], 0.0, value - value[0])
+        mass = torch.where(torch.isinf(gap), gap, gap / float(temperature[r])).exp()      # (an infinite gap is one at an infinite temperature too)
         ahead = mass.cumsum(0) - mass
         keep = (ahead <= max(float(top_p[r]), 0.0) * mass.sum()) & (mass >= min(float(min_p[r]), 1.0))
         mass, token = mass[keep], token[keep]

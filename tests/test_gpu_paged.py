@@ -316,6 +316,23 @@ def test_sample_rows_numbers_strides_and_repeats():
     assert a.tolist() == [int(top[0, 0]), int(top[1, -1]), int(top[2, -1]), int(top[3, 0])]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sample_rows_extreme_numbers(dtype):
+    """Temperatures from next to nothing to infinite, cuts of every size, infinite scores, tokens named in the history over and over."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    temps = [1e-38, 1e-8, 1e-4, 0.02, 1.0, 300.0, 1e9, 1e30, float("inf"), float("nan"), -1.0]
+    B, V = 8 * len(temps), 30011
+    x = (3 * torch.randn(B, V, generator=g, device="cuda")).to(dtype)
+    x[::7, 50:60] = float("inf")
+    x[1::7, ::2] = float("-inf")
+    x[2::7, 1::2] = float("nan")
+    x[3::7] += 1000
+    pick = lambda vals, t: torch.tensor([vals[i % len(vals)] for i in range(B)], dtype=t, device="cuda")  # noqa: E731
+    numbers = (pick(temps, torch.float32), pick([0, 0, 7, 1024, 1025, 30010, -5, 300], torch.int32), pick([1.0, 0.6, 2.0, -1.0, 0.9999], torch.float32),
+               pick([0.0, 1e-3, 2.0, -1.0, 0.3, 1e-30], torch.float32), pick([1.0, 1.5], torch.float32))
+    _sample_case(B, V, dtype, 11, numbers=numbers, scores=x)
+
+
 def test_sample_rows_draws_by_mass():
     """20,000 evenly spaced numbers over ten tokens: every token is named as often as its probability says, but for one at either border."""
     n = 20000
