@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -53,8 +54,17 @@ def _fn(name: str):
     return f
 
 
+@functools.lru_cache(maxsize=1024)
+def _scratch(name: str, *sizes: int) -> int:
+    return _fn(name)(*sizes)
+
+
 def _p(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _here = contextlib.nullcontext()
@@ -122,6 +132,10 @@ class PagePlan:
     max_len: Optional[int] = None
     info: Optional[torch.Tensor] = None   # int32 [2]: free pages after the step, refusal code
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_good", None)   # (tokens, device) that the tensors have been checked for
+
     @property
     def count(self) -> torch.Tensor:
         """int32 [1]: free pages after the step."""
@@ -150,18 +164,21 @@ def page_plan(pool: PagePool, fresh: torch.Tensor, tokens: int, commit: bool = T
     _ints(fresh, "fresh", (pool.rows,), pool.device)
     i32 = dict(dtype=torch.int32, device=pool.device)
     R = pool.rows
-    # one allocation: starts, slots, positions, info, lengths
-    buf = torch.empty(2 * R + 3 + 2 * tokens, **i32)
-    starts, slots, positions = buf[:R + 1], buf[R + 1:R + 1 + tokens], buf[R + 1 + tokens:R + 1 + 2 * tokens]
-    info = buf[R + 1 + 2 * tokens:R + 3 + 2 * tokens]
-    lengths = pool.lengths if commit else buf[R + 3 + 2 * tokens:]
+    # one allocation: starts, slots, positions, free pages and refusal, lengths
+    sizes = (R + 1, tokens, tokens, 2, 0 if commit else R)
+    buf = torch.empty(sum(sizes), **i32)
+    starts, slots, positions, info, lengths = buf.split_with_sizes(sizes)
+    if commit:
+        lengths = pool.lengths
     plan = PagePlan(starts, slots, positions, lengths, pool.tables, pool.page_size, max_new, max_len, info)
     if not pool.device.type == "cuda":
         _page_plan_reference(pool, fresh, plan, commit)
         return plan
+    at = buf.data_ptr()
     with _on(pool.device):
-        _lib.check(_fn("ats_page_plan")(_p(pool.lengths), _p(fresh), _p(pool.tables), _p(pool.free), _p(pool.state), _p(starts), _p(slots), _p(positions), _p(lengths), _p(info), R,
-                     pool.width, pool.pages, pool.page_size, tokens, int(commit), _lib.stream_ptr(pool.device)), "ats_page_plan")
+        _lib.check(_fn("ats_page_plan")(
+            _p(pool.lengths), _p(fresh), _p(pool.tables), _p(pool.free), _p(pool.state), at, at + 4 * (R + 1), at + 4 * (R + 1 + tokens), _p(lengths), at + 4 * (R + 1 + 2 * tokens), R,
+            pool.width, pool.pages, pool.page_size, tokens, int(commit), _stream(pool.device)), "ats_page_plan")
     return plan
 
 
@@ -210,18 +227,29 @@ def _page_plan_reference(pool: PagePool, fresh: torch.Tensor, plan: PagePlan, co
 # writing new tokens
 # ----------------------------------------------------------------------------------------------------------
 def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, like: torch.Tensor):
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.shape[1] == plan.page_size,
-          "k_pages, v_pages: contiguous [pages, page_size, n_kv, d] tensors of the plan's page size are needed")
-    _need(k_pages.dtype == v_pages.dtype == like.dtype and k_pages.device == v_pages.device == like.device, "pages and tokens: one type, one device")
+    if not (k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.shape[1] == plan.page_size):
+        raise ValueError("k_pages, v_pages: contiguous [pages, page_size, n_kv, d] tensors of the plan's page size are needed")
+    device = like.device
+    if not (k_pages.dtype == v_pages.dtype == like.dtype and k_pages.device == v_pages.device == device):
+        raise ValueError("pages and tokens: one type, one device")
     pages, ps, n_kv, d = k_pages.shape
-    R, T = plan.tables.shape[0], like.shape[0]
-    _need(pages * ps <= MAX_SLOTS and plan.tables.shape[1] * ps <= MAX_SLOTS and R <= MAX_ROWS, "slots have to stay below 2^31 - 256, rows at 4096")
-    _ints(plan.tables, "plan.tables", plan.tables.shape, like.device)
-    _ints(plan.lengths, "plan.lengths", (R,), like.device)
-    _ints(plan.starts, "plan.starts", (R + 1,), like.device)
-    _ints(plan.slots, "plan.slots", (T,), like.device)
-    _ints(plan.positions, "plan.positions", (T,), like.device)
+    if pages * ps > MAX_SLOTS:
+        raise ValueError("slots have to stay below 2^31 - 256")
+    if plan._good != (like.shape[0], device):
+        _check_plan(plan, like.shape[0], device)
     return pages, ps, n_kv, d
+
+
+def _check_plan(plan: PagePlan, T: int, device: torch.device) -> None:
+    R, width = plan.tables.shape
+    if width * plan.page_size > MAX_SLOTS or not 1 <= R <= MAX_ROWS:
+        raise ValueError("a table reaches below 2^31 - 256 tokens and has up to 4096 rows")
+    _ints(plan.tables, "plan.tables", (R, width), device)
+    _ints(plan.lengths, "plan.lengths", (R,), device)
+    _ints(plan.starts, "plan.starts", (R + 1,), device)
+    _ints(plan.slots, "plan.slots", (T,), device)
+    _ints(plan.positions, "plan.positions", (T,), device)
+    object.__setattr__(plan, "_good", (T, device))
 
 
 def _kernel_type(t: torch.Tensor, d: int) -> None:
@@ -233,6 +261,8 @@ def _kernel_type(t: torch.Tensor, d: int) -> None:
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """A [T, heads, d] (or [T, width]) tensor as its kernel takes it: rows of contiguous heads that start at multiples of 16 bytes."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     inner = t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == t.shape[2])
     if inner and (t.shape[0] == 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0:
         return t
@@ -262,10 +292,11 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
     q = torch.empty(T, n_q, d, dtype=qkv.dtype, device=qkv.device) if cos is not None else src[:, :n_q * d].unflatten(1, (n_q, d))
     if T == 0:
         return q
-    with _on(qkv.device):
+    device = qkv.device
+    with _on(device):
         _lib.check(_fn("ats_paged_append")(
             _p(src), src.stride(0) if T > 1 else src.shape[1], _p(cos), _p(sin), 0 if cos is None else cos.shape[0], _p(plan.positions), _p(plan.slots), _p(q), _p(k_pages),
-            _p(v_pages), T, n_q, n_kv, d, pages * ps, int(qkv.dtype == torch.float32), _p(_lib.status_tensor(qkv.device)), _lib.stream_ptr(qkv.device)),
+            _p(v_pages), T, n_q, n_kv, d, pages * ps, int(qkv.dtype == torch.float32), _p(_lib.status_tensor(device)), _stream(device)),
             "ats_paged_append")
     return q
 
@@ -295,11 +326,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """q [T, n_q, d], a step's queries (rotated; rows may be views of a wider projection) -> [T, n_q, d].  Token i of a row's new tokens attends to the
     row's tokens up to itself, in the pages of ``plan.tables``; its keys and values are there already.  ``scale`` (default 1 / sqrt(d)) times the scores.
     Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given.  Heads of up to 256 dimensions (multiples of 8)."""
-    _need(q.dim() == 3, "q: [tokens, heads, d] is needed")
+    if q.dim() != 3:
+        raise ValueError("q: [tokens, heads, d] is needed")
     pages, ps, n_kv, d = _check_pages(k_pages, v_pages, plan, q)
-    T, n_q = q.shape[:2]
-    if q.shape[2] != d or n_q < n_kv or n_q % n_kv:
-        raise ValueError(f"{n_q} query heads of {q.shape[2]} over {n_kv} key heads of {d}")
+    T, n_q, d_q = q.shape
+    if d_q != d or n_q < n_kv or n_q % n_kv:
+        raise ValueError(f"{n_q} query heads of {d_q} over {n_kv} key heads of {d}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _need(scale > 0 and math.isfinite(scale), "scale: a positive number")
     if out is not None:
@@ -314,12 +346,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if T == 0:
         return out
     q = _rows_of(q)
-    ldq, ldo = (t.stride(0) if T > 1 else n_q * d for t in (q, out))
+    ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (n_q * d, n_q * d)
     R, width = plan.tables.shape
     rep, new, keys = n_q // n_kv, min(plan.max_new or T, T), min(plan.max_len or width * ps, width * ps)
-    status, stream = _p(_lib.status_tensor(q.device)), _lib.stream_ptr(q.device)
+    device = q.device
+    status, stream = _p(_lib.status_tensor(device)), _stream(device)
     head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
-    with _on(q.device):
+    with _on(device):
         if q.dtype != torch.bfloat16 or d not in (64, 128) or ps < 8 or rep > 128 or (keys // 16 + 1) * R * n_kv >= 1 << 31:
             _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
             return out
@@ -328,10 +361,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         limit = 0 if rep > 16 else 8 if new * rep <= 8 or rep <= 8 < 16 < new * rep else 16
         portions = new * rep > limit
         if portions:
-            scratch = torch.empty(_fn("ats_paged_portion_scratch")(d), dtype=torch.uint8, device=q.device)
+            scratch = torch.empty(_scratch("ats_paged_portion_scratch", d), dtype=torch.uint8, device=device)
             _lib.check(_fn("ats_paged_portion")(*head, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_portion")
         if limit:
-            scratch = torch.empty(_fn("ats_paged_decode_scratch")(R, n_kv, d, keys, limit), dtype=torch.uint8, device=q.device)
+            scratch = torch.empty(_scratch("ats_paged_decode_scratch", R, n_kv, d, keys, limit), dtype=torch.uint8, device=device)
             _lib.check(_fn("ats_paged_decode")(*head, keys, T if portions else new, limit, scale, int(not keep_tail and not portions), _p(scratch), status, stream), "ats_paged_decode")
     return out
 

@@ -12,7 +12,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .paged import _fn, _need, _on, _p
+from .paged import _fn, _need, _on, _p, _stream
 
 MAX_VOCAB = 1 << 20
 PerRow = Union[int, float, torch.Tensor]
@@ -22,7 +22,7 @@ def _numbers(value: PerRow, dtype: torch.dtype):
     """-> (tensor [B] or None, number)."""
     if not isinstance(value, torch.Tensor):
         return None, (int if dtype == torch.int32 else float)(value)
-    return value.to(dtype).contiguous(), 0
+    return (value if value.dtype == dtype and value.is_contiguous() else value.to(dtype).contiguous()), 0
 
 
 def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: PerRow = 1.0, top_k: PerRow = 0, top_p: PerRow = 1.0, min_p: PerRow = 0.0,
@@ -60,11 +60,11 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: PerRow
     tp, tp1 = _numbers(top_p, torch.float32)
     mp, mp1 = _numbers(min_p, torch.float32)
     rp, rp1 = _numbers(repetition_penalty, torch.float32)
-    u = uniform.float().contiguous()
+    u, _ = _numbers(uniform, torch.float32)
     n = 0 if history is None else history.shape[1]
     with _on(logits.device):
         _lib.check(_fn("ats_sample_rows")(_p(logits), int(logits.dtype == torch.float32), logits.stride(0), B, V, _p(u), _p(t), t1, _p(k), k1, _p(tp), tp1, _p(mp), mp1, _p(rp), rp1,
-                     _p(history) if n else 0, n, history.stride(0) if n else 0, _p(out), _lib.stream_ptr(logits.device)), "ats_sample_rows")
+                     _p(history) if n else 0, n, history.stride(0) if n else 0, _p(out), _stream(logits.device)), "ats_sample_rows")
     return out
 
 

@@ -566,7 +566,8 @@ template <int D>
 static int launch_paged_portion(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PagedPortionArgs& p, cudaStream_t s) {
   using SM = PagedPortionSmem<D>;
   static_assert(SM::TOTAL <= 227 * 1024, "does not fit an SM");
-  cudaError_t ce = cudaFuncSetAttribute(paged_portion_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
+  static DeviceOnce once;
+  cudaError_t ce = once.smem(paged_portion_kernel<D>, SM::TOTAL);
   if (ce == cudaSuccess) ce = launch_pdl(paged_portion_kernel<D>, dim3(p.ctas), dim3(PC_THREADS), SM::TOTAL, s, mq, mk, mv, p);
   if (ce == cudaSuccess && p.ctas > 1) ce = launch_pdl(paged_portion_join_kernel<D>, dim3(p.ctas - 1, 256 / PCJ_ROWS), dim3(PCJ_THREADS), 0, s, p);
   if (ce != cudaSuccess) return int(ce);

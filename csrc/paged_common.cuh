@@ -1,6 +1,7 @@
 // What the tensor-core kernels over paged caches share.
 #pragma once
 #include "common.cuh"
+#include <atomic>
 
 namespace ats {
 
@@ -23,6 +24,20 @@ inline int make_tmap_tokens(CUtensorMap* out, const void* base, uint64_t rows, u
 inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, uint64_t n_kv, uint64_t d, uint32_t box_rows) {
   return make_tmap_tokens(out, base, rows, n_kv, d, n_kv * d, 1, box_rows);
 }
+
+// A kernel's shared-memory limit, raised once per device.
+struct DeviceOnce {
+  std::atomic<unsigned long long> done{0};
+  template <typename K>
+  cudaError_t smem(K kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+  }
+};
 
 struct PagedRows {
   const int* starts;    // [R + 1] packed starts of the rows' new tokens

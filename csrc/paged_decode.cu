@@ -453,7 +453,8 @@ static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
 
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
-  cudaError_t ce = cudaFuncSetAttribute(paged_decode_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_SMEM);
+  static DeviceOnce once;
+  cudaError_t ce = once.smem(paged_decode_kernel<D, NR>, PD_SMEM);
   if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
   // slots of a pair, if the rows are about as long as each other
   const int slots = p.warps / (p.rows.R * p.n_kv);
