@@ -62,44 +62,52 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
   if (tid == 0) s_bad = 0;
   __syncthreads();
   const int n_free = p.state[0];
-  int carry[3] = {0, 0, 0};
-  for (int r0 = 0; r0 < p.R; r0 += PLAN_THREADS) {
-    const int r = r0 + tid;
-    int v[3] = {0, 0, 0};
-    if (r < p.R) {
-      const int old = p.lengths[r], fresh = p.fresh[r];
-      // 1: more tokens than the row's table or the packed batch holds (or a length that no row has)
-      if (old < 0 || old > room || fresh < -1 || fresh > p.tokens || old + (long long)max(fresh, 0) > room) {
-        s_bad = 1;
-      } else {
-        const int held = (old + page - 1) >> p.page_log;
-        v[0] = max(fresh, 0);
-        if (fresh < 0) v[2] = held;
-        else v[1] = ((old + fresh + page - 1) >> p.page_log) - held;
-      }
+  // every thread sums up a share of consecutive rows
+  const int share = (p.R + PLAN_THREADS - 1) / PLAN_THREADS, r0 = min(tid * share, p.R), r1 = min(r0 + share, p.R);
+  auto row = [&](int old, int fresh, int (&v)[3]) {   // tokens, pages taken, pages returned
+    v[0] = v[1] = v[2] = 0;
+    // 1: more tokens than the row's table or the packed batch holds (or a length that no row has)
+    if (old < 0 || old > room || fresh < -1 || fresh > p.tokens || old + (long long)max(fresh, 0) > room) {
+      s_bad = 1;
+      return;
     }
-    int incl[3];
+    const int held = (old + page - 1) >> p.page_log;
+    v[0] = max(fresh, 0);
+    if (fresh < 0) v[2] = held;
+    else v[1] = ((old + fresh + page - 1) >> p.page_log) - held;
+  };
+  int sum[3] = {0, 0, 0}, v[3];
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) {
+    row(p.lengths[r], p.fresh[r], v);
+    sum[0] += v[0], sum[1] += v[1], sum[2] += v[2];
+  }
+  int carry[3], before[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      incl[i] = v[i];
+  for (int i = 0; i < 3; ++i) {
+    int incl = sum[i];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl[i], o);
-        if (lane >= o) incl[i] += u;
-      }
-      if (lane == 31) s_warp[i][warp] = incl[i];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
     }
-    __syncthreads();
+    if (lane == 31) s_warp[i][warp] = incl;
+    before[i] = incl - sum[i];
+  }
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      int before = carry[i];
-      for (int w = 0; w < PLAN_THREADS / 32; ++w) {
-        if (w < warp) before += s_warp[i][w];
-        carry[i] += s_warp[i][w];
-      }
-      if (r < p.R) (i == 0 ? starts : i == 1 ? taken : returned)[r] = before + incl[i] - v[i];
+  for (int i = 0; i < 3; ++i) {
+    carry[i] = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_THREADS / 32; ++w) {
+      if (w < warp) before[i] += s_warp[i][w];
+      carry[i] += s_warp[i][w];
     }
-    __syncthreads();
+  }
+  for (int r = r0; r < r1; ++r) {
+    starts[r] = before[0], taken[r] = before[1], returned[r] = before[2];
+    row(p.lengths[r], p.fresh[r], v);
+    before[0] += v[0], before[1] += v[1], before[2] += v[2];
   }
   if (tid == 0) starts[p.R] = carry[0], taken[p.R] = carry[1], returned[p.R] = carry[2];
   __syncthreads();
@@ -161,11 +169,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Append.  One CTA per token.  A lane holds eight columns of a head's first half and the eight that they are rotated with, and keeps its
-// eight cosines and sines for all heads that it serves; a warp's lanes cover whole halves of consecutive heads, so that every access is
-// whole sectors.  Bound by memory: the projection is read once, queries, keys and values are written once.
+// Append.  One CTA per token, a thread for every item: eight columns of a head's first half and the eight that they are rotated with, or sixteen columns that
+// only move.  A thread asks for its columns before the token's place is known; a warp's lanes cover whole halves of consecutive heads, so that every
+// access is whole sectors.  Bound by memory: the projection is read once, queries, keys and values are written once.
 // ------------------------------------------------------------------------------------------------
-constexpr int APP_THREADS = 256;
+constexpr int APP_MAX_THREADS = 512;
 
 struct AppendArgs {
   const void* qkv;         // [tokens, ld]: n_q query heads, n_kv key heads, n_kv value heads of d
@@ -183,50 +191,51 @@ struct AppendArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(APP_THREADS) paged_append_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(APP_MAX_THREADS) paged_append_kernel(const AppendArgs p) {
   pdl_prologue();
-  const int t = blockIdx.x, tid = threadIdx.x;
+  const int t = blockIdx.x, half = p.d >> 1;
   const T* row = static_cast<const T*>(p.qkv) + (long long)t * p.ld;
-  int slot = p.slots[t];
-  const int pos = p.positions[t];
-  if (slot >= p.n_slots || (p.cos_t && (pos < 0 || pos >= p.table))) {   // a plan of another pool, or positions that the tables do not reach
-    if (tid == 0) atomicCAS(p.status, 0, int(kBadArgument));
-    return;
-  }
-  const long long kv = (long long)max(slot, 0) * p.n_kv * p.d;
-  T* k_row = static_cast<T*>(p.k_pages) + kv;
-  T* v_row = static_cast<T*>(p.v_pages) + kv;
-  const int first = p.cos_t ? 0 : p.n_q;   // first head to go through
-  if (p.cos_t) {
-    const int half = p.d >> 1, lanes = half >> 3;   // lanes of a head (a multiple of 16 columns each)
-    const int per = APP_THREADS / lanes;            // heads at a time
-    const int c = (tid % lanes) * 8;
-    if (tid < per * lanes) {
-      float cs[8], sn[8];
-      Typed<float>::load8(p.cos_t + (long long)pos * half + c, cs);
-      Typed<float>::load8(p.sin_t + (long long)pos * half + c, sn);
-      for (int h = tid / lanes; h < p.n_q + p.n_kv; h += per) {
-        float u[8], w[8], a[8], b[8];
-        Typed<T>::load8(row + (long long)h * p.d + c, u);
-        Typed<T>::load8(row + (long long)h * p.d + half + c, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] = u[e] * cs[e] - w[e] * sn[e];
-          b[e] = w[e] * cs[e] + u[e] * sn[e];
-        }
-        T* dst = h < p.n_q ? static_cast<T*>(p.q_out) + ((long long)t * p.n_q + h) * p.d : k_row + (long long)(h - p.n_q) * p.d;
-        if (h < p.n_q || slot >= 0) {
-          Typed<T>::store8(dst + c, a);
-          Typed<T>::store8(dst + half + c, b);
-        }
+  const int lanes = half >> 3, turned = p.cos_t ? (p.n_q + p.n_kv) * lanes : 0;   // lanes of a head, items that are rotated
+  const int from = p.cos_t ? (p.n_q + p.n_kv) * p.d : p.n_q * p.d;                // first column that only moves
+  const int pieces = ((p.n_q + 2 * p.n_kv) * p.d - from) >> 3, items = turned + ((pieces + 1) >> 1);
+  int slot = -1, pos = -1;
+  for (int i = threadIdx.x; i < items; i += blockDim.x) {
+    const bool turn = i < turned;
+    const int h = turn ? i / lanes : 0, c = turn ? (i - h * lanes) * 8 : 0;
+    const int c0 = turn ? h * p.d + c : from + (i - turned) * 16, c1 = turn ? c0 + half : c0 + 8;
+    const bool second = turn || 2 * (i - turned) + 1 < pieces;
+    const typename Typed<T>::Raw8 a = Typed<T>::raw8(row + c0), b = Typed<T>::raw8(row + (second ? c1 : c0));
+    if (pos < 0) {
+      slot = p.slots[t];
+      pos = p.positions[t];
+      if (slot >= p.n_slots || pos < 0 || (p.cos_t && pos >= p.table)) {   // a plan of another pool, or positions that the tables do not reach
+        if (threadIdx.x == 0) atomicCAS(p.status, 0, int(kBadArgument));
+        return;
       }
     }
+    const long long kv = (long long)max(slot, 0) * p.n_kv * p.d;
+    if (turn) {
+      if (h >= p.n_q && slot < 0) continue;
+      float u[8], w[8], cs[8], sn[8], x[8], y[8];
+      Typed<float>::load8(p.cos_t + (long long)pos * half + c, cs);
+      Typed<float>::load8(p.sin_t + (long long)pos * half + c, sn);
+      Typed<T>::unpack8(a, u);
+      Typed<T>::unpack8(b, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = u[e] * cs[e] - w[e] * sn[e];
+        y[e] = w[e] * cs[e] + u[e] * sn[e];
+      }
+      T* dst = h < p.n_q ? static_cast<T*>(p.q_out) + ((long long)t * p.n_q + h) * p.d : static_cast<T*>(p.k_pages) + kv + (long long)(h - p.n_q) * p.d;
+      Typed<T>::store8(dst + c, x);
+      Typed<T>::store8(dst + half + c, y);
+    } else if (slot >= 0) {
+      const int keys = (p.n_q + p.n_kv) * p.d;   // columns up to here are queries and keys
+      auto place = [&](int col) { return col < keys ? static_cast<T*>(p.k_pages) + kv + (col - p.n_q * p.d) : static_cast<T*>(p.v_pages) + kv + (col - keys); };
+      Typed<T>::store_raw8(place(c0), a);
+      if (second) Typed<T>::store_raw8(place(c1), b);
+    }
   }
-  if (slot < 0) return;
-  const int kv8 = p.n_kv * p.d >> 3;
-  const T* src = row + (long long)p.n_q * p.d;
-  for (int i = tid + (first ? 0 : kv8); i < 2 * kv8; i += APP_THREADS)
-    Typed<T>::store_raw8(i < kv8 ? k_row + i * 8 : v_row + (i - kv8) * 8, Typed<T>::raw8(src + (long long)i * 8));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -387,7 +396,7 @@ ATS_API int ats_page_plan(int* lengths, const int* fresh, int* tables, int* free
   p.lengths = lengths; p.fresh = fresh; p.tables = tables; p.free = free_stack; p.state = state; p.starts = starts; p.slots = slots;
   p.positions = positions; p.lengths_out = lengths_out; p.info = info;
   p.R = R; p.width = width; p.pages = pages; p.page_log = __builtin_ctz(page); p.tokens = tokens; p.commit = commit;
-  const int blocks = max(1, min(148, (tokens + R + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS)));
+  const int blocks = max(1, min(148, (max(tokens, R) + PLAN_THREADS - 1) / PLAN_THREADS));   // (a token a thread: chains of dependent loads run side by side)
   const size_t smem = 3 * size_t(R + 1) * sizeof(int);
   cudaError_t ce = cudaSuccess;
   if (smem > 48 * 1024) ce = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
@@ -404,8 +413,10 @@ ATS_API int ats_paged_append(const void* qkv, long long ld, const float* cos_t, 
   p.qkv = qkv; p.ld = ld; p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.slots = slots; p.q_out = q_out; p.k_pages = k_pages;
   p.v_pages = v_pages; p.tokens = tokens; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.table = table; p.n_slots = n_slots; p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t ce = fp32 ? launch_pdl(paged_append_kernel<float>, dim3(tokens), dim3(APP_THREADS), 0, s, p)
-                              : launch_pdl(paged_append_kernel<__nv_bfloat16>, dim3(tokens), dim3(APP_THREADS), 0, s, p);
+  const int items = cos_t ? (n_q + n_kv) * (d >> 4) + (n_kv * (d >> 3) + 1) / 2 : n_kv * (d >> 3);
+  const dim3 threads(min(APP_MAX_THREADS, (items + 31) / 32 * 32));
+  const cudaError_t ce = fp32 ? launch_pdl(paged_append_kernel<float>, dim3(tokens), threads, 0, s, p)
+                              : launch_pdl(paged_append_kernel<__nv_bfloat16>, dim3(tokens), threads, 0, s, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }
