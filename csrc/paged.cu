@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Append.  One CTA per token, a thread for every item: eight columns of a head's first half and the eight that they are rotated with, or sixteen columns that
-// only move.  A thread asks for its columns before the token's place is known; a warp's lanes cover whole halves of consecutive heads, so that every
+// Append.  A CTA takes every so many-th token, a thread of it always the same item: eight columns of a head's first half and the eight that they are rotated with, or sixteen columns that
+// only move.  A thread asks for the next token's columns before it works on this one's; a warp's lanes cover whole halves of consecutive heads, so that every
 // access is whole sectors.  Bound by memory: the projection is read once, queries, keys and values are written once.
 // ------------------------------------------------------------------------------------------------
 constexpr int APP_MAX_THREADS = 512;
@@ -193,47 +193,58 @@ struct AppendArgs {
 template <typename T>
 __global__ void __launch_bounds__(APP_MAX_THREADS) paged_append_kernel(const AppendArgs p) {
   pdl_prologue();
-  const int t = blockIdx.x, half = p.d >> 1;
-  const T* row = static_cast<const T*>(p.qkv) + (long long)t * p.ld;
+  using Raw = typename Typed<T>::Raw8;
+  const int half = p.d >> 1;
   const int lanes = half >> 3, turned = p.cos_t ? (p.n_q + p.n_kv) * lanes : 0;   // lanes of a head, items that are rotated
   const int from = p.cos_t ? (p.n_q + p.n_kv) * p.d : p.n_q * p.d;                // first column that only moves
   const int pieces = ((p.n_q + 2 * p.n_kv) * p.d - from) >> 3, items = turned + ((pieces + 1) >> 1);
-  int slot = -1, pos = -1;
+  const int keys = (p.n_q + p.n_kv) * p.d;   // columns up to here are queries and keys
   for (int i = threadIdx.x; i < items; i += blockDim.x) {
     const bool turn = i < turned;
     const int h = turn ? i / lanes : 0, c = turn ? (i - h * lanes) * 8 : 0;
     const int c0 = turn ? h * p.d + c : from + (i - turned) * 16, c1 = turn ? c0 + half : c0 + 8;
     const bool second = turn || 2 * (i - turned) + 1 < pieces;
-    const typename Typed<T>::Raw8 a = Typed<T>::raw8(row + c0), b = Typed<T>::raw8(row + (second ? c1 : c0));
-    if (pos < 0) {
+    // where the item's columns go, as far as the slot does not matter
+    T* base = turn && h < p.n_q ? static_cast<T*>(p.q_out) : c0 < keys ? static_cast<T*>(p.k_pages) : static_cast<T*>(p.v_pages);
+    T* base1 = turn ? base + half : c1 < keys ? static_cast<T*>(p.k_pages) : static_cast<T*>(p.v_pages);
+    const bool to_q = turn && h < p.n_q;
+    const int off = to_q ? h * p.d + c : c0 < keys ? c0 - p.n_q * p.d : c0 - keys, off1 = turn ? off : c1 < keys ? c1 - p.n_q * p.d : c1 - keys;
+    auto fetch = [&](int t, Raw& a, Raw& b, int& slot, int& pos) {
+      const T* row = static_cast<const T*>(p.qkv) + (long long)t * p.ld;
+      a = Typed<T>::raw8(row + c0);
+      b = Typed<T>::raw8(row + (second ? c1 : c0));
       slot = p.slots[t];
       pos = p.positions[t];
+    };
+    Raw a, b, a_next, b_next;
+    int slot, pos, slot_next = -1, pos_next = 0;
+    int t = blockIdx.x;
+    fetch(t, a, b, slot, pos);
+    for (; t < p.tokens; t += gridDim.x, a = a_next, b = b_next, slot = slot_next, pos = pos_next) {
+      if (t + int(gridDim.x) < p.tokens) fetch(t + gridDim.x, a_next, b_next, slot_next, pos_next);   // the next token's, under this one's
       if (slot >= p.n_slots || pos < 0 || (p.cos_t && pos >= p.table)) {   // a plan of another pool, or positions that the tables do not reach
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, int(kBadArgument));
-        return;
+        if (i == 0) atomicCAS(p.status, 0, int(kBadArgument));
+        continue;
       }
-    }
-    const long long kv = (long long)max(slot, 0) * p.n_kv * p.d;
-    if (turn) {
-      if (h >= p.n_q && slot < 0) continue;
-      float u[8], w[8], cs[8], sn[8], x[8], y[8];
-      Typed<float>::load8(p.cos_t + (long long)pos * half + c, cs);
-      Typed<float>::load8(p.sin_t + (long long)pos * half + c, sn);
-      Typed<T>::unpack8(a, u);
-      Typed<T>::unpack8(b, w);
+      if (!to_q && slot < 0) continue;
+      const long long place = to_q ? (long long)t * p.n_q * p.d : (long long)slot * p.n_kv * p.d;
+      if (turn) {
+        float u[8], w[8], cs[8], sn[8], x[8], y[8];
+        Typed<float>::load8(p.cos_t + (long long)pos * half + c, cs);
+        Typed<float>::load8(p.sin_t + (long long)pos * half + c, sn);
+        Typed<T>::unpack8(a, u);
+        Typed<T>::unpack8(b, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = u[e] * cs[e] - w[e] * sn[e];
-        y[e] = w[e] * cs[e] + u[e] * sn[e];
+        for (int e = 0; e < 8; ++e) {
+          x[e] = u[e] * cs[e] - w[e] * sn[e];
+          y[e] = w[e] * cs[e] + u[e] * sn[e];
+        }
+        Typed<T>::store8(base + place + off, x);
+        Typed<T>::store8(base1 + place + off1, y);
+      } else {
+        Typed<T>::store_raw8(base + place + off, a);
+        if (second) Typed<T>::store_raw8(base1 + place + off1, b);
       }
-      T* dst = h < p.n_q ? static_cast<T*>(p.q_out) + ((long long)t * p.n_q + h) * p.d : static_cast<T*>(p.k_pages) + kv + (long long)(h - p.n_q) * p.d;
-      Typed<T>::store8(dst + c, x);
-      Typed<T>::store8(dst + half + c, y);
-    } else if (slot >= 0) {
-      const int keys = (p.n_q + p.n_kv) * p.d;   // columns up to here are queries and keys
-      auto place = [&](int col) { return col < keys ? static_cast<T*>(p.k_pages) + kv + (col - p.n_q * p.d) : static_cast<T*>(p.v_pages) + kv + (col - keys); };
-      Typed<T>::store_raw8(place(c0), a);
-      if (second) Typed<T>::store_raw8(place(c1), b);
     }
   }
 }
@@ -415,8 +426,9 @@ ATS_API int ats_paged_append(const void* qkv, long long ld, const float* cos_t, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int items = cos_t ? (n_q + n_kv) * (d >> 4) + (n_kv * (d >> 3) + 1) / 2 : n_kv * (d >> 3);
   const dim3 threads(min(APP_MAX_THREADS, (items + 31) / 32 * 32));
-  const cudaError_t ce = fp32 ? launch_pdl(paged_append_kernel<float>, dim3(tokens), threads, 0, s, p)
-                              : launch_pdl(paged_append_kernel<__nv_bfloat16>, dim3(tokens), threads, 0, s, p);
+  const dim3 grid(min(tokens, 148 * max(1, 1536 / int(threads.x))));
+  const cudaError_t ce = fp32 ? launch_pdl(paged_append_kernel<float>, grid, threads, 0, s, p)
+                              : launch_pdl(paged_append_kernel<__nv_bfloat16>, grid, threads, 0, s, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }
