@@ -25,6 +25,22 @@ inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, ui
   return make_tmap_tokens(out, base, rows, n_kv, d, n_kv * d, 1, box_rows);
 }
 
+// Launches a kernel that begins with pdl_prologue() right behind one of the same operator that asks for it (griddepcontrol.launch_dependents behind its own
+// wait): it is set up while that one ends, whatever launches the thread makes else.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
 // A kernel's shared-memory limit, raised once per device.
 struct DeviceOnce {
   std::atomic<unsigned long long> done{0};

@@ -97,11 +97,16 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
     for (int i = 0; i < PD_STAGES; ++i) mbar_init(&full[i], 1);
     mbar_fence_init();
   }
-  if (tid == 0) s_abort = 0;
+  if (tid == 0) {
+    s_abort = 0;
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
   // where the rows begin on the line: every thread sums up a share of the rows
   const int share = (rows.R + PD_THREADS - 1) / PD_THREADS, r0 = min(tid * share, rows.R), r1 = min(r0 + share, rows.R);
   uint32_t mine = 0;
   for (int r = r0; r < r1; ++r) mine += pd_units<UNIT>(p, r);
+  const int fresh_last = r0 < rows.R ? rows.starts[r0 + 1] - rows.starts[r0] : 0;
   uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -120,10 +125,10 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   const PdShares shares(p, total);
   const uint32_t me0 = blockIdx.x * PD_WARPS;
   for (int r = r0; r < r1; ++r) {
-    const uint32_t n = pd_units<UNIT>(p, r), at = before * p.n_kv;
+    const uint32_t n = share == 1 ? mine : pd_units<UNIT>(p, r), at = before * p.n_kv;
     if (blockIdx.x == 0) {
       p.line[r] = before;
-      if (rows.starts[r + 1] - rows.starts[r] > p.max_new) atomicCAS(p.status, 0, int(kBadArgument));   // more than the caller promised: nobody serves the row
+      if ((share == 1 ? fresh_last : rows.starts[r + 1] - rows.starts[r]) > p.max_new) atomicCAS(p.status, 0, int(kBadArgument));   // more than the caller promised: nobody serves the row
     }
 #pragma unroll
     for (int w = 0; w < PD_WARPS; ++w) {
@@ -134,13 +139,16 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
   }
   if (blockIdx.x == 0 && tid == 0) p.line[rows.R] = total / p.n_kv;
   __syncthreads();
-  if (p.zero_tail) {
+  auto zero_tail = [&]() {
     const int tail = min(max(rows.starts[rows.R], 0), rows.tokens), vecs = p.n_kv * p.rep * (D / 8);
     for (long long i = (long long)blockIdx.x * PD_THREADS + tid; i < (long long)(rows.tokens - tail) * vecs; i += (long long)gridDim.x * PD_THREADS)
       *reinterpret_cast<uint4*>(p.out + (tail + i / vecs) * p.ldo + (i % vecs) * 8) = make_uint4(0, 0, 0, 0);
-  }
+  };
   const uint32_t me = me0 + warp;
-  if (me >= shares.n) return;
+  if (me >= shares.n) {
+    if (p.zero_tail) zero_tail();
+    return;
+  }
   const uint32_t lo = shares.begin(me);
   const int n_mine = int(shares.begin(me + 1) - lo);
 
@@ -379,6 +387,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
     u0 = 0;
     if (++hk == p.n_kv) hk = 0, ++row;
   }
+  if (p.zero_tail) zero_tail();
 }
 
 // The scratch slots of a pair (row, key head) that several warps shared.  D / 4 lanes hold an MMA row's columns; G such groups take the row's slots
@@ -448,7 +457,7 @@ template <int D, int NR, int G>
 static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
   constexpr int AT_ONCE = PJ_THREADS / (G * D / 4);
   const int n = min(p.limit, p.rows_most);
-  return launch_pdl(paged_join_kernel<D, NR, G>, dim3((n + AT_ONCE - 1) / AT_ONCE, p.n_kv, p.rows.R), dim3(PJ_THREADS), 0, s, p);
+  return launch_behind(paged_join_kernel<D, NR, G>, dim3((n + AT_ONCE - 1) / AT_ONCE, p.n_kv, p.rows.R), dim3(PJ_THREADS), s, p);
 }
 
 template <int D, int NR>
