@@ -12,6 +12,9 @@
 // that its last token sees and PC_PIECE more for its beginning and end, form one line, and each of 148 CTAs takes an equal stretch of it.  The roles of a CTA run through the pieces of
 // the stretch independently, so the loads and the first scores of the next piece overlap the end of this one.  A pair of tiles that CTAs share
 // leaves fp32 sums in scratch slots, joined by a second launch in the order of the line: results do not depend on timing.
+// A block on the diagonal, or with the row's last key, holds values that some or all rows of the tiles must not see: a probability of zero does not
+// keep a NaN or an infinity out of a product.  Two warps of their own clear such values in shared memory before the product (those that no row
+// sees altogether), and a query that does see them adds them to its output at the end.
 // Every wait is bounded (status word + clean unwind); no load uses cluster multicast.
 #include "paged_common.cuh"
 
@@ -19,10 +22,11 @@ namespace ats {
 
 constexpr int PC_CTAS = 148;
 constexpr int PC_PIECE = 192;    // keys that take as long as the first loads and scores and the outputs of a pair of tiles (4 us, a block of 128 keys 2.4 us)
-constexpr int PC_THREADS = 320;  // soft-max A (warps 0-3), soft-max B (4-7), TMA (8), MMA (9)
+constexpr int PC_THREADS = 384;  // soft-max A (warps 0-3), soft-max B (4-7), TMA (8), MMA (9), values of blocks on the diagonal (10, 11)
 
 struct PagedPortionArgs {
   PagedRows rows;
+  const __nv_bfloat16* v_pages;
   __nv_bfloat16* out;       // [tokens, ldo]
   long long ldo;
   int n_kv, rep, limit;     // rows with more than `limit` query rows (new tokens times rep) are taken
@@ -44,6 +48,8 @@ struct PcPlace {
   unsigned long long base, pad2;
   __device__ __forceinline__ void find(const PagedPortionArgs& p, int r, unsigned long long row_base, unsigned long long x);   // x within row r
 };
+
+constexpr int PC_EDGE = 4;   // blocks of a piece with values that not every row sees: 256 tokens touch three
 
 template <int D>
 struct PagedPortionSmem {
@@ -102,7 +108,7 @@ __device__ __forceinline__ int pc_block(unsigned long long base, unsigned long l
   return x > base + PC_PIECE ? int((x - base - PC_PIECE) >> 7) : 0;
 }
 
-// A piece: key blocks [j0, j1) of a pair of tiles.
+// A piece: key blocks [j0, j1) of a pair of tiles (none: the stretch has ended).
 struct PcPiece {
   int row, hk, first, fresh, keys, tok0;   // tok0: first token of tile A within the portion
   int j0, j1, blocks;                      // of all the pair's blocks
@@ -110,18 +116,22 @@ struct PcPiece {
   bool opens;                              // the piece that the CTA's stretch begins with
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == blocks; }
   __device__ __forceinline__ int end(int x) const { return min(j1, n[x]); }
+  // the last key that every row of the piece sees, and the first block with others
+  __device__ __forceinline__ int open(const PagedPortionArgs& p) const { return keys - fresh + tok0 + (end(0) > j0 ? 0 : p.tile); }
+  __device__ __forceinline__ int edge(const PagedPortionArgs& p) const { return max(open(p) + 1, 0) >> 7; }
 };
 
 struct PcWalk {
   const PagedPortionArgs& p;
   PcPlace at;
   unsigned long long lo, hi;
-  __device__ __forceinline__ PcWalk(const PagedPortionArgs& args, const PcPlace& start, unsigned long long from, unsigned long long to) : p(args), at(start), lo(from), hi(to) {}
+  PcRow w;   // of row at.row: a piece of the row before costs no loads
+  __device__ __forceinline__ PcWalk(const PagedPortionArgs& args, const PcPlace& start, unsigned long long from, unsigned long long to)
+      : p(args), at(start), lo(from), hi(to), w(args, min(start.row, args.rows.R - 1)) {}
   __device__ __forceinline__ bool next(PcPiece& s) {
     while (at.base < hi) {
-      const PcRow w(p, at.row);
       if (w.cost == 0) {
-        ++at.row;
+        w = PcRow(p, ++at.row);
         continue;
       }
       const int pair = 2 * p.tile, seen = w.at + min((at.k + 1) * pair, w.fresh);
@@ -135,7 +145,10 @@ struct PcWalk {
       at.base += PC_PIECE + seen;
       if (++at.k == w.pairs) {
         at.k = 0;
-        if (++at.hk == p.n_kv) at.hk = 0, ++at.row;
+        if (++at.hk == p.n_kv) {
+          at.hk = 0;
+          if (at.base < hi) w = PcRow(p, ++at.row);   // (a row is to come)
+        }
       }
       if (s.j0 < s.j1) return true;
     }
@@ -158,16 +171,22 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   uint64_t* q_empty = bars + 1;         // 1: all scores of a piece are done
   uint64_t* k_full = bars + 2;          // [ST]
   uint64_t* k_empty = bars + 6;         // [ST]
-  uint64_t* v_full = bars + 10;         // [ST]
+  uint64_t* v_full = bars + 10;         // [ST], 2 arrivals
   uint64_t* v_empty = bars + 14;        // [ST]
-  uint64_t* v_raw = bars + 18;          // 1: values that end inside the block have landed
-  uint64_t* s_full = bars + 19;         // [2] per tile
-  uint64_t* p_full = bars + 21;         // [2] per tile, 4 arrivals
-  uint64_t* o_done = bars + 23;         // [2] per tile: last P V of a piece finished
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  uint64_t* v_raw = bars + 18;          // [ST]: values that not every row sees have landed
+  uint64_t* s_full = bars + 22;         // [2] per tile
+  uint64_t* p_full = bars + 24;         // [2] per tile, 4 arrivals
+  uint64_t* o_done = bars + 26;         // [2] per tile: last P V of a piece finished
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ unsigned long long s_sum[PC_THREADS / 32], s_base;
   __shared__ int s_row;
+  // per piece: keys whose values each of the two warps cleared, 128 bits a block from the first block on the diagonal on.  They are ahead of the warps
+  // that read these by the stages of the ring at most.
+  __shared__ uint32_t s_cleared[8][2][PC_EDGE * 4], s_any[8][2];
+  // The pieces, told by the producer: it is ahead of the others by the stages of the ring at most (every piece takes one), so eight places are enough.
+  __shared__ PcPiece s_piece[8];
+  __shared__ uint64_t s_told[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedRows& rows = p.rows;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -176,11 +195,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   if (tid == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    mbar_init(v_raw, 1);
     for (int x = 0; x < ST; ++x) {
+      mbar_init(&v_raw[x], 1);
       mbar_init(&k_full[x], 1);
       mbar_init(&k_empty[x], 1);
-      mbar_init(&v_full[x], 1);
+      mbar_init(&v_full[x], 2);
       mbar_init(&v_empty[x], 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -188,6 +207,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       mbar_init(&p_full[x], 4);
       mbar_init(&o_done[x], 1);
     }
+    for (int x = 0; x < 8; ++x) mbar_init(&s_told[x], 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_q);
@@ -237,17 +257,30 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   if (lo < hi) start.find(p, s_row, s_base, lo);
   else start.base = hi;
   if (tid == 0) p.begins[blockIdx.x] = start;
-  PcWalk walk(p, start, lo, hi);
-  PcPiece s;
+  auto next_piece = [&](uint32_t n) -> const PcPiece* {   // the n-th, or null behind the last one (and where a wait ran out)
+    if (!mbar_wait_bounded(&s_told[n & 7], (n >> 3) & 1, abort_flag, p.status, kTimeoutFull)) return nullptr;
+    const PcPiece* s = &s_piece[n & 7];
+    return s->j0 < s->j1 ? s : nullptr;
+  };
   // columns: S_A [0,128)  S_B [128,256)  O_A [256, 256 + D)  O_B [256 + D, 256 + 2 D)
 
   if (warp == 8) {
     // ------------------------------------------------------------------ producer: a whole warp, a page's copies from a lane each
     const int page = 1 << rows.page_log, box = min(128, page), copies = 128 / box * DC;   // copies of a block
     const int c = lane % DC, at = lane / DC * box;                                         // 64-column piece and first key of this lane's copy
-    uint32_t n_blocks = 0, n_raw = 0, n_pieces = 0;
+    uint32_t n_blocks = 0, n_pieces = 0;
     bool ok = true;
-    while (ok && walk.next(s)) {
+    PcWalk walk(p, start, lo, hi);
+    PcPiece s;
+    while (ok) {
+      const bool more = walk.next(s);
+      if (!more) s.j0 = s.j1 = 0;
+      if (lane == 0) {
+        s_piece[n_pieces & 7] = s;
+        mbar_arrive(&s_told[n_pieces & 7]);
+      }
+      if (!more) break;
+      const int edge = s.edge(p);
       const int* table = rows.tables + (long long)s.row * rows.width;
       const int n_pages = (s.keys + page - 1) >> rows.page_log;
       auto look_up = [&](int j) {
@@ -269,6 +302,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         if (lane == 0) mbar_expect_tx(&k_full[st], T);
         __syncwarp();
         if (lane < copies) tma_load_3d(sK + st * T + c * 16384 + at * 128, &map_k, &k_full[st], 64 * c, s.hk, here);
+        if (!(ok = mbar_wait_warp(&v_empty[st], ph ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
+        uint64_t* bar = j >= edge ? &v_raw[st] : &v_full[st];
+        if (lane == 0) {
+          mbar_expect_tx(bar, T);
+          if (j < edge) mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (lane < copies) tma_load_3d(sV + st * T + c * 16384 + at * 128, &map_v, bar, 64 * c, s.hk, here);
         if (j == s.j0) {   // the queries, once the last piece's scores are done
           if (!(ok = mbar_wait_warp(q_empty, (n_pieces & 1) ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
           ++n_pieces;
@@ -280,24 +321,6 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < DC; ++i) tma_load_3d(sQ + x * T + i * 16384, &map_q, q_full, 64 * i, s.hk * p.rep, s.first + s.tok0 + x * p.tile);
           }
-        }
-        if (!(ok = mbar_wait_warp(&v_empty[st], ph ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
-        const int live = s.keys - j * 128;   // values behind these are whatever earlier generations left in the page
-        uint64_t* bar = live < 128 ? v_raw : &v_full[st];
-        if (lane == 0) mbar_expect_tx(bar, T);
-        __syncwarp();
-        if (lane < copies) tma_load_3d(sV + st * T + c * 16384 + at * 128, &map_v, bar, 64 * c, s.hk, here);
-        if (live < 128) {
-          if (!(ok = mbar_wait_warp(v_raw, n_raw & 1, abort_flag, p.status, kTimeoutFull))) break;
-          ++n_raw;
-          const int from = max(live, 0);
-          for (int i = lane; i < (128 - from) * 8 * DC; i += 32) {
-            const int piece = i / ((128 - from) * 8), at16 = i - piece * (128 - from) * 8;
-            *reinterpret_cast<uint4*>(sV + st * T + piece * 16384 + from * 128 + at16 * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[st]);
         }
       }
     }
@@ -330,27 +353,29 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       };
       uint32_t n_blocks = 0, n_pieces = 0, n_p[2] = {0, 0};
       bool ok = true;
-      while (ok && walk.next(s)) {
-        const int ends[2] = {s.end(0), s.end(1)};
+      while (ok) {
+        const PcPiece* told = next_piece(n_pieces);
+        if (!told) break;
+        const int j0 = told->j0, j1 = told->j1, ends[2] = {told->end(0), told->end(1)};
         ok = mbar_wait_bounded(q_full, n_pieces & 1, abort_flag, p.status, kTimeoutFull);
         ok = ok && mbar_wait_bounded(&k_full[n_blocks % ST], (n_blocks / ST) & 1, abort_flag, p.status, kTimeoutFull);
         if (!ok) break;
         ++n_pieces;
         tc_fence_after();
         for (int x = 0; x < 2; ++x)
-          if (s.j0 < ends[x]) issue_s(x, n_blocks % ST);
+          if (j0 < ends[x]) issue_s(x, n_blocks % ST);
         tc_commit(&k_empty[n_blocks % ST]);
-        if (s.j0 + 1 == s.j1) tc_commit(q_empty);
-        for (int j = s.j0; j < s.j1; ++j, ++n_blocks) {
+        if (j0 + 1 == j1) tc_commit(q_empty);
+        for (int j = j0; j < j1; ++j, ++n_blocks) {
           const uint32_t st = n_blocks % ST, nst = (n_blocks + 1) % ST;
-          const bool more = j + 1 < s.j1;
+          const bool more = j + 1 < j1;
           if (!(ok = mbar_wait_bounded(&v_full[st], (n_blocks / ST) & 1, abort_flag, p.status, kTimeoutFull))) break;
           for (int x = 0; ok && x < 2; ++x) {
             if (j < ends[x]) {
               if (!(ok = mbar_wait_bounded(&p_full[x], n_p[x] & 1, abort_flag, p.status, kTimeoutTmemFull))) break;
               ++n_p[x];
               tc_fence_after();
-              issue_pv(x, st, j == s.j0);
+              issue_pv(x, st, j == j0);
               if (j + 1 == ends[x]) tc_commit(&o_done[x]);
             }
             if (x == 1) tc_commit(&v_empty[st]);
@@ -360,12 +385,56 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
               if (j + 1 < ends[x]) issue_s(x, nst);
               if (x == 1) {
                 tc_commit(&k_empty[nst]);
-                if (j + 2 == s.j1) tc_commit(q_empty);
+                if (j + 2 == j1) tc_commit(q_empty);
               }
             }
           }
           if (!ok) break;
         }
+      }
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------------ values of blocks on the diagonal: every other 32 pieces of 16 bytes each
+    const int me = warp - 10;
+    uint32_t n_blocks = 0, n_pieces = 0, phases = 0;   // phases: one bit a stage
+    bool ok = true;
+    for (; ok; ++n_pieces) {
+      const PcPiece* told = next_piece(n_pieces);
+      if (!__all_sync(0xffffffffu, told != nullptr)) break;
+      const PcPiece s = *told;
+      const int edge = s.edge(p), open = s.open(p), seen = s.keys - s.fresh + min(s.tok0 + 2 * p.tile, s.fresh);   // keys that some row sees
+      uint32_t* cleared = s_cleared[n_pieces & 7][me];
+      if (lane < PC_EDGE * 4) cleared[lane] = 0;
+      if (lane == 0) s_any[n_pieces & 7][me] = 0;
+      __syncwarp();
+      for (int j = s.j0; j < s.j1; ++j, ++n_blocks) {
+        if (j < edge) continue;
+        const int st = n_blocks % ST;
+        if (!(ok = mbar_wait_warp(&v_raw[st], phases >> st & 1, abort_flag, p.status, kTimeoutFull))) break;
+        phases ^= 1u << st;
+        const int live = min(max(seen - j * 128, 0), 128), from = max(open + 1 - j * 128, 0);   // rows [from, live) are some query's but not every one's
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          uint4* rows16 = reinterpret_cast<uint4*>(sV + st * T + c * 16384);   // eight to a row, in an order of their own
+#pragma unroll 4
+          for (int i = from * 8 + me * 32 + lane; i < live * 8; i += 64) {
+            const uint4 w = rows16[i];
+            // an exponent of ones carries into the sign's place of its half
+            auto up = [](uint32_t v) { return (v & 0x7f807f80u) + 0x00800080u; };
+            if ((up(w.x) | up(w.y) | up(w.z) | up(w.w)) & 0x80008000u) {
+              auto clear = [&](uint32_t v) { return v & ~(((up(v) & 0x80008000u) >> 15) * 0xffffu); };
+              rows16[i] = make_uint4(clear(w.x), clear(w.y), clear(w.z), clear(w.w));
+              const int bit = (j - edge) * 128 + (i >> 3);
+              if (bit < PC_EDGE * 128) atomicOr(&cleared[bit >> 5], 1u << (bit & 31));
+              s_any[n_pieces & 7][me] = 1;
+            }
+          }
+#pragma unroll 4
+          for (int i = live * 8 + me * 32 + lane; i < 1024; i += 64) rows16[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
       }
     }
   } else {
@@ -377,9 +446,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
     const uint32_t tmem_S = tmem_base + x * 128 + lane_base;
     const uint32_t tmem_O = tmem_base + 256 + x * D + lane_base;
     const int my_tok = r / p.rep, my_head = r - my_tok * p.rep;
-    uint32_t n_s = 0, n_o = 0;
+    uint32_t n_s = 0, n_o = 0, n_pieces = 0;
     bool ok = true;
-    while (ok && walk.next(s)) {
+    for (; ok; ++n_pieces) {
+      const PcPiece* told = next_piece(n_pieces);
+      if (!__all_sync(0xffffffffu, told != nullptr)) break;
+      const PcPiece& s = *told;   // (stays until the warp is through with it)
       const int tile_tok = s.tok0 + x * p.tile, tok = tile_tok + my_tok;
       const bool live = my_tok < p.tile && tok < s.fresh;
       const int first_pos = s.keys - s.fresh + tile_tok;        // of the tile's first token
@@ -463,12 +535,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       float* part = p.part_o + slot * D;
       if (live && !whole) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(any ? m : -INFINITY, l);
       if (any) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32(tmem_O + c * 32, o);
-          tmem_ld_wait();
-          if (!live) continue;
+        auto put = [&](int c, const uint32_t (&o)[32]) {
           if (whole) {
             uint4 w[4];
 #pragma unroll
@@ -490,6 +557,36 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
             for (int e = 0; e < 4; ++e)
               st_global_32B(part + c * 32 + e * 8, make_uint4(o[8 * e], o[8 * e + 1], o[8 * e + 2], o[8 * e + 3]),
                             make_uint4(o[8 * e + 4], o[8 * e + 5], o[8 * e + 6], o[8 * e + 7]));
+          }
+        };
+        if ((s_any[n_pieces & 7][0] | s_any[n_pieces & 7][1]) == 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(tmem_O + c * 32, o);
+            tmem_ld_wait();
+            if (live) put(c, o);
+          }
+        } else {   // values that are not finite, of keys that this query sees
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(tmem_O + c * 32, o);
+            tmem_ld_wait();
+            if (!live) continue;
+            for (int bit = 0; bit < PC_EDGE * 128; ++bit) {
+              const int key = s.edge(p) * 128 + bit;
+              if (key > my_pos || !((s_cleared[n_pieces & 7][0][bit >> 5] | s_cleared[n_pieces & 7][1][bit >> 5]) >> (bit & 31) & 1)) continue;
+              const int id = rows.tables[(long long)s.row * rows.width + (key >> rows.page_log)];
+              if (id < 0 || id >= rows.pages) continue;
+              const __nv_bfloat16* v = p.v_pages + ((((long long)id << rows.page_log) + (key & ((1 << rows.page_log) - 1))) * p.n_kv + s.hk) * D + c * 32;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float f = __bfloat162float(v[e]);
+                if ((__float_as_uint(f) & 0x7f800000u) == 0x7f800000u) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+              }
+            }
+            put(c, o);
           }
         }
         tc_fence_before();   // O has been read: the next piece's first P, which this warp announces, may be followed by a P V over it
@@ -596,7 +693,7 @@ ATS_API int ats_paged_portion(const void* q, long long ldq, const void* k_pages,
   }
   PagedPortionArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
-  p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
+  p.v_pages = static_cast<const __nv_bfloat16*>(v_pages); p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
   p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.tile = 128 / p.rep; p.ctas = PC_CTAS; p.zero_tail = zero_tail; p.wide = !(reinterpret_cast<uintptr_t>(out) & 31) && !(ldo & 15);
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   static_assert(sizeof(PcPlace) % 32 == 0, "the sums are written 32 bytes at a time");

@@ -5,7 +5,7 @@
 // A row takes this kernel when its new tokens times the query heads of a group are at most 8 (or 16): they are the rows of a warp-level MMA
 // (m16n8k16), and the step is a stream of the cache, each key and value read once.  Bound by memory.
 //
-// * Every warp moves units of 8 KB (K and V of 2048 / D keys) by TMA into a ring of two of its own, 192 KB an SM in flight over three CTAs,
+// * Every warp moves units of 8 KB (K and V of 2048 / D keys) by TMA into a ring of its own, 192 KB an SM in flight,
 //   and keeps a running softmax; the fragments come out of the swizzled units as in the decode kernel over contiguous rows (inference.cu).
 //   The page of a unit comes from the row's table, which the lanes read 32 entries at a time.
 // * Rows of a batch are of any length, so the work is dealt out by units, not by rows: the units of all rows and key heads form one line, and
@@ -17,8 +17,12 @@
 namespace ats {
 
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS;
-constexpr int PD_STAGES = 2, PD_UNIT_BYTES = 8192;
-constexpr int PD_SMEM = 1024 + PD_WARPS * PD_STAGES * PD_UNIT_BYTES;
+constexpr int PD_UNIT_BYTES = 8192;
+// Eight MMA rows leave registers for three CTAs of four warps an SM with a ring of two units each; sixteen (twice the sums and queries) for two with three
+// (8 rows of 5,000 to 31,000 keys, four tokens each: 92 us, with three CTAs and spilled registers 100): 192 KB in flight either way.
+__host__ __device__ constexpr int pd_ctas(int nr) { return nr > 1 ? 2 : 3; }
+__host__ __device__ constexpr int pd_stages(int nr) { return nr > 1 ? 3 : 2; }
+
 
 struct PagedDecodeArgs {
   PagedRows rows;
@@ -55,6 +59,9 @@ __device__ __forceinline__ float pd_exp2(float x) {
 }
 __device__ __forceinline__ float pd_from(float m, float base) { return m == -INFINITY ? 0.f : pd_exp2(m - base); }
 
+// The halves of two bf16 values that are not finite, at their signs' places: an exponent of ones carries into these.
+__device__ __forceinline__ uint32_t pd_odd(uint32_t v) { return ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
 // Units of row r on this kernel's line, per key head (0: the row is empty or another kernel's).
 template <int UNIT>
 __device__ __forceinline__ int pd_units(const PagedDecodeArgs& p, int r) {
@@ -62,6 +69,11 @@ __device__ __forceinline__ int pd_units(const PagedDecodeArgs& p, int r) {
   paged_row(p.rows, r, &first, &fresh, &keys);
   return fresh > 0 && (long long)fresh * p.rep <= p.limit ? (max(keys, 1) + UNIT - 1) / UNIT : 0;
 }
+
+template <bool V>
+struct PdBool {
+  static constexpr bool value = V;
+};
 
 // A line of `total` units (below 2^31) shared out over as many warps as there are, one more unit to each of the first `extra`.
 struct PdShares {
@@ -79,8 +91,9 @@ struct PdShares {
 };
 
 template <int D, int NR>  // NR: sets of eight MMA rows (1 or 2)
-__global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(PD_THREADS, pd_ctas(NR)) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                      const PagedDecodeArgs p) {
+  constexpr int PD_STAGES = pd_stages(NR);
   constexpr int UNIT = 2048 / D, NT = UNIT / 8, KB = UNIT / 16, JD = D / 32, RD = D / 64, ROWS = 8 * NR;
   extern __shared__ uint8_t pd_smem[];
   __shared__ uint64_t s_full[PD_WARPS][PD_STAGES];
@@ -251,18 +264,10 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
         for (int e = 0; e < 4; ++e) oe[rd][i][e] = oo[rd][i][e] = 0.f;
 #pragma unroll
     for (int x = 0; x < NR; ++x) m[x] = -INFINITY, l[x] = 0.f;
-#pragma unroll 1
-    for (int u = 0; u < count; ++u, ++done) {
-      const uint32_t stage = done % PD_STAGES;
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], (done / PD_STAGES) & 1, &s_abort, p.status, kTimeoutFull))) {
-        const uint64_t t0 = globaltimer_ns();   // copies that were issued land before the warp gives its shared memory back
-        while (globaltimer_ns() - t0 < 10000000ull) {
-        }
-        return;
-      }
-      const int k0 = (u0 + u) * UNIT;
+    // EDGE: the unit holds keys that some row does not see
+    auto unit = [&](auto edge_c, const int k0, const uint32_t stage) {
+      constexpr bool EDGE = decltype(edge_c)::value;
       const uint32_t ks = k_at + stage * PD_UNIT_BYTES, vs = v_at + stage * PD_UNIT_BYTES;
-      const bool edge = k0 + UNIT > open;   // the unit holds keys that some row does not see
       uint4 vv[KB][RD][4];
       float s[NT][2 * NR];
 #pragma unroll
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int rd = 0; rd < RD; ++rd) vv[kb][rd][i] = pd_lds(vs + (rd * UNIT + kb * 16 + (i >> 1) * 8) * 128 + vpiece[i & 1]);
-      if (edge) {
+      if (EDGE) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -333,23 +338,82 @@ __global__ void __launch_bounds__(PD_THREADS, 3) paged_decode_kernel(const __gri
         }
       // Word i of a V piece holds dims 8 g + 2 i, + 1: the low halves of two keys form the B fragment of the column tile "even dims of
       // word i", the high halves that of "odd dims of word i".
+      auto weigh = [&](const float (&pr)[NT][2 * NR], const uint4 (&vv)[KB][RD][4]) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        uint32_t pa[4] = {pack_bf16x2(s[2 * kb][0], s[2 * kb][1]), 0u, pack_bf16x2(s[2 * kb + 1][0], s[2 * kb + 1][1]), 0u};
-        if (NR > 1) pa[1] = pack_bf16x2(s[2 * kb][2 * NR - 2], s[2 * kb][2 * NR - 1]), pa[3] = pack_bf16x2(s[2 * kb + 1][2 * NR - 2], s[2 * kb + 1][2 * NR - 1]);
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t pa[4] = {pack_bf16x2(pr[2 * kb][0], pr[2 * kb][1]), 0u, pack_bf16x2(pr[2 * kb + 1][0], pr[2 * kb + 1][1]), 0u};
+          if (NR > 1) pa[1] = pack_bf16x2(pr[2 * kb][2 * NR - 2], pr[2 * kb][2 * NR - 1]), pa[3] = pack_bf16x2(pr[2 * kb + 1][2 * NR - 2], pr[2 * kb + 1][2 * NR - 1]);
 #pragma unroll
-        for (int rd = 0; rd < RD; ++rd) {
-          const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][0]);
-          const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][1]);
-          const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][2]);
-          const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][3]);
+          for (int rd = 0; rd < RD; ++rd) {
+            const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][0]);
+            const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][1]);
+            const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][2]);
+            const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vv[kb][rd][3]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            pd_mma(oe[rd][i], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w2[i], w3[i], 0x5410));
-            pd_mma(oo[rd][i], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x7632));
+            for (int i = 0; i < 4; ++i) {
+              pd_mma(oe[rd][i], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w2[i], w3[i], 0x5410));
+              pd_mma(oo[rd][i], pa[0], pa[1], pa[2], pa[3], __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x7632));
+            }
           }
         }
+      };
+      bool odd_unit = false;
+      if (EDGE && fresh > 1) {
+        // Values that some rows do not see: a probability of zero does not keep one that is not finite out of a product.  Such ones are cleared ...
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k0 + kb * 16 + 2 * t + (i & 1) + (i >> 1) * 8 >= open)
+#pragma unroll
+              for (int rd = 0; rd < RD; ++rd) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&vv[kb][rd][i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t odd = pd_odd(w[e]);
+                  odd_unit |= odd != 0;
+                  w[e] &= ~((odd >> 15) * 0xffffu);
+                }
+              }
+        odd_unit = __any_sync(0xffffffffu, odd_unit);
       }
+      weigh(s, vv);
+      if (EDGE && odd_unit) {
+        // ... and added by the rows that do see them
+#pragma unroll 1
+        for (int k = max(open - k0, 0); k < min(keys - k0, UNIT); ++k)
+#pragma unroll
+          for (int rd = 0; rd < RD; ++rd)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint4 piece16 = pd_lds(smem_u32(ring) + stage * PD_UNIT_BYTES + PD_UNIT_BYTES / 2 + (rd * UNIT + k) * 128 + (((2 * t + e) ^ (k & 7)) << 4));
+              const uint32_t w[4] = {piece16.x, piece16.y, piece16.z, piece16.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t odd = pd_odd(w[i]);
+                const float2 f = unpack_bf16x2(w[i]);
+#pragma unroll
+                for (int x = 0; x < NR; ++x)
+                  if (k0 + k <= last[x]) {
+                    if (odd & 0x8000u) oe[rd][i][2 * x + e] += f.x;
+                    if (odd & 0x80000000u) oo[rd][i][2 * x + e] += f.y;
+                  }
+              }
+            }
+      }
+    };
+#pragma unroll 1
+    for (int u = 0; u < count; ++u, ++done) {
+      const uint32_t stage = done % PD_STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], (done / PD_STAGES) & 1, &s_abort, p.status, kTimeoutFull))) {
+        const uint64_t t0 = globaltimer_ns();   // copies that were issued land before the warp gives its shared memory back
+        while (globaltimer_ns() - t0 < 10000000ull) {
+        }
+        return;
+      }
+      const int k0 = (u0 + u) * UNIT;
+      if (k0 + UNIT > open) unit(PdBool<true>{}, k0, stage);
+      else unit(PdBool<false>{}, k0, stage);
       __syncwarp();   // the stage has been read
       if (asked < n_mine) request();
     }
@@ -462,6 +526,7 @@ static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
 
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
+  constexpr int PD_STAGES = pd_stages(NR), PD_SMEM = 1024 + PD_WARPS * PD_STAGES * PD_UNIT_BYTES;
   static DeviceOnce once;
   cudaError_t ce = once.smem(paged_decode_kernel<D, NR>, PD_SMEM);
   if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
@@ -472,10 +537,11 @@ static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, con
   return int(cudaGetLastError());
 }
 
-// Warps of the main launch for up to `keys` keys in each of R rows: three CTAs an SM, but no more warps than there are units.
-static int paged_decode_warps(int R, int n_kv, int D, long long keys) {
+// Warps of the main launch for up to `keys` keys in each of R rows: as many as run at once, but no more than there are units.
+static int paged_decode_warps(int R, int n_kv, int D, long long keys, int limit) {
+  const int most = 148 * pd_ctas(limit > 8 ? 2 : 1) * PD_WARPS;
   const long long units = (keys + 2048 / D - 1) / (2048 / D) * R * n_kv;
-  return int(units < 1 ? 1 : units > 444 * PD_WARPS ? 444 * PD_WARPS : units);
+  return int(units < 1 ? 1 : units > most ? most : units);
 }
 
 }  // namespace ats
@@ -484,7 +550,7 @@ using namespace ats;
 
 // Bytes of scratch that `ats_paged_decode` needs (16-byte aligned).
 ATS_API long long ats_paged_decode_scratch(int R, int n_kv, int D, long long max_keys, int limit) {
-  return (R + 4ll) / 4 * 16 + 2ll * paged_decode_warps(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
+  return (R + 4ll) / 4 * 16 + 2ll * paged_decode_warps(R, n_kv, D, max_keys, limit) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
 }
 
 // Rows whose new tokens times n_q / n_kv are at most `limit` (8 or 16).  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens
@@ -508,7 +574,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys, limit); p.zero_tail = zero_tail;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.line = static_cast<uint32_t*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);

@@ -181,6 +181,45 @@ def test_attention_borders(old, new, n_q, n_kv, d):
     _attend_case(old, new, 64, n_q, n_kv, d, torch.bfloat16, scale=0.3)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n_q,n_kv,d", [(32, 4, 64), (6, 2, 128), (8, 8, 128), (16, 1, 64)])
+@pytest.mark.parametrize("old,new,odd", [([100, 9], [4, 1], [102, 3]), ([0, 0], [2, 2], [1, 0]), ([0, 300], [400, 200], [130, 333]), ([0, 50], [129, 64], [128, 51]), ([700], [300], [900])])
+def test_attention_values_that_are_not_finite_reach_no_token_before_their_own(old, new, odd, n_q, n_kv, d, dtype):
+    """Row r's token odd[r] holds an infinity in one column of its first head and nothing but NaN in its last head, and the keys behind it are NaN."""
+    plan, pages = make_plan(old, new, 16, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(d)
+    k, v = (torch.randn(pages, 16, n_kv, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn(sum(new), n_q, d, generator=g, device="cuda").to(dtype)
+    plan.max_new, plan.max_len = max(new), max(o + n for o, n in zip(old, new))
+    ref, mass = attend64(q, k, v, plan, 1 / math.sqrt(d))
+    at = [int(plan.tables[r, t // 16]) * 16 + t % 16 for r, t in enumerate(odd)]
+    late = [[int(plan.tables[r, t // 16]) * 16 + t % 16 for t in range(odd[r] + 1, old[r] + new[r])] for r in range(len(old))]
+    kept = k.clone()
+    v.view(-1, n_kv, d)[at, 0, 5] = float("inf")
+    v.view(-1, n_kv, d)[at, n_kv - 1] = float("nan")
+    for rows in late:
+        k.view(-1, n_kv, d)[rows] = float("nan")
+    out = ops.paged_attention(q, k, v, plan)
+    bound = _attention_bound(dtype, ref, mass, plan.max_len, d)
+    rep = n_q // n_kv
+    for r, (o, n) in enumerate(zip(old, new)):
+        a = int(plan.starts[r])
+        for i in range(n):
+            err = (out[a + i].double() - ref[a + i]).abs()
+            if o + i < odd[r]:
+                assert bool((err <= bound[a + i]).all()), (r, i)
+            elif o + i > odd[r] and odd[r] + 1 < o + n:
+                assert out[a + i].isnan().all(), (r, i)      # a key that is NaN
+            else:
+                first, last = out[a + i, :rep], out[a + i, (n_kv - 1) * rep:]
+                assert last.isnan().all()
+                if n_kv > 1:
+                    assert (first[:, 5] == float("inf")).all()
+                    cols = [c for c in range(d) if c != 5]
+                    assert bool((err[:rep][:, cols] <= bound[a + i, :rep][:, cols]).all())
+    assert not torch.equal(k, kept) or all(len(x) == 0 for x in late)
+
+
 def test_attention_fp32_portion():
     _attend_case([0, 50], [90, 33], 16, 6, 2, 128, torch.float32, tail=3)
 
