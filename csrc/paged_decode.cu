@@ -18,11 +18,11 @@ namespace ats {
 
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS;
 constexpr int PD_UNIT_BYTES = 8192;
-// Eight MMA rows leave registers for three CTAs of four warps an SM with a ring of two units each; sixteen (twice the sums and queries) for two with three
-// (8 rows of 5,000 to 31,000 keys, four tokens each: 92 us, with three CTAs and spilled registers 100): 192 KB in flight either way.
-__host__ __device__ constexpr int pd_ctas(int nr) { return nr > 1 ? 2 : 3; }
-__host__ __device__ constexpr int pd_stages(int nr) { return nr > 1 ? 3 : 2; }
-
+// Two CTAs of four warps an SM with a ring of three units each, against three with a ring of two (192 KB in flight either way): 64 rows x 4 key heads of 64,
+// 200 to 2,000 keys 21.3 / 24.1 us, one row of 60,000 x 8 of 128 56 / 67 (fewer slots to join), 64 rows x 8 of 128, 2,000 keys 94.7 / 93.8, 128 x 4 of 64,
+// 100 to 4,000 55.5 / 54.1; with sixteen MMA rows (twice the sums and queries in registers) 8 rows of 5,000 to 31,000 keys 92 / 100.
+constexpr int PD_CTAS = 2, PD_STAGES = 3;
+constexpr int PD_SMEM = 1024 + PD_WARPS * PD_STAGES * PD_UNIT_BYTES;
 
 struct PagedDecodeArgs {
   PagedRows rows;
@@ -91,9 +91,8 @@ struct PdShares {
 };
 
 template <int D, int NR>  // NR: sets of eight MMA rows (1 or 2)
-__global__ void __launch_bounds__(PD_THREADS, pd_ctas(NR)) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(PD_THREADS, PD_CTAS) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                      const PagedDecodeArgs p) {
-  constexpr int PD_STAGES = pd_stages(NR);
   constexpr int UNIT = 2048 / D, NT = UNIT / 8, KB = UNIT / 16, JD = D / 32, RD = D / 64, ROWS = 8 * NR;
   extern __shared__ uint8_t pd_smem[];
   __shared__ uint64_t s_full[PD_WARPS][PD_STAGES];
@@ -526,7 +525,6 @@ static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
 
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
-  constexpr int PD_STAGES = pd_stages(NR), PD_SMEM = 1024 + PD_WARPS * PD_STAGES * PD_UNIT_BYTES;
   static DeviceOnce once;
   cudaError_t ce = once.smem(paged_decode_kernel<D, NR>, PD_SMEM);
   if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
@@ -538,8 +536,8 @@ static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, con
 }
 
 // Warps of the main launch for up to `keys` keys in each of R rows: as many as run at once, but no more than there are units.
-static int paged_decode_warps(int R, int n_kv, int D, long long keys, int limit) {
-  const int most = 148 * pd_ctas(limit > 8 ? 2 : 1) * PD_WARPS;
+static int paged_decode_warps(int R, int n_kv, int D, long long keys) {
+  const int most = 148 * PD_CTAS * PD_WARPS;
   const long long units = (keys + 2048 / D - 1) / (2048 / D) * R * n_kv;
   return int(units < 1 ? 1 : units > most ? most : units);
 }
@@ -550,7 +548,7 @@ using namespace ats;
 
 // Bytes of scratch that `ats_paged_decode` needs (16-byte aligned).
 ATS_API long long ats_paged_decode_scratch(int R, int n_kv, int D, long long max_keys, int limit) {
-  return (R + 4ll) / 4 * 16 + 2ll * paged_decode_warps(R, n_kv, D, max_keys, limit) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
+  return (R + 4ll) / 4 * 16 + 2ll * paged_decode_warps(R, n_kv, D, max_keys) * (limit > 8 ? 16 : 8) * (D + 2) * 4;
 }
 
 // Rows whose new tokens times n_q / n_kv are at most `limit` (8 or 16).  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens
@@ -574,7 +572,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys, limit); p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.line = static_cast<uint32_t*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);
