@@ -149,10 +149,12 @@ class PagedPool:
         del self.lengths[slot], self.reserved[slot]
         self.slots.free(torch.tensor([slot]))
 
-    def _grow(self, slot: int, n: int) -> None:
-        if self.cache.pool.pages_for(self.lengths[slot] + n) > self.reserved[slot]:
-            raise RuntimeError(f"row {slot} was opened for {self.reserved[slot]} pages and holds {self.lengths[slot]} tokens: no room for {n} more")
-        self.lengths[slot] += n
+    def _grow(self, more: Dict[int, int]) -> None:
+        for slot, n in more.items():
+            if self.cache.pool.pages_for(self.lengths[slot] + n) > self.reserved[slot]:
+                raise RuntimeError(f"row {slot} was opened for {self.reserved[slot]} pages and holds {self.lengths[slot]} tokens: no room for {n} more")
+        for slot, n in more.items():
+            self.lengths[slot] += n
 
     # -- tokens ---------------------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -161,8 +163,7 @@ class PagedPool:
         ids = {slot: torch.as_tensor(part, dtype=torch.long).flatten() for slot, part in portions}
         if len(ids) != len(portions) or not portions or any(t.numel() == 0 for t in ids.values()):
             raise ValueError("portions of at least one token, of different rows, are needed")
-        for slot, part in ids.items():
-            self._grow(slot, part.numel())
+        self._grow({slot: part.numel() for slot, part in ids.items()})
         order = sorted(ids)                                # rows lie in the packed batch in their own order
         fresh = torch.zeros(self.rows, dtype=torch.int32)
         fresh[order] = torch.tensor([ids[s].numel() for s in order], dtype=torch.int32)
@@ -204,8 +205,9 @@ class PagedPool:
     def decode(self, slots: Sequence[int]) -> torch.Tensor:
         """One decode step: every row of ``slots`` feeds its token in ``last`` -> logits [rows, V] (rows outside ``slots`` are meaningless; a static
         buffer that the next step overwrites)."""
-        for s in slots:
-            self._grow(s, 1)
+        if len(set(slots)) != len(slots):
+            raise ValueError("every row decodes one token of a step")
+        self._grow({s: 1 for s in slots})
         if self.use_graph and self._graph is None:
             self._capture()
         if self._live != tuple(slots):

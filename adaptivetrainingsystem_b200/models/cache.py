@@ -91,6 +91,10 @@ class PagedKVCache(SequenceCache):
         self.device_lengths, self.device_positions = (self.step.lengths, self.step.positions) if single else (None, None)
         return self.step
 
+    def reset(self) -> None:
+        fresh = torch.full((self.batch,), -1, dtype=torch.int32, device=self.device)
+        self.plan(fresh, 0)
+
     def advance(self, n: int) -> None:
         pass   # the plan moves the rows on
 

@@ -274,7 +274,8 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
     """qkv [T, (n_q + 2 n_kv) d], the packed projection of a step's new tokens -> queries [T, n_q, d]; keys and values go to ``plan.slots``
     of ``k_pages`` / ``v_pages`` [pages, page_size, n_kv, d] (slot -1: nowhere).  Queries and keys are rotated at ``plan.positions`` with the
     tables ``cos`` / ``sin`` [max position, d / 2] fp32 (halves of a head, d a multiple of 16); with ``cos`` = ``None`` they are rotated already and the
-    queries are a view of ``qkv``."""
+    queries are a view of ``qkv``.  No two tokens of a step have the same slot (a plan's never have).  A slot outside the pages or a position behind the
+    tables is reported by ``ops.check_status``, and nothing of that token is written.  For serving: no gradients."""
     T = qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * d:
         raise ValueError(f"qkv: [tokens, {(n_q + 2 * n_kv) * d}] is needed")
@@ -325,7 +326,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, n_q, d], a step's queries (rotated; rows may be views of a wider projection) -> [T, n_q, d].  Token i of a row's new tokens attends to the
     row's tokens up to itself, in the pages of ``plan.tables``; its keys and values are there already.  ``scale`` (default 1 / sqrt(d)) times the scores.
-    Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given.  Heads of up to 256 dimensions (multiples of 8)."""
+    Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given.  Heads of up to 256 dimensions (multiples of 8).
+    A table entry outside the pool is reported by ``ops.check_status`` and reads as zeros.  bf16: scores, statistics and sums in fp32, probabilities rounded to
+    bf16 for their product with the values; fp32 in true 32-bit.  For serving: no gradients."""
     if q.dim() != 3:
         raise ValueError("q: [tokens, heads, d] is needed")
     pages, ps, n_kv, d = _check_pages(k_pages, v_pages, plan, q)
@@ -353,7 +356,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status, stream = _p(_lib.status_tensor(device)), _stream(device)
     head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
     with _on(device):
-        if q.dtype != torch.bfloat16 or d not in (64, 128) or ps < 8 or rep > 128 or (keys // 16 + 1) * R * n_kv >= 1 << 31:
+        if q.dtype != torch.bfloat16 or d not in (64, 128) or ps < 8 or rep > 128 or (width * ps // 16 + 1) * R * n_kv >= 1 << 32:
             _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
             return out
         # Rows of a few query rows (new tokens times heads of a group) are a stream of the cache, longer portions a matter of the tensor cores.  A batch may

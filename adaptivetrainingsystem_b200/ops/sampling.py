@@ -14,7 +14,7 @@ import torch
 from . import _lib
 from .paged import _fn, _need, _on, _p, _stream
 
-MAX_VOCAB = 1 << 20
+MAX_ROWS, MAX_VOCAB = 65535, 1 << 20
 PerRow = Union[int, float, torch.Tensor]
 
 
@@ -37,6 +37,7 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature: PerRow
     of nothing but -infinity gives its first token."""
     _need(logits.dim() == 2 and logits.shape[1] >= 1 and logits.shape[1] <= MAX_VOCAB, f"logits: [rows, vocabulary], at most {MAX_VOCAB} wide")
     B, V = logits.shape
+    _need(B <= MAX_ROWS, "at most 65535 rows")
     _need(isinstance(uniform, torch.Tensor) and uniform.shape == (B,) and uniform.device == logits.device, "uniform: one number per row on the logits' device")
     if history is not None:
         _need(history.dim() == 2 and history.shape[0] == B and history.dtype == torch.int64 and history.device == logits.device,

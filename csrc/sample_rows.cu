@@ -16,7 +16,7 @@
 // tokens are counted by how far below the largest they lie (4,095 bins over the 30.5 T that have any mass, and one for the rest), which brackets a
 // cut between two bins; only the tokens of the bracket are collected, sorted and cut exactly.
 //   top-k           the largest of every eight tokens is counted: k of these above a bin mean k tokens above it, and the tokens from there up are a
-//                   little more than k.  They are all that is kept, so nothing but these few needs an exponential.
+//                   little more than k (k above half of the eights: all tokens are counted).  They are all that is kept, so nothing but these few needs an exponential.
 //   top-p alone     one pass for the masses' sum and the counts; the counts bound the cumulative mass to a bin's width (0.75 %) from either side, the
 //                   bracket is what lies between; a second pass sums what is above it, and if the bracket holds too many tokens still, its own sum
 //                   is now uncertain by 0.75 % only: the next bracket is a hundredth of it.
@@ -517,16 +517,25 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   };
 
   if (by_k && !bisect) {
-    // ---- counts of the largest of every eight tokens, eight bins in one
+    // ---- counts of the largest of every eight tokens (of all tokens where k is more than half of the eights), eight bins in one
     constexpr int WIDE = SR_BINS / SR_THREADS;
+    const bool all_tokens = top_k > V / 16;
     for (int g = tid; g < groups; g += SR_THREADS) {
       float x[8];
       load8(g, x);
-      float m = x[0];
+      if (all_tokens) {
 #pragma unroll
-      for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
-      const int bin = bin_of(m);
-      if (bin < SR_BINS - 1) atomicAdd(&hist[bin / WIDE], 1u);
+        for (int e = 0; e < 8; ++e) {
+          const int bin = bin_of(x[e]);
+          if (bin < SR_BINS - 1) atomicAdd(&hist[bin / WIDE], 1u);
+        }
+      } else {
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
+        const int bin = bin_of(m);
+        if (bin < SR_BINS - 1) atomicAdd(&hist[bin / WIDE], 1u);
+      }
     }
     csync();
     uint32_t c = 0, all;

@@ -372,6 +372,18 @@ def test_sample_rows_extreme_numbers(dtype):
     _sample_case(B, V, dtype, 11, numbers=numbers, scores=x)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [270001, 1000003, 1 << 20])
+def test_sample_rows_large_vocabularies(V, dtype):
+    """Slices that stay in shared memory and such that do not fit; the last token of the largest vocabulary can be drawn."""
+    _sample_case(10, V, dtype, seed=V)
+    x = torch.zeros(2, V, device="cuda", dtype=dtype)
+    x[:, -1] = 60.0
+    u = torch.tensor([0.0, 0.999], device="cuda")
+    for k in (0, 1, 40):
+        assert ops.sample_rows(x, u, 1.0, k, 0.9).tolist() == [V - 1, V - 1]
+
+
 def test_sample_rows_draws_by_mass():
     """20,000 evenly spaced numbers over ten tokens: every token is named as often as its probability says, but for one at either border."""
     n = 20000

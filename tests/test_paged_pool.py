@@ -62,10 +62,20 @@ def test_pool_refusals():
         pool.open(17)
     with pytest.raises(RuntimeError, match="no room"):
         pool.extend(a, torch.zeros(25, dtype=torch.long))
+    b = pool.open(2)
+    pool.extend_many([(a, [1] * 17), (b, [1])])
+    with pytest.raises(RuntimeError, match="no room"):
+        pool.extend_many([(b, [1]), (a, [1] * 9)])
+    assert pool.lengths == {a: 17, b: 1}      # nothing of a refused step has happened
+    with pytest.raises(ValueError, match="one token"):
+        pool.decode([b, b])
+    pool.close(b)
     with pytest.raises(ValueError, match="different rows"):
         pool.extend_many([(a, [1]), (a, [2])])
     with pytest.raises(ValueError, match="at least one token"):
         pool.extend_many([(a, [])])
+    pool.cache.reset()
+    assert pool.cache.pool.lengths.tolist() == [0, 0] and int(pool.cache.pool.state[0]) == 5
     with pytest.raises(ValueError, match="power of two"):
         PagedPool(model, 2, 32, page_size=12)
     with pytest.raises(ValueError, match="Mixture-of-Depths"):
