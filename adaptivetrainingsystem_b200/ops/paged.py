@@ -20,7 +20,6 @@ import contextlib
 import ctypes
 import functools
 import math
-from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -118,23 +117,26 @@ class PagePool:
             raise RuntimeError(f"the step was refused: {_REFUSED.get(code, code)}")
 
 
-@dataclass
 class PagePlan:
-    """What the operators of one step read.  ``max_new`` / ``max_len``: the longest portion and the longest row of the step as far as the host
-    knows them (upper bounds that choose kernels and grids; by default the packed batch and the tables' width)."""
-    starts: torch.Tensor            # int32 [rows + 1]: row r's new tokens are packed at starts[r] .. starts[r + 1]
-    slots: torch.Tensor             # int32 [tokens], -1: no row's token
-    positions: torch.Tensor         # int32 [tokens]
-    lengths: torch.Tensor           # int32 [rows]: tokens of the row, the new ones among them
-    tables: torch.Tensor            # int32 [rows, width]
-    page_size: int
-    max_new: Optional[int] = None
-    max_len: Optional[int] = None
-    info: Optional[torch.Tensor] = None   # int32 [2]: free pages after the step, refusal code
+    """What the operators of one step read:
+
+    * ``starts`` int32 [rows + 1]: row r's new tokens are packed at starts[r] .. starts[r + 1];
+    * ``slots``, ``positions`` int32 [tokens] (slot -1: no row's token);
+    * ``lengths`` int32 [rows]: tokens of the row, the new ones among them;
+    * ``tables`` int32 [rows, width], ``page_size``;
+    * ``max_new`` / ``max_len``: the longest portion and the longest row of the step as far as the host knows them (upper bounds that choose kernels and
+      grids; by default the packed batch and the tables' width);
+    * ``info`` int32 [2]: free pages after the step, refusal code."""
+
+    def __init__(self, starts: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor, tables: torch.Tensor, page_size: int,
+                 max_new: Optional[int] = None, max_len: Optional[int] = None, info: Optional[torch.Tensor] = None):
+        # (_good: the tokens and the device that the tensors have been checked for)
+        self.__dict__.update(starts=starts, slots=slots, positions=positions, lengths=lengths, tables=tables, page_size=page_size, max_new=max_new, max_len=max_len,
+                             info=info, _good=None)
 
     def __setattr__(self, name, value):
-        object.__setattr__(self, name, value)
-        object.__setattr__(self, "_good", None)   # (tokens, device) that the tensors have been checked for
+        self.__dict__[name] = value
+        self.__dict__["_good"] = None
 
     @property
     def count(self) -> torch.Tensor:
@@ -249,7 +251,7 @@ def _check_plan(plan: PagePlan, T: int, device: torch.device) -> None:
     _ints(plan.starts, "plan.starts", (R + 1,), device)
     _ints(plan.slots, "plan.slots", (T,), device)
     _ints(plan.positions, "plan.positions", (T,), device)
-    object.__setattr__(plan, "_good", (T, device))
+    plan.__dict__["_good"] = (T, device)
 
 
 def _kernel_type(t: torch.Tensor, d: int) -> None:
