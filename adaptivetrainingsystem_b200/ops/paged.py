@@ -235,6 +235,10 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, l
     if not (k_pages.dtype == v_pages.dtype == like.dtype and k_pages.device == v_pages.device == device):
         raise ValueError("pages and tokens: one type, one device")
     pages, ps, n_kv, d = k_pages.shape
+    if not (pages and n_kv and d):
+        raise ValueError("pages without tokens, heads or columns")
+    if (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError("k_pages, v_pages: they have to begin at a multiple of 16 bytes")
     if pages * ps > MAX_SLOTS:
         raise ValueError("slots have to stay below 2^31 - 256")
     if plan._good != (like.shape[0], device):
@@ -288,6 +292,7 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
         _need(sin is not None and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d // 2 and cos.dtype == sin.dtype == torch.float32
               and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == qkv.device and (d % 16 == 0 or not qkv.is_cuda and d % 2 == 0),
               "cos, sin: contiguous float32 tables [positions, d / 2] on the projection's device, d a multiple of 16")
+        _need((cos.data_ptr() | sin.data_ptr()) % 16 == 0, "cos, sin: they have to begin at a multiple of 16 bytes")
     if not qkv.is_cuda:
         return _paged_append_reference(qkv, cos, sin, plan, k_pages, v_pages, n_q, n_kv, d)
     _kernel_type(qkv, d)
@@ -328,8 +333,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, n_q, d], a step's queries (rotated; rows may be views of a wider projection) -> [T, n_q, d].  Token i of a row's new tokens attends to the
     row's tokens up to itself, in the pages of ``plan.tables``; its keys and values are there already.  ``scale`` (default 1 / sqrt(d)) times the scores.
-    Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given.  Heads of up to 256 dimensions (multiples of 8).
-    A table entry outside the pool is reported by ``ops.check_status`` and reads as zeros.  bf16: scores, statistics and sums in fp32, probabilities rounded to
+    Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given (``q`` itself may be: answers replace their queries).  Heads of up to 256 dimensions (multiples of 8).
+    A table entry outside the pool is reported by ``ops.check_status`` and nothing is read there (what its row gets has no meaning).  bf16: scores, statistics and sums in fp32, probabilities rounded to
     bf16 for their product with the values; fp32 in true 32-bit.  For serving: no gradients."""
     if q.dim() != 3:
         raise ValueError("q: [tokens, heads, d] is needed")
@@ -340,8 +345,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _need(scale > 0 and math.isfinite(scale), "scale: a positive number")
     if out is not None:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and (T == 0 or _rows_of(out) is out),
-              "out: like q, rows of contiguous heads that start at multiples of 16 bytes")
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and (T == 0 or _rows_of(out) is out) and (T < 2 or out.stride(0) >= n_q * d),
+              "out: like q, rows of contiguous heads that start at multiples of 16 bytes and do not overlap")
     if not q.is_cuda:
         return _paged_attention_reference(q, k_pages, v_pages, plan, scale, out)
     _kernel_type(q, d)

@@ -21,7 +21,9 @@ PerRow = Union[int, float, torch.Tensor]
 def _numbers(value: PerRow, dtype: torch.dtype):
     """-> (tensor [B] or None, number)."""
     if not isinstance(value, torch.Tensor):
-        return None, (int if dtype == torch.int32 else float)(value)
+        return None, min(max(int(value), 0), MAX_VOCAB) if dtype == torch.int32 else float(value)
+    if dtype == torch.int32 and value.dtype != dtype:
+        value = value.clamp(0, MAX_VOCAB)   # (64-bit numbers keep their meaning)
     return (value if value.dtype == dtype and value.is_contiguous() else value.to(dtype).contiguous()), 0
 
 

@@ -392,3 +392,25 @@ def test_sample_rows_draws_by_mass():
     f = torch.bincount(ops.sample_rows(x, u), minlength=10).double() / n
     p = torch.softmax(x[0].double(), 0)
     assert ((f - p).abs() <= 2 / n).all()
+
+
+@pytest.mark.parametrize("old,new", [([200, 5, 63], [1, 1, 1]), ([0, 100, 40], [150, 1, 20]), ([6000], [1])])
+@pytest.mark.parametrize("n_q,n_kv,d", [(8, 2, 64), (4, 4, 128), (6, 2, 96)])
+def test_attention_replaces_its_queries(old, new, n_q, n_kv, d):
+    """``out`` may be ``q``: the same numbers, and rows of the batch that belong to no row keep what they hold."""
+    plan, pages = make_plan(old, new, 16, "cuda", tail=2)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(pages, 16, n_kv, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(sum(new) + 2, n_q, d, generator=g, device="cuda").bfloat16()
+    want = ops.paged_attention(q, k, v, plan)
+    tail = q[-2:].clone()
+    assert ops.paged_attention(q, k, v, plan, out=q) is q
+    assert torch.equal(q[:-2], want[:-2]) and torch.equal(q[-2:], tail)
+
+
+def test_sample_rows_takes_any_top_k_on_the_gpu():
+    logits = torch.randn(3, 4000, generator=torch.Generator().manual_seed(0)).cuda()
+    u = torch.tensor([0.2, 0.6, 0.95], device="cuda")
+    everything = ops.sample_rows(logits, u)
+    for k in (4000, 1 << 31, 1 << 40, -5, torch.tensor([1 << 40, -(1 << 40), 0], device="cuda")):
+        assert torch.equal(ops.sample_rows(logits, u, top_k=k), everything)

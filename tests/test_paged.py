@@ -157,3 +157,32 @@ def test_sample_rows_definition():
     hist = torch.randint(-1, V + 3, (B, 9), generator=g)
     got = ops.sample_rows(logits, u, t, k, p, low, pen, hist)
     assert torch.equal(got, sample64(logits, u, t, k, p, low, pen, hist))
+
+
+def test_refusals_of_memory_that_the_kernels_cannot_take():
+    plan, pages = make_plan([3], [2], 4, "cpu")
+    n = pages * 4 * 2 * 16
+    k, odd = torch.zeros(pages, 4, 2, 16), torch.zeros(n + 1)[1:].view(pages, 4, 2, 16)   # four bytes behind a multiple of sixteen
+    q = torch.zeros(2, 4, 16)
+    for a, b in ((k, odd), (odd, k)):
+        with pytest.raises(ValueError, match="16 bytes"):
+            ops.paged_attention(q, a, b, plan)
+        with pytest.raises(ValueError, match="16 bytes"):
+            ops.paged_append(torch.zeros(2, 128), None, None, plan, a, b, 4, 2, 16)
+    cos, sin = ops.rope_tables(32, 16, 10000.0)
+    late = torch.zeros(sin.numel() + 1)[1:].view_as(sin)
+    with pytest.raises(ValueError, match="cos, sin"):
+        ops.paged_append(torch.zeros(2, 128), cos, late, plan, k, k.clone(), 4, 2, 16)
+    for out in (torch.zeros(1, 4, 16).expand(2, 4, 16), torch.zeros(3 * 64).as_strided((2, 4, 16), (32, 16, 1))):   # tokens whose answers lie on one another
+        with pytest.raises(ValueError, match="out"):
+            ops.paged_attention(q, k, k, plan, out=out)
+    with pytest.raises(ValueError, match="without"):
+        ops.paged_attention(torch.zeros(2, 0, 16), k[:, :, :0], k[:, :, :0], plan)
+
+
+def test_sample_rows_takes_any_top_k():
+    logits = torch.randn(3, 40, generator=torch.Generator().manual_seed(0))
+    u = torch.tensor([0.2, 0.6, 0.95])
+    everything = ops.sample_rows(logits, u)
+    for k in (40, 1 << 31, 1 << 40, -5, torch.tensor([1 << 40, -(1 << 40), 0])):
+        assert torch.equal(ops.sample_rows(logits, u, top_k=k), everything)
