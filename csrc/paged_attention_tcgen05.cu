@@ -6,15 +6,19 @@
 // pages are read once for the whole group and short portions fill tiles too.  A CTA works on two tiles that share the K / V stream and
 // ping-pong on the tensor cores, as in gqa_attention_tcgen05.cu: one query row per soft-max thread, P overwrites S in tensor memory and is
 // the A operand of P V, O stays in tensor memory and is rescaled only when the running maximum grows by more than 2^8.
-// Bound by the tensor cores and the exponentials (per block of 128 keys and tile 2 x 128 x 128 x D products, 16,384 exponentials).
+// Bound by the tensor cores, whose operands come from shared memory (both for S, the values for P V), and the exponentials (per block of 128 keys and tile
+// 2 x 128 x 128 x D products, 16,384 exponentials).  32 / 8 heads of 128: 1,000 tokens behind 15,000 (255 GFLOP) 251 us = 1,000 TFLOP/s, 0.6 of the library
+// product's rate; six prompts of 300 to 2,500 tokens (96 GFLOP) 158 us = 610, which counts no product of a block that the diagonal halves and all beginnings and
+// ends of pieces.  Two soft-max threads a row took 180 us for the latter (from 153), products cut to the diagonal's columns 176 (from 164).
 //
 // Rows, portions and caches are of any length, so work is dealt out in key blocks: all (row, key head, pair of tiles), each as long as the keys
-// that its last token sees and PC_PIECE more for its beginning and end, form one line, and each of 148 CTAs takes an equal stretch of it.  The roles of a CTA run through the pieces of
-// the stretch independently, so the loads and the first scores of the next piece overlap the end of this one.  A pair of tiles that CTAs share
-// leaves fp32 sums in scratch slots, joined by a second launch in the order of the line: results do not depend on timing.
+// that its last token sees and PC_PIECE more for its beginning and end, form one line, and each of 148 CTAs takes an equal stretch of it (272 -> 155 us for the
+// six prompts against pairs dealt out by blocks alone).  The roles of a CTA run through the pieces of the stretch independently, so the loads and the first
+// scores of the next piece overlap the end of this one.  A pair of tiles that CTAs share leaves fp32 sums in scratch slots, joined by a second launch in the
+// order of the line: results do not depend on timing.
 // A block on the diagonal, or with the row's last key, holds values that some or all rows of the tiles must not see: a probability of zero does not
 // keep a NaN or an infinity out of a product.  Two warps of their own clear such values in shared memory before the product (those that no row
-// sees altogether), and a query that does see them adds them to its output at the end.
+// sees altogether), and a query that does see them adds them to its output at the end; 5 us of the six prompts'.
 // Every wait is bounded (status word + clean unwind); no load uses cluster multicast.
 #include "paged_common.cuh"
 
