@@ -35,7 +35,9 @@ constexpr int SR_MASS_BITS = 42;
 constexpr int SR_MAX_VOCAB = 1 << 20;
 constexpr int SR_BINS = 4096;          // the last one: no mass
 constexpr float SR_RANGE = 30.5f;      // in units of T: exp(-30.49) 2^42 rounds to nothing
+constexpr int SR_MASS_BINS = SR_BINS / 2;
 constexpr int SR_LIST = 2048;
+static_assert(SR_LIST >= SR_MASS_BINS);
 constexpr int SR_MAX_K = 1024;
 constexpr int SR_FEW = SR_THREADS / 2;
 constexpr int SR_CHUNK = 256;
@@ -155,17 +157,17 @@ template <typename T>
 __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const SampleRowsArgs p) {
   pdl_prologue();
   extern __shared__ __align__(16) uint8_t sr_smem[];
-  __shared__ uint64_t red[SR_WARPS], s_top, s_sum[2], s_cut;
-  __shared__ double red_d[SR_WARPS], s_table[32];
+  __shared__ uint64_t red[SR_WARPS], s_range[SR_WARPS], s_top, s_sum[2], s_cut;
+  __shared__ double s_table[32];
   __shared__ uint32_t red_u[SR_WARPS], s_count, s_found, s_base;   // tokens of the bracket: this CTA's, the cluster's (rank 0), in front of this CTA's
-  __shared__ int s_bracket[3];
+  __shared__ int s_bracket[2], s_place;
+  __shared__ uint32_t s_few;
   constexpr int PER = 16 / sizeof(T);
   const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, groups = p.slice / 8;
   const SampleRowsSmem<T> at(p.slice, p.cached);
   uint32_t* hist = reinterpret_cast<uint32_t*>(sr_smem + at.hist);
   uint64_t* near = reinterpret_cast<uint64_t*>(sr_smem + at.hist);
   uint64_t* list = reinterpret_cast<uint64_t*>(sr_smem + at.list);
-  uint32_t* counts = reinterpret_cast<uint32_t*>(sr_smem + at.list);
   uint64_t* chunks = reinterpret_cast<uint64_t*>(sr_smem + at.chunks);
   uint32_t* seen = reinterpret_cast<uint32_t*>(sr_smem + at.seen);
   T* raw = reinterpret_cast<T*>(sr_smem + at.raw);
@@ -321,35 +323,21 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     csync();   // everybody has read: a list that holds all that is kept needs no other CTA any more
     return found;
   };
-  // what is kept, per SR_CHUNK consecutive tokens (one group a lane): `kept(x, j)` says whether the token is, as far as its mass does not.  -> the mass
-  // of these before min-p, this thread's share
-  auto sum_chunks = [&](auto kept, bool add) -> uint64_t {   // (add: to the sums that are there)
-    uint64_t all = 0;
+  // what is kept, per SR_CHUNK consecutive tokens (one group a lane): `kept(x, j)` says whether the token is, as far as min-p does not
+  auto sum_chunks = [&](auto kept) {
     for (int g = tid; g < groups; g += SR_THREADS) {
       float x[8];
       load8(g, x);
       uint64_t v = 0;
-      if (low > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double w = weight(x[e]);
-          const uint64_t m = kept(x[e], 8 * g + e) ? fixed(w) : 0;
-          all += m;
-          v += w >= low ? m : 0;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint64_t m = fixed(weight(x[e]));
-          v += kept(x[e], 8 * g + e) ? m : 0;
-        }
-        all += v;
+      for (int e = 0; e < 8; ++e) {
+        const double w = weight(x[e]);
+        v += kept(x[e], 8 * g + e) && !(w < low) ? fixed(w) : 0;
       }
       v = sr_warp_sum(v);
-      if (lane == 0) chunks[g >> 5] = add ? chunks[g >> 5] + v : v;
+      if (lane == 0) chunks[g >> 5] = v;
     }
     __syncthreads();
-    return all;
   };
 
   const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.f;
@@ -360,7 +348,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
   }
   bool bisect = by_k && top_k > SR_MAX_K, listed = false;   // listed: the answer is among the list's tokens
   int b_lo = 0;
-  uint64_t cut = 0, z = 0, above = 0;   // tokens with at least the key `cut` are kept
+  uint64_t cut = 0, z = 0, above = 0, own_kept = 0;   // tokens with at least the key `cut` are kept; this CTA's mass of them
   // rank 0, with `found` tokens in the list, `above` the mass of what is in front of them: the cut, and the answer if nothing is in front of them
   auto finish_list = [&](uint32_t found) {
     if (found <= SR_FEW) {
@@ -418,104 +406,124 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       if (half == 0 && before <= target && target < before + m) p.out[b] = int(0xffffffffu - uint32_t(k));
       return;
     }
-    constexpr int EACH = SR_LIST / SR_THREADS;   // four consecutive entries a thread
-    uint64_t v[EACH];
-    auto scan = [&](uint64_t mine, uint64_t* all) -> uint64_t { return sr_block_scan<uint64_t>(mine, red, all); };
-    // The entries of all threads, largest first (bitonic; `m` of them are not zero): pairs that lie in a thread or in a warp are exchanged in registers.
-    auto sort = [&](uint32_t m) {
-      uint32_t size = 2;
-      while (size < m) size *= 2;
-      for (uint32_t k = 2; k <= size; k *= 2)
-        for (uint32_t j = k / 2; j > 0; j /= 2) {
-          if (j >= 32 * EACH) {
-            __syncthreads();
+    // More tokens: four a thread, in registers.  A cut is where the cumulative weight in falling order of a key passes a limit; it is found by counting
+    // weights over 512 places of the keys' range, then over the one place that holds the cut, until that holds one token.
+    constexpr int EACH = SR_LIST / SR_THREADS;
+    uint64_t* sums = list;                                                      // [SR_THREADS]
+    uint32_t* many = reinterpret_cast<uint32_t*>(list + SR_THREADS);            // [SR_THREADS]
+    uint64_t v[EACH], w[EACH];
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) list[tid * EACH + e] = v[e];
-            __syncthreads();
-          }
-          if (warp * 32 * EACH >= size) continue;   // (nothing but zeros)
-          if (j >= EACH) {
+    for (int e = 0; e < EACH; ++e) v[e] = tid + e * SR_THREADS < found ? list[tid + e * SR_THREADS] : 0;
+    // the smallest key (of tokens whose key is not 0; they are all different) with at most `limit` of weight in front of it, `run` of which is there already; ~0: none
+    auto narrow = [&](const uint64_t (&key)[EACH], auto weight_at, uint64_t run, auto within) -> uint64_t {
+      uint64_t lo = ~0ull, hi = 0;
 #pragma unroll
-            for (int e = 0; e < EACH; ++e) {
-              const uint32_t i = tid * EACH + e;
-              const uint64_t o = j >= 32 * EACH ? list[i ^ j] : __shfl_xor_sync(0xffffffffu, v[e], j / EACH);
-              const bool larger = ((i & k) == 0) == ((i & j) == 0);   // this place keeps the larger one
-              v[e] = (v[e] > o) == larger ? v[e] : o;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) {
-              const int f = e ^ int(j);
-              if (f > e) {
-                const bool desc = ((tid * EACH + e) & k) == 0;
-                const uint64_t x = v[e], y = j == 1 ? v[e ^ 1] : v[e ^ 2];
-                const bool swap = (x < y) == desc;
-                v[e] = swap ? y : x;
-                if (j == 1) v[e ^ 1] = swap ? x : y;
-                else v[e ^ 2] = swap ? x : y;
-              }
-            }
-          }
-        }
-    };
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) v[e] = tid * EACH + e < found ? list[tid * EACH + e] : 0;
-    sort(found);
-    const uint32_t m = by_k ? min(found, uint32_t(top_k)) : found;
-    uint64_t w[EACH], own = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      w[e] = tid * EACH + e < m ? mass(key_value(uint32_t(v[e] >> 32))) : 0;
-      own += w[e];
-    }
-    uint64_t all, run = scan(own, &all) + above;
-    const double limit = by_p ? double(fmaxf(top_p, 0.f)) * double(by_k ? all : z) : INFINITY;
-    uint64_t last = ~0ull;
-    own = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      // both rules keep a leading run; a token without mass is never the answer
-      if (tid * EACH + e >= m) break;
-      const bool in = double(run) <= limit;
-      run += in ? w[e] : 0;
-      if (in) last = v[e];
-      if (!in || (low > 0 && !(weight(key_value(uint32_t(v[e] >> 32))) >= low))) w[e] = 0;
-      own += w[e];
-    }
-    if (!listed) {   // the smallest key that is kept
+      for (int e = 0; e < EACH; ++e)
+        if (key[e]) lo = key[e] < lo ? key[e] : lo, hi = key[e] > hi ? key[e] : hi;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t u2 = __shfl_xor_sync(0xffffffffu, last, o);
-        last = u2 < last ? u2 : last;
+        const uint64_t a = __shfl_xor_sync(0xffffffffu, lo, o), c = __shfl_xor_sync(0xffffffffu, hi, o);
+        lo = a < lo ? a : lo, hi = c > hi ? c : hi;
       }
       __syncthreads();
-      if (lane == 0) red[warp] = last;
+      if (lane == 0) red[warp] = lo, s_range[warp] = hi;
       __syncthreads();
-      if (tid == 0) {
-        for (int i = 1; i < SR_WARPS; ++i) last = red[i] < last ? red[i] : last;
-        s_cut = last;
+#pragma unroll
+      for (int i = 0; i < SR_WARPS; ++i) lo = red[i] < lo ? red[i] : lo, hi = s_range[i] > hi ? s_range[i] : hi;
+      if (hi == 0) return ~0ull;
+      for (;;) {
+        const int shift = max(0, 55 - __clzll((long long)(hi - lo)));   // places of 2^shift keys: at most 512
+        sums[tid] = 0, many[tid] = 0;
+        if (tid == 0) s_place = -1;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+          if (key[e] && key[e] >= lo && key[e] <= hi) {
+            const int at = SR_THREADS - 1 - int((key[e] - lo) >> shift);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sums[at]), (unsigned long long)weight_at(e));
+            atomicAdd(&many[at], 1u);
+          }
+        __syncthreads();
+        uint64_t all;
+        const uint64_t before = run + sr_block_scan<uint64_t>(sums[tid], red, &all);
+        const uint32_t ok = __ballot_sync(0xffffffffu, many[tid] > 0 && within(before));   // (a leading run of the places that hold tokens)
+        if (ok && lane == 31 - __clz(ok)) atomicMax(&s_place, tid);
+        __syncthreads();
+        const int place = s_place;
+        if (place < 0) return ~0ull;
+        if (tid == place) s_sum[0] = before;
+        if (tid == 0) s_few = 0;
+        const uint64_t from = lo + (uint64_t(SR_THREADS - 1 - place) << shift);
+        const uint32_t n = many[place];
+        __syncthreads();
+        if (n <= 32) {   // a warp compares each with all
+#pragma unroll
+          for (int e = 0; e < EACH; ++e)
+            if (key[e] >= from && key[e] <= hi && (key[e] - from) >> shift == 0) {
+              const uint32_t i = atomicAdd(&s_few, 1u);
+              sums[i] = key[e], sums[32 + i] = weight_at(e);
+            }
+          __syncthreads();
+          if (warp == 0) {
+            const uint64_t k = lane < n ? sums[lane] : 0, m = lane < n ? sums[32 + lane] : 0;
+            uint64_t in_front = s_sum[0];
+            for (uint32_t j = 0; j < n; ++j) {
+              const uint64_t k_j = __shfl_sync(0xffffffffu, k, j), m_j = __shfl_sync(0xffffffffu, m, j);
+              in_front += k_j > k ? m_j : 0;
+            }
+            uint64_t best = lane < n && within(in_front) ? k : ~0ull;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+              const uint64_t c = __shfl_xor_sync(0xffffffffu, best, o);
+              best = c < best ? c : best;
+            }
+            if (lane == 0) s_cut = best;
+          }
+          __syncthreads();
+          return s_cut;
+        }
+        run = s_sum[0];
+        const uint64_t to = from + ((1ull << shift) - 1);   // (more than one key: shift is not 0)
+        lo = from, hi = to < hi ? to : hi;
       }
+    };
+    if (!listed) {   // the smallest key that is kept: by_p without by_k
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) w[e] = v[e] ? mass(key_value(uint32_t(v[e] >> 32))) : 0;
+      const double limit = double(fmaxf(top_p, 0.f)) * double(z);
+      const uint64_t last = narrow(v, [&](int e) { return w[e]; }, above, [&](uint64_t before) { return double(before) <= limit; });
+      __syncthreads();
+      if (tid == 0) s_cut = last;
       return;
     }
-    // all that is kept is here: in index order (the index in the upper bits, inverted, the mass in the lower 43), the token whose mass covers the target
-    uint64_t kept;
-    scan(own, &kept);
-    const uint64_t target = target_of(kept);
+    if (by_k && found > uint32_t(top_k)) {
+      const uint64_t last = narrow(v, [](int) { return 1ull; }, 0, [&](uint64_t before) { return before < uint64_t(top_k); });
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) v[e] = w[e] ? (uint64_t(uint32_t(v[e]) & (SR_MAX_VOCAB - 1)) << (SR_MASS_BITS + 1)) | w[e] : 0;
-    sort(m);
+      for (int e = 0; e < EACH; ++e) v[e] = v[e] >= last ? v[e] : 0;
+    }
+    uint64_t own = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      w[e] = v[e] ? mass(key_value(uint32_t(v[e] >> 32))) : 0;
+      own += w[e];
+    }
+    if (by_p) {
+      const uint64_t all = by_k ? sr_block_sum(own, red) : z;
+      const double limit = double(fmaxf(top_p, 0.f)) * double(all);
+      const uint64_t last = narrow(v, [&](int e) { return w[e]; }, 0, [&](uint64_t before) { return double(before) <= limit; });
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) w[e] = v[e] >= last ? w[e] : 0;
+    }
     own = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      w[e] = v[e] & ((2ull << SR_MASS_BITS) - 1);
+      if (low > 0 && w[e] && !(weight(key_value(uint32_t(v[e] >> 32))) >= low)) w[e] = 0;
       own += w[e];
+      v[e] = w[e] ? uint32_t(v[e]) : 0;   // the order of the indices, lowest first
     }
-    run = scan(own, &all);
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      if (run <= target && target < run + w[e]) p.out[b] = (SR_MAX_VOCAB - 1) - int(v[e] >> (SR_MASS_BITS + 1));
-      run += w[e];
-    }
+    const uint64_t target = target_of(sr_block_sum(own, red));
+    const uint64_t drawn = narrow(v, [&](int e) { return w[e]; }, 0, [&](uint64_t before) { return before <= target; });
+    if (tid == 0) p.out[b] = int(0xffffffffu - uint32_t(drawn));
   };
 
   if (by_k && !bisect) {
@@ -570,100 +578,75 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       return;
     }
   } else if (by_p && !bisect) {
-    // ---- counts of all tokens, and the masses' sum
-    uint64_t v = 0;
+    // ---- masses by distance, two bins in one: lower halves of the sums, then upper ones
+    uint32_t* lower = hist;
+    uint32_t* upper = hist + SR_MASS_BINS;
     for (int g = tid; g < groups; g += SR_THREADS) {
       float x[8];
       load8(g, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int bin = bin_of(x[e]);
-        v += fixed(weight(x[e]));   // (nothing in the last bin)
-        if (bin < SR_BINS - 1) atomicAdd(&hist[bin], 1u);
+        const uint64_t m = fixed(weight(x[e]));
+        if (bin < SR_BINS - 1 && m) {
+          const uint32_t was = atomicAdd(&lower[bin / 2], uint32_t(m)), more = uint32_t(m >> 32) + (was + uint32_t(m) < was);
+          if (more) atomicAdd(&upper[bin / 2], more);
+        }
       }
-    }
-    z = cluster_sum(v, 0);
-    // a share of the bins each, into rank 0's counts
-    for (int i = rank * (SR_BINS / C) + tid; i < (rank + 1) * (SR_BINS / C); i += SR_THREADS) {
-      uint32_t c = 0;
-      for (int r = 0; r < C; ++r) c += sr_ld_u32(&hist[i], r);
-      sr_st_u32(&counts[i], 0, c);
     }
     csync();
-    // ---- the bracket, in rounds: what is above it is summed exactly, which narrows the next one to a bin's width of what is left
-    int done = 0;        // bins that are summed
-    bool last = false;
-    for (int round = 0; !last; ++round) {
-      if (rank == 0) {
-        constexpr int EACH = SR_BINS / SR_THREADS;
-        if (tid == 0) s_bracket[0] = done, s_bracket[1] = SR_BINS - 2;
-        // bounds of the cumulative mass through each bin, in units of the largest mass: a bin's tokens lie within a hundredth of a bin of it, a
-        // mass is rounded by 2^-43, and the sums here by less than a part in 10^9
-        constexpr double width = double(SR_RANGE) / (SR_BINS - 1), unit = 1.0 / double(1ll << SR_MASS_BITS);
-        constexpr double down = 1.0 - width * (1.0 - width / 2 * (1.0 - width / 3 * (1.0 - width / 4)));   // exp(-width), to 2^-44
-        constexpr double wide = 1.0 + 0.021 * width, near_end = 1.0 - 1.021 * width;                       // beyond exp(0.02 width), exp(-1.02 width)
-        const double limit = double(fmaxf(top_p, 0.f)) * double(z) * unit;
-        double most[EACH], least[EACH], own_most = 0, own_least = 0, f = sr_exp_neg(width * (tid * EACH), s_table);
-        uint32_t c[EACH];
+    // a share of the bins each, into rank 0's list
+    for (int i = rank * (SR_MASS_BINS / C) + tid; i < (rank + 1) * (SR_MASS_BINS / C); i += SR_THREADS) {
+      uint64_t v = 0;
+      for (int r = 0; r < C; ++r) v += (uint64_t(sr_ld_u32(&upper[i], r)) << 32) + sr_ld_u32(&lower[i], r);
+      sr_st_u64(&list[i], 0, v);
+    }
+    csync();
+    if (rank == 0) {   // the last bin whose first token is kept holds the cut
+      constexpr int EACH = SR_MASS_BINS / SR_THREADS;
+      uint64_t v[EACH], own = 0, all, before = 0;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int i = tid * EACH + e;
-          c[e] = i < SR_BINS - 1 ? counts[i] : 0;
-          const double n = i >= done ? double(c[e]) : 0.0;
-          most[e] = n * (f * wide + unit);
-          least[e] = n * fmax(f * near_end - unit, 0.0);
-          own_most += most[e];
-          own_least += least[e];
-          f *= down;
-        }
-        double all, run_most = sr_block_scan<double>(own_most, red_d, &all) + double(above) * unit;
-        double run_least = sr_block_scan<double>(own_least, red_d, &all) + double(above) * unit;
+      for (int e = 0; e < EACH; ++e) v[e] = list[tid * EACH + e], own += v[e];
+      uint64_t run = sr_block_scan<uint64_t>(own, red, &all);
+      const double limit = double(fmaxf(top_p, 0.f)) * double(all);
+      int at_bin = -1;
+      uint64_t in_bin = 0;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int i = tid * EACH + e;
-          if (run_most * (1 + 1e-9) <= limit && (run_most + most[e]) * (1 + 1e-9) > limit) s_bracket[0] = i;
-          if (run_least * (1 - 1e-9) <= limit && (run_least + least[e]) * (1 - 1e-9) > limit) s_bracket[1] = i;
-          run_most += most[e], run_least += least[e];
-        }
-        __syncthreads();
-        // does the bracket fit the list, or even all tokens down to its end?
-        const int from = s_bracket[0], to = s_bracket[1];
-        uint64_t both = 0;
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int i = tid * EACH + e;
-          both += i <= to ? uint64_t(c[e]) << 32 | (i >= from ? c[e] : 0u) : 0;
-        }
-        both = sr_block_sum(both, red);
-        const uint32_t n_upto = uint32_t(both >> 32), n_in = uint32_t(both);
-        if (tid == 0) {
-          if (done == 0 && n_upto <= SR_LIST / 4) s_bracket[0] = 0;
-          s_bracket[2] = n_in <= SR_LIST / 2 || from == done || round == 4;   // (the last two: it gets no narrower)
-        }
+      for (int e = 0; e < EACH; ++e) {
+        if (v[e] && double(run) <= limit) at_bin = tid * EACH + e, before = run, in_bin = v[e];
+        run += v[e];
       }
-      csync();
-      b_lo = int(sr_ld_u32(&s_bracket[0], 0));
-      const int b_hi = int(sr_ld_u32(&s_bracket[1], 0));
-      last = b_lo == 0 || sr_ld_u32(&s_bracket[2], 0) != 0;
-      csync();   // the counts have been read: the last round's tokens take their place
-      // sum what is above the bracket, collect its tokens once it is the last
-      uint64_t more = 0;
-      if (b_lo > 0)
-        more = sum_chunks([&](float x, int j) -> bool {
-          const int bin = bin_of(x);
-          if (last && bin >= b_lo && bin <= b_hi) collect(x, j);
-          return bin >= done && bin < b_lo;
-        }, done > 0);
-      else
-        for (int g = tid; g < groups; g += SR_THREADS) {
-          float x[8];
-          load8(g, x);
+      if (tid == 0) s_place = -1;
+      __syncthreads();
+      const uint32_t ok = __ballot_sync(0xffffffffu, at_bin >= 0);
+      if (ok && lane == 31 - __clz(ok)) atomicMax(&s_place, at_bin);
+      __syncthreads();
+      if (at_bin >= 0 && at_bin == s_place) {
+        // all tokens up to the bin's end have at least this mass each (rounding moves a border by less than a hundredth of a bin): do so many fit the list?
+        const double least = sr_exp_neg(double(SR_RANGE) / (SR_BINS - 1) * (2 * at_bin + 2.02), s_table) * double(1ll << SR_MASS_BITS) - 1.0;
+        const bool fit = double(before + in_bin) <= SR_LIST * 0.999 * least;
+        s_bracket[0] = fit ? 0 : 2 * at_bin;
+        s_bracket[1] = min(2 * at_bin + 1, SR_BINS - 2);
+        s_sum[0] = fit ? 0 : before;
+        s_sum[1] = all;
+      }
+    }
+    csync();
+    b_lo = int(sr_ld_u32(&s_bracket[0], 0));
+    const int b_hi = int(sr_ld_u32(&s_bracket[1], 0));
+    above = sr_ld_u64(&s_sum[0], 0);
+    z = sr_ld_u64(&s_sum[1], 0);
+    uint64_t part = 0;
+    for (int i = tid; i < b_lo / 2; i += SR_THREADS) part += (uint64_t(upper[i]) << 32) + lower[i];
+    own_kept = sr_block_sum(part, red);   // (and the counts have been read: the bracket's tokens take their place)
+    for (int g = tid; g < groups; g += SR_THREADS) {
+      float x[8];
+      load8(g, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (bin_of(x[e]) <= b_hi) collect(x[e], 8 * g + e);
-        }
-      above += cluster_sum(more, (round & 1) ^ 1);
-      done = b_lo;
+      for (int e = 0; e < 8; ++e) {
+        const int bin = bin_of(x[e]);
+        if (bin >= b_lo && bin <= b_hi) collect(x[e], 8 * g + e);
+      }
     }
     const uint32_t found = hand_over();
     bisect = found > SR_LIST;
@@ -676,17 +659,16 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       if (rank == 0) finish_list(found);
       csync();
       cut = sr_ld_u64(&s_cut, 0);
-      for (uint32_t i = tid; i < s_count; i += SR_THREADS)   // the bracket's part of what is kept
-        if (near[i] >= cut) {
-          const float x = key_value(uint32_t(near[i] >> 32));
-          const double w = weight(x);
-          if (w >= low) atomicAdd(reinterpret_cast<unsigned long long*>(&chunks[(int(0xffffffffu - uint32_t(near[i])) - i0) / SR_CHUNK]), (unsigned long long)fixed(w));
-        }
-      __syncthreads();
+      part = 0;
+      if (low > 0) sum_chunks([&](float x, int j) -> bool { return key_of(x, j) >= cut; });
+      else
+        for (uint32_t i = tid; i < s_count; i += SR_THREADS)   // the bracket's part of what is kept
+          if (near[i] >= cut) part += mass(key_value(uint32_t(near[i] >> 32)));
+      own_kept += sr_block_sum(part, red);
     }
   }
   {
-    const bool chunked = !bisect && by_p;   // the chunks hold what is kept
+    const bool summed = !bisect && by_p && !(low > 0);   // this CTA's part of what is kept is known, not yet where it lies
     int slot = 0;
     if (bisect) {
       csync();   // the sum last taken may still be read
@@ -724,14 +706,15 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
         cut = lo;
       }
     }
-    const bool cuts = bisect || chunked;
-    auto is_kept = [&](float x, int j) -> bool { return !cuts || (chunked && bin_of(x) < b_lo) || key_of(x, j) >= cut; };
-    if (!cuts) sum_chunks([](float, int) { return true; }, false);
-    else if (bisect) sum_chunks(is_kept, false);
+    const bool cuts = bisect || by_p;
+    auto is_kept = [&](float x, int j) -> bool { return !cuts || key_of(x, j) >= cut; };
+    if (!cuts) sum_chunks([](float, int) { return true; });
+    else if (bisect) sum_chunks(is_kept);
     uint64_t mine = 0;
-    for (int c = tid; c < p.slice / SR_CHUNK; c += SR_THREADS) mine += chunks[c];
+    if (!summed)
+      for (int c = tid; c < p.slice / SR_CHUNK; c += SR_THREADS) mine += chunks[c];
     // (the sums of the CTAs one by one: where the target lies)
-    const uint64_t own = sr_block_sum(mine, red);
+    const uint64_t own = summed ? own_kept : sr_block_sum(mine, red);
     if (tid == 0) s_sum[slot ^ 1] = own;
     csync();
     uint64_t total = 0, before = 0;
@@ -741,7 +724,9 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
       total += v;
     }
     const uint64_t target = target_of(total);
-    if (own > 0 && target >= before && target < before + own && warp == 0) {
+    const bool here = own > 0 && target >= before && target < before + own;
+    if (here && summed) sum_chunks(is_kept);
+    if (here && warp == 0) {
       // one warp: the chunk, 32 at a time, then the group of eight, then the token
       uint64_t run = before;
       auto step = [&](uint64_t v, int* which) -> bool {   // the lane whose value covers the target, or go on behind all of them
