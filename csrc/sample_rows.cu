@@ -14,18 +14,20 @@
 //
 // One cluster per row, a contiguous slice of the vocabulary per CTA, read once into shared memory where it fits.  No sort of the vocabulary:
 // tokens are counted by how far below the largest they lie (4,095 bins over the 30.5 T that have any mass, and one for the rest), which brackets a
-// cut between two bins; only the tokens of the bracket are collected, sorted and cut exactly.
+// cut between two bins; only the tokens of the bracket are collected and cut exactly.
 //   top-k           the largest of every eight tokens is counted: k of these above a bin mean k tokens above it, and the tokens from there up are a
 //                   little more than k (k above half of the eights: all tokens are counted).  They are all that is kept, so nothing but these few needs an exponential.
-//   top-p alone     one pass for the masses' sum and the counts; the counts bound the cumulative mass to a bin's width (0.75 %) from either side, the
-//                   bracket is what lies between; a second pass sums what is above it, and if the bracket holds too many tokens still, its own sum
-//                   is now uncertain by 0.75 % only: the next bracket is a hundredth of it.
+//   top-p alone     one pass sums the masses by distance, exactly (integers, two bins in one), so one bin holds the cut and everything above it is known,
+//                   for the row and for each CTA; the draw then looks into the slice of one CTA.
 //   neither         one pass of masses.
-// Cuts whose brackets do not fit the list (thousands of equal scores, k above 1,024) are found by bisection over the 64-bit order.
+// Up to 256 collected tokens are compared with one another, up to 2,048 are cut by weights counted over 512 places of the keys' range, then over the place that holds
+// the cut (sorting them took 30 us instead of 5).  Cuts whose brackets hold more (thousands of equal scores, k above 1,024) are found by bisection over the 64-bit order.
 // The draw works on sums per 256 consecutive tokens and looks into one of them.
-// Bound by the 64-bit exponentials of rows without top-k (13 FP64 operations a token and pass), else by latency: three to five cluster barriers.  256 x 131,072
-// bf16 (67 MB, 10 us at a copy's rate): greedy 29 us, top-k 50 72, no cut 84, rows of all kinds 170; 64 x 100,003 fp32, all with top-k 33; 4 x 32,000 11.  With
-// the first form, a bisection over the 64-bit order with a pass over the row per step, the last three took 8,146, 2,761 and 543 us.
+// Bound by the exponentials of rows without top-k (13 FP64 operations and 45 others a token), their shared-memory counts (rows of equal scores meet in a bin), else
+// by latency: three to five cluster barriers.  256 x 131,072 bf16 (67 MB, 10 us at a copy's rate): greedy 30 us, top-k 50 66, no cut 88, k = 1,000 119, top-p alone 160 to
+// 290, rows of all kinds 145; 64 x 100,003 fp32, all with top-k 34; 4 x 32,000 11.7.  With bounds from counts alone and a second sum for what they leave open the rows
+// of all kinds took 170 us (top-p alone 154 to 365), with two tokens at a time in the passes with exponentials 158; the first form, a bisection with a pass over the
+// row per step, took 8,146, 2,761 and 543 us.
 #include "common.cuh"
 
 namespace ats {
@@ -66,8 +68,8 @@ template <typename T>
 struct SampleRowsSmem {   // byte offsets of the dynamic shared memory
   int hist, list, chunks, seen, raw, total;
   __host__ __device__ SampleRowsSmem(int slice, bool cached) {
-    hist = 0;                            // u32 [SR_BINS]; later u64 [SR_LIST]: this CTA's tokens of the bracket
-    list = hist + SR_BINS * 4;           // u64 [SR_LIST]: the cluster's tokens of the bracket (rank 0); before that the cluster's counts
+    hist = 0;                            // u32 [SR_BINS], or halves of SR_MASS_BINS masses; later u64 [SR_LIST]: this CTA's tokens of the bracket
+    list = hist + SR_BINS * 4;           // u64 [SR_LIST]: the cluster's tokens of the bracket (rank 0); before that the cluster's masses by distance
     chunks = list + SR_LIST * 8;         // u64 [slice / SR_CHUNK]
     seen = chunks + slice / SR_CHUNK * 8;        // one bit per token of the slice
     raw = (seen + slice / 8 + 15) / 16 * 16;     // the slice
@@ -409,43 +411,52 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     // More tokens: four a thread, in registers.  A cut is where the cumulative weight in falling order of a key passes a limit; it is found by counting
     // weights over 512 places of the keys' range, then over the one place that holds the cut, until that holds one token.
     constexpr int EACH = SR_LIST / SR_THREADS;
-    uint64_t* sums = list;                                                      // [SR_THREADS]
-    uint32_t* many = reinterpret_cast<uint32_t*>(list + SR_THREADS);            // [SR_THREADS]
+    uint32_t* lower = reinterpret_cast<uint32_t*>(list);      // [SR_THREADS] each: halves of the weights' sums, tokens
+    uint32_t* upper = lower + SR_THREADS;
+    uint32_t* many = upper + SR_THREADS;
+    uint64_t* few = list + 2 * SR_THREADS;
     uint64_t v[EACH], w[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) v[e] = tid + e * SR_THREADS < found ? list[tid + e * SR_THREADS] : 0;
     // the smallest key (of tokens whose key is not 0; they are all different) with at most `limit` of weight in front of it, `run` of which is there already; ~0: none
     auto narrow = [&](const uint64_t (&key)[EACH], auto weight_at, uint64_t run, auto within) -> uint64_t {
-      uint64_t lo = ~0ull, hi = 0;
-#pragma unroll
-      for (int e = 0; e < EACH; ++e)
-        if (key[e]) lo = key[e] < lo ? key[e] : lo, hi = key[e] > hi ? key[e] : hi;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t a = __shfl_xor_sync(0xffffffffu, lo, o), c = __shfl_xor_sync(0xffffffffu, hi, o);
-        lo = a < lo ? a : lo, hi = c > hi ? c : hi;
-      }
-      __syncthreads();
-      if (lane == 0) red[warp] = lo, s_range[warp] = hi;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < SR_WARPS; ++i) lo = red[i] < lo ? red[i] : lo, hi = s_range[i] > hi ? s_range[i] : hi;
-      if (hi == 0) return ~0ull;
+      uint64_t lo = 1, hi = ~0ull;
+      uint32_t left = 0;   // (of 0: the range is not known to be a narrow one)
       for (;;) {
+        if (left == 0) {   // the ends of what there is
+          uint64_t first = ~0ull, last = 0;
+#pragma unroll
+          for (int e = 0; e < EACH; ++e)
+            if (key[e] >= lo && key[e] <= hi) first = key[e] < first ? key[e] : first, last = key[e] > last ? key[e] : last;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t a = __shfl_xor_sync(0xffffffffu, first, o), c = __shfl_xor_sync(0xffffffffu, last, o);
+            first = a < first ? a : first, last = c > last ? c : last;
+          }
+          __syncthreads();
+          if (lane == 0) red[warp] = first, s_range[warp] = last;
+          __syncthreads();
+          lo = ~0ull, hi = 0;
+#pragma unroll
+          for (int i = 0; i < SR_WARPS; ++i) lo = red[i] < lo ? red[i] : lo, hi = s_range[i] > hi ? s_range[i] : hi;
+          if (hi == 0) return ~0ull;
+        }
         const int shift = max(0, 55 - __clzll((long long)(hi - lo)));   // places of 2^shift keys: at most 512
-        sums[tid] = 0, many[tid] = 0;
+        lower[tid] = 0, upper[tid] = 0, many[tid] = 0;
         if (tid == 0) s_place = -1;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < EACH; ++e)
           if (key[e] && key[e] >= lo && key[e] <= hi) {
             const int at = SR_THREADS - 1 - int((key[e] - lo) >> shift);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sums[at]), (unsigned long long)weight_at(e));
+            const uint64_t weight = weight_at(e);
+            const uint32_t was = atomicAdd(&lower[at], uint32_t(weight)), more = uint32_t(weight >> 32) + (was + uint32_t(weight) < was);
+            if (more) atomicAdd(&upper[at], more);
             atomicAdd(&many[at], 1u);
           }
         __syncthreads();
         uint64_t all;
-        const uint64_t before = run + sr_block_scan<uint64_t>(sums[tid], red, &all);
+        const uint64_t before = run + sr_block_scan<uint64_t>((uint64_t(upper[tid]) << 32) + lower[tid], red, &all);
         const uint32_t ok = __ballot_sync(0xffffffffu, many[tid] > 0 && within(before));   // (a leading run of the places that hold tokens)
         if (ok && lane == 31 - __clz(ok)) atomicMax(&s_place, tid);
         __syncthreads();
@@ -461,11 +472,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
           for (int e = 0; e < EACH; ++e)
             if (key[e] >= from && key[e] <= hi && (key[e] - from) >> shift == 0) {
               const uint32_t i = atomicAdd(&s_few, 1u);
-              sums[i] = key[e], sums[32 + i] = weight_at(e);
+              few[i] = key[e], few[32 + i] = weight_at(e);
             }
           __syncthreads();
           if (warp == 0) {
-            const uint64_t k = lane < n ? sums[lane] : 0, m = lane < n ? sums[32 + lane] : 0;
+            const uint64_t k = lane < n ? few[lane] : 0, m = lane < n ? few[32 + lane] : 0;
             uint64_t in_front = s_sum[0];
             for (uint32_t j = 0; j < n; ++j) {
               const uint64_t k_j = __shfl_sync(0xffffffffu, k, j), m_j = __shfl_sync(0xffffffffu, m, j);
@@ -485,6 +496,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
         run = s_sum[0];
         const uint64_t to = from + ((1ull << shift) - 1);   // (more than one key: shift is not 0)
         lo = from, hi = to < hi ? to : hi;
+        left = n > found / 2 ? 0 : 1;   // most of them in one place: many equal scores, whose keys differ in the lowest bits alone
       }
     };
     if (!listed) {   // the smallest key that is kept: by_p without by_k
@@ -597,8 +609,12 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_rows_kernel(const Sample
     csync();
     // a share of the bins each, into rank 0's list
     for (int i = rank * (SR_MASS_BINS / C) + tid; i < (rank + 1) * (SR_MASS_BINS / C); i += SR_THREADS) {
+      uint32_t up[SR_MAX_CLUSTER], low_[SR_MAX_CLUSTER];
+#pragma unroll
+      for (int r = 0; r < SR_MAX_CLUSTER; ++r) up[r] = r < C ? sr_ld_u32(&upper[i], r) : 0, low_[r] = r < C ? sr_ld_u32(&lower[i], r) : 0;
       uint64_t v = 0;
-      for (int r = 0; r < C; ++r) v += (uint64_t(sr_ld_u32(&upper[i], r)) << 32) + sr_ld_u32(&lower[i], r);
+#pragma unroll
+      for (int r = 0; r < SR_MAX_CLUSTER; ++r) v += (uint64_t(up[r]) << 32) + low_[r];
       sr_st_u64(&list[i], 0, v);
     }
     csync();
