@@ -384,6 +384,19 @@ def test_sample_rows_large_vocabularies(V, dtype):
         assert ops.sample_rows(x, u, 1.0, k, 0.9).tolist() == [V - 1, V - 1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,scale", [(3000, 0.02), (3000, 1.0), (50257, 0.3), (50257, 2.0), (131072, 1.0), (131072, 4.0), (300001, 0.7)])
+def test_sample_rows_undecided(V, scale, dtype):
+    """Cuts that lie among hundreds or thousands of tokens of about equal mass: the bracket's list short, long and overflowing, with min-p beside it and without."""
+    B = 40
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = scale * torch.randn(B, V, generator=g, device="cuda")
+    pick = lambda vals, t: torch.tensor([vals[i % len(vals)] for i in range(B)], dtype=t, device="cuda")  # noqa: E731
+    numbers = (pick([1.0, 0.7, 1.3], torch.float32), pick([0, 0, 0, 400, 1000], torch.int32), pick([0.9, 0.5, 0.98, 0.999], torch.float32),
+               pick([0.0, 0.0, 1e-4, 0.0, 0.02], torch.float32), pick([1.0, 1.2], torch.float32))
+    _sample_case(B, V, dtype, V, numbers=numbers, scores=x)
+
+
 def test_sample_rows_draws_by_mass():
     """20,000 evenly spaced numbers over ten tokens: every token is named as often as its probability says, but for one at either border."""
     n = 20000
