@@ -35,7 +35,7 @@ _SIGNATURES = {
     "ats_page_plan": [_vp] * 10 + [_ci] * 6 + [_vp],
     "ats_paged_append": [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp],
     "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp],
-    "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _vp, _vp, _vp],
+    "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _ci, _vp, _vp, _vp],
     "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
     "ats_paged_portion": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 9 + [_cf, _ci, _vp, _vp, _vp],
     "ats_paged_portion_scratch": [_ci],
@@ -375,7 +375,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             _lib.check(_fn("ats_paged_portion")(*head, limit, scale, int(not keep_tail), _p(scratch), status, stream), "ats_paged_portion")
         if limit:
             scratch = torch.empty(_scratch("ats_paged_decode_scratch", R, n_kv, d, keys, limit), dtype=torch.uint8, device=device)
-            _lib.check(_fn("ats_paged_decode")(*head, keys, T if portions else new, limit, scale, int(not keep_tail and not portions), _p(scratch), status, stream), "ats_paged_decode")
+            _lib.check(_fn("ats_paged_decode")(*head, keys, T if portions else new, limit, scale, int(not keep_tail and not portions), int(portions), _p(scratch), status, stream), "ats_paged_decode")
     return out
 
 

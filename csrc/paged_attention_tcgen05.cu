@@ -670,7 +670,7 @@ static int launch_paged_portion(const CUtensorMap& mq, const CUtensorMap& mk, co
   static DeviceOnce once;
   cudaError_t ce = once.smem(paged_portion_kernel<D>, SM::TOTAL);
   if (ce == cudaSuccess) ce = launch_pdl(paged_portion_kernel<D>, dim3(p.ctas), dim3(PC_THREADS), SM::TOTAL, s, mq, mk, mv, p);
-  if (ce == cudaSuccess && p.ctas > 1) ce = launch_behind(paged_portion_join_kernel<D>, dim3(p.ctas - 1, 256 / PCJ_ROWS), dim3(PCJ_THREADS), s, p);
+  if (ce == cudaSuccess && p.ctas > 1) ce = launch_behind(paged_portion_join_kernel<D>, dim3(p.ctas - 1, 256 / PCJ_ROWS), dim3(PCJ_THREADS), s, 0, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }

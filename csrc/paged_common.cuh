@@ -28,10 +28,11 @@ inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, ui
 // Launches a kernel that begins with pdl_prologue() right behind one of the same operator that asks for it (griddepcontrol.launch_dependents behind its own
 // wait): it is set up while that one ends, whatever launches the thread makes else.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -37,6 +37,7 @@ struct PagedDecodeArgs {
   int max_new;              // no row has more new tokens
   int rows_most;            // MMA rows of any row that is taken
   int zero_tail;            // tokens behind the last row get zeros
+  int behind;               // the launch before this one is of the same call
   float scale_log2;
   uint32_t* line;           // [R + 1]: where a row's units begin, per key head; the end of the line
   float* part_o;            // [warps, 2, rows of the MMA, D]
@@ -522,14 +523,15 @@ template <int D, int NR, int G>
 static cudaError_t launch_paged_join(const PagedDecodeArgs& p, cudaStream_t s) {
   constexpr int AT_ONCE = PJ_THREADS / (G * D / 4);
   const int n = min(p.limit, p.rows_most);
-  return launch_behind(paged_join_kernel<D, NR, G>, dim3((n + AT_ONCE - 1) / AT_ONCE, p.n_kv, p.rows.R), dim3(PJ_THREADS), s, p);
+  return launch_behind(paged_join_kernel<D, NR, G>, dim3((n + AT_ONCE - 1) / AT_ONCE, p.n_kv, p.rows.R), dim3(PJ_THREADS), s, 0, p);
 }
 
 template <int D, int NR>
 static int launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedDecodeArgs& p, cudaStream_t s) {
   static DeviceOnce once;
   cudaError_t ce = once.smem(paged_decode_kernel<D, NR>, PD_SMEM);
-  if (ce == cudaSuccess) ce = launch_pdl(paged_decode_kernel<D, NR>, dim3((p.warps + PD_WARPS - 1) / PD_WARPS), dim3(PD_THREADS), PD_SMEM, s, mk, mv, p);
+  const dim3 grid((p.warps + PD_WARPS - 1) / PD_WARPS), block(PD_THREADS);
+  if (ce == cudaSuccess) ce = p.behind ? launch_behind(paged_decode_kernel<D, NR>, grid, block, s, PD_SMEM, mk, mv, p) : launch_pdl(paged_decode_kernel<D, NR>, grid, block, PD_SMEM, s, mk, mv, p);
   // slots of a pair, if the rows are about as long as each other
   const int slots = p.warps / (p.rows.R * p.n_kv);
   if (ce == cudaSuccess) ce = slots >= 8 ? launch_paged_join<D, NR, 8>(p, s) : launch_paged_join<D, NR, 2>(p, s);
@@ -554,10 +556,11 @@ ATS_API long long ats_paged_decode_scratch(int R, int n_kv, int D, long long max
 }
 
 // Rows whose new tokens times n_q / n_kv are at most `limit` (8 or 16).  q [tokens, ldq], pages [pages * page, n_kv, D] bf16, D 64 or 128, pages of 8 tokens
-// (a power of two) or more; max_keys: no row has more.  zero_tail: tokens behind the last row get zeros.
+// (a power of two) or more; max_keys: no row has more.  zero_tail: tokens behind the last row get zeros.  behind: ats_paged_portion of the same call is the
+// stream's last launch, so this one is set up while it ends.
 ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
                              void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, long long max_keys, int max_new, int limit,
-                             float scale, int zero_tail, void* scratch, int* status, void* stream) {
+                             float scale, int zero_tail, int behind, void* scratch, int* status, void* stream) {
   if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_kv > 65535 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
       (limit != 8 && limit != 16) || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 15) || max_new < 1 || max_keys < 1 || ((long long)width * page / 16 + 1) * R * n_kv >= (1ll << 32) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
     return 1003;
@@ -574,7 +577,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   PagedDecodeArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.q = static_cast<const __nv_bfloat16*>(q); p.ldq = ldq; p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;
-  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail;
+  p.n_kv = n_kv; p.rep = n_q / n_kv; p.limit = limit; p.max_new = max_new; p.rows_most = int(min((long long)max_new * p.rep, (long long)limit)); p.warps = paged_decode_warps(R, n_kv, D, max_keys); p.zero_tail = zero_tail; p.behind = behind;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   p.line = static_cast<uint32_t*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.line + (R + 4) / 4 * 4);
