@@ -151,6 +151,8 @@ class PagedPool:
 
     def _grow(self, more: Dict[int, int]) -> None:
         for slot, n in more.items():
+            if self.lengths[slot] + n > self.max_len:
+                raise RuntimeError(f"cache overflow: {self.lengths[slot]}+{n} > {self.max_len}")
             if self.cache.pool.pages_for(self.lengths[slot] + n) > self.reserved[slot]:
                 raise RuntimeError(f"row {slot} was opened for {self.reserved[slot]} pages and holds {self.lengths[slot]} tokens: no room for {n} more")
         for slot, n in more.items():

@@ -78,7 +78,7 @@ class PagedKVCache(SequenceCache):
     ``[1, T]`` or, with ``single``, at most one token per row ``[rows, 1]`` (the form that is captured in a CUDA graph)."""
 
     def __init__(self, num_layers: int, batch: int, max_len: int, pages: int, page_size: int, n_kv: int, head_dim: int, dtype, device):
-        super().__init__(batch, max_len, device)
+        super().__init__(batch, -(-max_len // max(page_size, 1)) * page_size, device)   # a row may fill its last page: rotary tables reach that far
         self.pool = ops.PagePool(batch, max_len, pages, page_size, device)
         self.k = [torch.zeros(pages, page_size, n_kv, head_dim, dtype=dtype, device=device) for _ in range(num_layers)]
         self.v = [torch.zeros(pages, page_size, n_kv, head_dim, dtype=dtype, device=device) for _ in range(num_layers)]

@@ -85,9 +85,9 @@ def _ints(t: torch.Tensor, name: str, shape, device) -> None:
 
 
 class PagePool:
-    """Page tables of ``rows`` rows of up to ``max_len`` tokens over ``pages`` pages of ``page_size`` tokens (a power of two).  ``tables``
+    """Page tables of ``rows`` rows of up to ``max_len`` tokens (and what their last page holds beyond) over ``pages`` pages of ``page_size`` tokens (a power of two).  ``tables``
     [rows, max_len / page_size], ``lengths`` [rows] (tokens a row holds) and the stack ``free`` live on the device; ``state`` holds the number of free
-    pages and the refusal code of the last committed step."""
+    pages and the refusal code of the last committed step.  Steps of one pool follow one another: plan them on one stream, or order the streams."""
 
     def __init__(self, rows: int, max_len: int, pages: int, page_size: int = 64, device="cuda"):
         _need(page_size >= 1 and page_size & (page_size - 1) == 0, f"page_size {page_size}: a power of two is needed")

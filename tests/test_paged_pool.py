@@ -128,3 +128,26 @@ def test_min_p_in_sampling_params():
     x = torch.tensor([[0.0, 5.0, 4.0, -3.0]]).expand(200, -1)
     kept = sample_next(x, SamplingParams(temperature=1.0, top_k=0, top_p=1.0, repetition_penalty=1.0, min_p=0.2)).unique().tolist()
     assert kept == [1, 2]
+
+
+@torch.no_grad()
+def test_rows_whose_length_is_no_multiple_of_a_page():
+    """A pool's rows end at ``max_len``; a cache that is planned by hand may fill the last page, and positions reach as far."""
+    model = _model()
+    pool = PagedPool(model, 2, 70, page_size=16, use_graph=False)
+    ids = torch.randint(0, 97, (80,), generator=torch.Generator().manual_seed(3))
+    row = pool.open(70)
+    pool.extend(row, ids[:69])
+    pool.last[row] = ids[69]
+    pool.decode([row])
+    with pytest.raises(RuntimeError, match="overflow"):
+        pool.decode([row])
+    with pytest.raises(RuntimeError, match="overflow"):
+        pool.extend(row, ids[:1])
+    assert pool.lengths[row] == 70
+    cache = model.make_paged_cache(2, 70, 10, 16)
+    assert cache.max_len == 80
+    cache.plan(torch.tensor([0, 80], dtype=torch.int32), 80)
+    got = model(ids[None], cache=cache, return_aux_loss=False)[0]
+    want = model(ids[None], return_aux_loss=False)[0]
+    assert torch.allclose(got, want, atol=2e-4)
