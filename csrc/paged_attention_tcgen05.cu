@@ -6,8 +6,9 @@
 // pages are read once for the whole group and short portions fill tiles too.  A CTA works on two tiles that share the K / V stream and
 // ping-pong on the tensor cores, as in gqa_attention_tcgen05.cu: one query row per soft-max thread, P overwrites S in tensor memory and is
 // the A operand of P V, O stays in tensor memory and is rescaled only when the running maximum grows by more than 2^8.
-// Bound by the tensor cores, whose operands come from shared memory (both for S, the values for P V), and the exponentials (per block of 128 keys and tile
-// 2 x 128 x 128 x D products, 16,384 exponentials).  32 / 8 heads of 128: 1,000 tokens behind 15,000 (255 GFLOP) 251 us = 1,000 TFLOP/s, 0.6 of the library
+// Bound by the chain of a tile's block, scores -> soft-max -> P V, of which two overlap (2.4 us a pair of blocks of 128 keys and 128 dimensions, 1.1 of them
+// products), and in it by the soft-max warps' instructions: an eighth of the exponentials as polynomials on the FMA lanes takes 3 % longer, half of them 19 %,
+// and a P V that begins under the last exponentials gains nothing.  32 / 8 heads of 128: 1,000 tokens behind 15,000 (255 GFLOP) 251 us = 1,000 TFLOP/s, 0.6 of the library
 // product's rate; six prompts of 300 to 2,500 tokens (96 GFLOP) 158 us = 610, which counts no product of a block that the diagonal halves and all beginnings and
 // ends of pieces.  Two soft-max threads a row took 180 us for the latter (from 153), products cut to the diagonal's columns 176 (from 164).
 //
