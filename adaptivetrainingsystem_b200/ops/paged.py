@@ -34,7 +34,8 @@ _REFUSED = {1: "a row gets more tokens than its table or the packed batch holds"
 _SIGNATURES = {
     "ats_page_plan": [_vp] * 10 + [_ci] * 6 + [_vp],
     "ats_paged_append": [_vp, _cll, _vp, _vp, _ci, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cll, _ci, _vp, _vp],
-    "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _vp, _vp],
+    "ats_paged_attn_any": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cf, _ci, _ci, _ci, _vp, _vp, _vp],
+    "ats_paged_any_splits": [_ci, _ci, _ci, _cll],
     "ats_paged_decode": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 8 + [_cll, _ci, _ci, _cf, _ci, _ci, _vp, _vp, _vp],
     "ats_paged_decode_scratch": [_ci, _ci, _ci, _cll, _ci],
     "ats_paged_portion": [_vp, _cll, _vp, _vp, _vp, _vp, _vp, _vp, _cll] + [_ci] * 9 + [_cf, _ci, _vp, _vp, _vp],
@@ -48,7 +49,7 @@ def _fn(name: str):
     f = _fns.get(name)
     if f is None:
         f = getattr(_lib.cuda_lib(), name)
-        f.restype, f.argtypes = _cll if name.endswith("_scratch") else _ci, _SIGNATURES[name]
+        f.restype, f.argtypes = _cll if name.endswith(("_scratch", "_splits")) else _ci, _SIGNATURES[name]
         _fns[name] = f
     return f
 
@@ -364,7 +365,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     head = (_p(q), ldq, _p(k_pages), _p(v_pages), _p(plan.starts), _p(plan.lengths), _p(plan.tables), _p(out), ldo, T, R, n_q, n_kv, d, width, pages, ps)
     with _on(device):
         if q.dtype != torch.bfloat16 or d not in (64, 128) or ps < 8 or rep > 128 or (width * ps // 16 + 1) * R * n_kv >= 1 << 32:
-            _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), status, stream), "ats_paged_attn_any")
+            splits = _scratch("ats_paged_any_splits", T, n_q, n_kv, max(keys, 1))
+            part = torch.empty(splits * T * n_q * (d + 2), dtype=torch.float32, device=device) if splits > 1 else None
+            _lib.check(_fn("ats_paged_attn_any")(*head, scale, int(keep_tail), int(q.dtype == torch.float32), splits, _p(part), status, stream), "ats_paged_attn_any")
             return out
         # Rows of a few query rows (new tokens times heads of a group) are a stream of the cache, longer portions a matter of the tensor cores.  A batch may
         # hold both, and which is which the kernels find in the plan; the host only knows when there can be none of one kind.

@@ -8,6 +8,7 @@
 //   packed starts of the rows, slot and position of every new token.
 // * ats_paged_append: rotary embedding of the new tokens' queries and keys; keys and values go to their slots.
 // * ats_paged_attn_any: causal grouped-query attention of the new tokens over their rows' pages (the general form).
+#include "paged_common.cuh"
 #include "typed.cuh"
 
 namespace ats {
@@ -258,10 +259,11 @@ __global__ void __launch_bounds__(APP_MAX_THREADS) paged_append_kernel(const App
 // Attention, general form: any head width that is a multiple of 8 up to 256, any group, any page size, bf16 or fp32 with fp32 sums.
 // A CTA serves one token and up to four query heads of a group.  Its four warps take blocks of 32 keys in turn: a lane scores one key for
 // all heads, then the lanes share out the value's columns; softmax as a running maximum and sum per warp, warps joined at the end.  Bound by its fp32 FMAs
-// and, for one token of a long row, by that row being one CTA's: 64 rows x 4 key heads of 64 with 200 to 2,000 keys 566 us (21 in the kernel for these sizes).
+// (64 rows x 4 key heads of 64 with 200 to 2,000 keys 566 us, 21 in the kernel for these sizes).  Few tokens of long rows: the row's blocks of 128 keys are shared out
+// over `splits` CTAs, as many as make four an SM but no more than the longest row has blocks; their sums are joined in order by a second launch.
 // Tokens behind the last row get zeros (or stay, `keep_tail`), as does a token that sees no key.
 // ------------------------------------------------------------------------------------------------
-constexpr int ANY_WARPS = 4, ANY_HEADS = 4;
+constexpr int ANY_WARPS = 4, ANY_HEADS = 4, ANY_BLOCK = 32 * ANY_WARPS, ANY_MAX_SPLITS = 64;
 
 struct PagedAnyArgs {
   const void* q;         // [tokens, ldq]
@@ -274,12 +276,12 @@ struct PagedAnyArgs {
   void* out;             // [tokens, ldo]
   long long ldo;
   int tokens, R, n_q, n_kv, d, width, pages, page_log, keep_tail;
+  int splits;
+  float* part;           // [splits, tokens, n_q, d + 2]: sums, largest score, sum of weights (one split: not used)
   float scale;
   int* status;
 };
 
-// the row of packed token t: largest r with starts[r] <= t
-__device__ __forceinline__ int row_of(const int* starts, int R, int t) { return last_le(starts, R, t); }
 
 template <typename T>
 __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const PagedAnyArgs p) {
@@ -297,14 +299,21 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const Pa
   int n = 0, r = 0;
   const int tail = p.starts[p.R];
   if (t < tail) {
-    r = row_of(p.starts, p.R, t);
+    r = last_le(p.starts, p.R, t);
     n = p.lengths[r] - (p.starts[r + 1] - t) + 1;      // keys that this token sees
     n = (int)min((long long)n, (long long)p.width << p.page_log);
   } else if (p.keep_tail) {
     return;
   }
-  if (n <= 0) {
-    for (int i = tid; i < nh * d; i += 32 * ANY_WARPS) Typed<T>::store(orow + i, 0.f);
+  float* part = p.part + (((long long)blockIdx.z * p.tokens + t) * p.n_q + hk * rep + h0) * (d + 2);
+  const int blocks = (max(n, 0) + ANY_BLOCK - 1) / ANY_BLOCK;
+  const int from = int((long long)blocks * blockIdx.z / p.splits) * ANY_BLOCK;
+  n = min(n, int((long long)blocks * (blockIdx.z + 1) / p.splits) * ANY_BLOCK);   // (keys of this CTA end here)
+  if (n <= from) {
+    if (p.splits > 1)
+      for (int i = tid; i < nh * (d + 2); i += 32 * ANY_WARPS) part[i] = i % (d + 2) == d ? -INFINITY : 0.f;
+    else
+      for (int i = tid; i < nh * d; i += 32 * ANY_WARPS) Typed<T>::store(orow + i, 0.f);
     return;
   }
   const T* qrow = static_cast<const T*>(p.q) + (long long)t * p.ldq + (long long)(hk * rep + h0) * d;
@@ -320,7 +329,7 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const Pa
   float* wp = sp + warp * ANY_HEADS * 32;
   const int* table = p.tables + (long long)r * p.width;
   const long long ld = (long long)p.n_kv * d;
-  for (int k0 = warp * 32; k0 < n; k0 += ANY_WARPS * 32) {
+  for (int k0 = from + warp * 32; k0 < n; k0 += ANY_BLOCK) {
     const int j = k0 + lane;
     float s[ANY_HEADS];
 #pragma unroll
@@ -333,7 +342,8 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const Pa
     }
     if (at >= 0) {
       const T* krow = static_cast<const T*>(p.k_pages) + at;
-      for (int c = 0; c < d; c += 8) {
+#pragma unroll 4
+      for (int c = 0; c < d; c += 8) {   // (loads of several pieces under way at once: few warps share an SM where tokens are few)
         float kv[8];
         Typed<T>::load8(krow + c, kv);
 #pragma unroll
@@ -359,18 +369,28 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const Pa
     }
     __syncwarp();
     const int cnt = min(32, n - k0);
-    for (int i = 0; i < cnt; ++i) {
-      const long long vat = __shfl_sync(0xffffffffu, at, i);
-      if (vat < 0) continue;
-      const T* vrow = static_cast<const T*>(p.v_pages) + vat;
+    for (int i = 0; i < cnt; i += 4) {   // (keys from cnt on: no place, no weight)
+      const T* vrow[4];
+      bool there[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long vat = __shfl_sync(0xffffffffu, at, i + j);
+        there[j] = vat >= 0;
+        vrow[j] = static_cast<const T*>(p.v_pages) + vat;
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int c = lane + 32 * e;
         if (c < d) {
-          const float vv = Typed<T>::load(vrow + c);
+          float vv[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vv[j] = there[j] ? Typed<T>::load(vrow[j] + c) : 0.f;
 #pragma unroll
           for (int h = 0; h < ANY_HEADS; ++h)
-            if (h < nh) acc[h][e] = fmaf(wp[h * 32 + i], vv, acc[h][e]);
+            if (h < nh) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[h][e] = fmaf(wp[h * 32 + i + j], vv[j], acc[h][e]);
+            }
         }
       }
     }
@@ -396,7 +416,30 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) paged_attn_any_kernel(const Pa
       o += so[(w * ANY_HEADS + h) * d + c] * f;
       sum += s_l[w][h] * f;
     }
-    Typed<T>::store(orow + i, sum > 0.f ? o / sum : o);   // (a sum that is no number stays one)
+    if (p.splits > 1) {
+      part[h * (d + 2) + c] = o;
+      if (c == 0) part[h * (d + 2) + d] = top, part[h * (d + 2) + d + 1] = sum;
+    } else {
+      Typed<T>::store(orow + i, sum > 0.f ? o / sum : o);   // (a sum that is no number stays one)
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) paged_any_join_kernel(const PagedAnyArgs p) {
+  pdl_prologue();
+  const int t = blockIdx.x, h = blockIdx.y, d = p.d;
+  if (p.keep_tail && t >= p.starts[p.R]) return;
+  const float* part = p.part + ((long long)t * p.n_q + h) * (d + 2);
+  const long long step = (long long)p.tokens * p.n_q * (d + 2);
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * step + d]);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int s = 0; s < p.splits; ++s) sum += part[s * step + d + 1] * expf(part[s * step + d] - base);
+  for (int c = threadIdx.x; c < d; c += 128) {
+    float o = 0.f;
+    for (int s = 0; s < p.splits; ++s) o += part[s * step + c] * expf(part[s * step + d] - base);
+    Typed<T>::store(static_cast<T*>(p.out) + (long long)t * p.ldo + (long long)h * d + c, sum > 0.f ? o / sum : o);
   }
 }
 
@@ -439,21 +482,31 @@ ATS_API int ats_paged_append(const void* qkv, long long ld, const float* cos_t, 
   return int(cudaGetLastError());
 }
 
+// CTAs that share a token's keys, of which there are `keys` at most.
+ATS_API long long ats_paged_any_splits(int tokens, int n_q, int n_kv, long long keys) {
+  const long long ctas = (long long)tokens * n_kv * ((n_q / n_kv + ANY_HEADS - 1) / ANY_HEADS);
+  const long long splits = min((keys + ANY_BLOCK - 1) / ANY_BLOCK, 4 * 148 / max(ctas, 1ll));
+  return max(1ll, min(splits, (long long)ANY_MAX_SPLITS));
+}
+
+// splits > 1: `part` is scratch of splits * tokens * n_q * (d + 2) floats.
 ATS_API int ats_paged_attn_any(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
                                void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int d, int width, int pages, int page, float scale, int keep_tail,
-                               int fp32, int* status, void* stream) {
-  if (tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || d < 8 || d > 256 || (d & 7) || (ldq & 7) || (ldo & 7) || page < 1 || (page & (page - 1))) return 1003;
+                               int fp32, int splits, float* part, int* status, void* stream) {
+  if (splits < 1 || splits > ANY_MAX_SPLITS || (splits > 1 && !part) || n_q > 65535 || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || d < 8 || d > 256 || (d & 7) || (ldq & 7) || (ldo & 7) || page < 1 || (page & (page - 1))) return 1003;
   const int groups = (n_q / n_kv + ANY_HEADS - 1) / ANY_HEADS;
   if ((long long)n_kv * groups > 65535) return 1003;
   PagedAnyArgs p;
   p.q = q; p.ldq = ldq; p.k_pages = k_pages; p.v_pages = v_pages; p.starts = starts; p.lengths = lengths; p.tables = tables; p.out = out; p.ldo = ldo;
   p.tokens = tokens; p.R = R; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.width = width; p.pages = pages; p.page_log = __builtin_ctz(page);
-  p.keep_tail = keep_tail; p.scale = scale; p.status = status;
+  p.keep_tail = keep_tail; p.scale = scale; p.splits = splits; p.part = part; p.status = status;
   const size_t smem = sizeof(float) * (ANY_HEADS * d + ANY_WARPS * ANY_HEADS * 32 + ANY_WARPS * ANY_HEADS * d);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(tokens, n_kv * groups);
-  const cudaError_t ce = fp32 ? launch_pdl(paged_attn_any_kernel<float>, grid, dim3(32 * ANY_WARPS), smem, s, p)
-                              : launch_pdl(paged_attn_any_kernel<__nv_bfloat16>, grid, dim3(32 * ANY_WARPS), smem, s, p);
+  const dim3 grid(tokens, n_kv * groups, splits);
+  cudaError_t ce = fp32 ? launch_pdl(paged_attn_any_kernel<float>, grid, dim3(32 * ANY_WARPS), smem, s, p)
+                        : launch_pdl(paged_attn_any_kernel<__nv_bfloat16>, grid, dim3(32 * ANY_WARPS), smem, s, p);
+  if (ce == cudaSuccess && splits > 1)
+    ce = fp32 ? launch_behind(paged_any_join_kernel<float>, dim3(tokens, n_q), dim3(128), s, 0, p) : launch_behind(paged_any_join_kernel<__nv_bfloat16>, dim3(tokens, n_q), dim3(128), s, 0, p);
   if (ce != cudaSuccess) return int(ce);
   return int(cudaGetLastError());
 }

@@ -427,3 +427,11 @@ def test_sample_rows_takes_any_top_k_on_the_gpu():
     everything = ops.sample_rows(logits, u)
     for k in (4000, 1 << 31, 1 << 40, -5, torch.tensor([1 << 40, -(1 << 40), 0], device="cuda")):
         assert torch.equal(ops.sample_rows(logits, u, top_k=k), everything)
+
+
+@pytest.mark.parametrize("hints", [True, False])
+@pytest.mark.parametrize("n_q,n_kv,d,page,dtype", [(8, 2, 96, 64, torch.bfloat16), (4, 4, 64, 16, torch.float32), (6, 1, 256, 4, torch.float32), (3, 3, 8, 1, torch.bfloat16)])
+def test_attention_general_form_of_long_rows(n_q, n_kv, d, page, dtype, hints):
+    """Rows whose keys several thread blocks share, beside rows shorter than one block's share, tokens of no row and a row without new tokens."""
+    _attend_case([9000, 0, 130, 2047, 50], [1, 1, 2, 1, 0], page, n_q, n_kv, d, dtype, tail=2, hints=hints)
+    _attend_case([20011], [1], page, n_q, n_kv, d, dtype, hints=hints, strided=True)
