@@ -259,8 +259,10 @@ __global__ void __launch_bounds__(APP_MAX_THREADS) paged_append_kernel(const App
 // Attention, general form: any head width that is a multiple of 8 up to 256, any group, any page size, bf16 or fp32 with fp32 sums.
 // A CTA serves one token and up to four query heads of a group.  Its four warps take blocks of 32 keys in turn: a lane scores one key for
 // all heads, then the lanes share out the value's columns; softmax as a running maximum and sum per warp, warps joined at the end.  Bound by its fp32 FMAs
-// (64 rows x 4 key heads of 64 with 200 to 2,000 keys 566 us, 21 in the kernel for these sizes).  Few tokens of long rows: the row's blocks of 128 keys are shared out
-// over `splits` CTAs, as many as make four an SM but no more than the longest row has blocks; their sums are joined in order by a second launch.
+// and the latency of its loads.  Few tokens: a row's blocks of 128 keys are shared out over `splits` CTAs, as many as make eight
+// an SM but no more than the longest row has blocks; their sums are joined in order by a second launch.  One row of 32,000 keys x 8 heads of 96 in bf16 111 us (one
+// CTA a token and group 4,800), 64 rows of 200 to 2,000 keys x 8 of 96 251 (373), x 4 of 64 in fp32 186 (282); with four an SM 112, 372, 283 and 8 rows of 4,000 x 8 of
+// 128 in fp32 164 instead of 179; with twelve 113, 244, 180 and 188.
 // Tokens behind the last row get zeros (or stay, `keep_tail`), as does a token that sees no key.
 // ------------------------------------------------------------------------------------------------
 constexpr int ANY_WARPS = 4, ANY_HEADS = 4, ANY_BLOCK = 32 * ANY_WARPS, ANY_MAX_SPLITS = 64;
@@ -485,7 +487,7 @@ ATS_API int ats_paged_append(const void* qkv, long long ld, const float* cos_t, 
 // CTAs that share a token's keys, of which there are `keys` at most.
 ATS_API long long ats_paged_any_splits(int tokens, int n_q, int n_kv, long long keys) {
   const long long ctas = (long long)tokens * n_kv * ((n_q / n_kv + ANY_HEADS - 1) / ANY_HEADS);
-  const long long splits = min((keys + ANY_BLOCK - 1) / ANY_BLOCK, 4 * 148 / max(ctas, 1ll));
+  const long long splits = min((keys + ANY_BLOCK - 1) / ANY_BLOCK, 8 * 148 / max(ctas, 1ll));
   return max(1ll, min(splits, (long long)ANY_MAX_SPLITS));
 }
 
