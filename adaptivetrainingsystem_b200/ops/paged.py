@@ -267,13 +267,15 @@ def _kernel_type(t: torch.Tensor, d: int) -> None:
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    """A [T, heads, d] (or [T, width]) tensor as its kernel takes it: rows of contiguous heads that start at multiples of 16 bytes."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == t.shape[2])
-    if inner and (t.shape[0] == 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0:
-        return t
-    return t.contiguous()
+    """A [T, heads, d] (or [T, width]) tensor as its kernel takes it: rows of contiguous heads, one behind the other, that start at multiples of 16 bytes.
+    Any other one is copied."""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        inner = t.stride(-1) == 1 and (t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == t.shape[2])
+        if inner and (t.shape[0] == 1 or t.stride(0) % 8 == 0 and t.stride(0) >= t.numel() // t.shape[0]):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)   # (contiguous() would give back one that only starts off 16 bytes)
 
 
 def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], plan: PagePlan, k_pages: torch.Tensor, v_pages: torch.Tensor, n_q: int,

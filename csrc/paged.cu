@@ -470,7 +470,7 @@ ATS_API int ats_page_plan(int* lengths, const int* fresh, int* tables, int* free
 // fp32: 0 = bf16.  cos_t null: no rotation, q_out is not written.  d a multiple of 16 (of 8 without rotation), at most 256.
 ATS_API int ats_paged_append(const void* qkv, long long ld, const float* cos_t, const float* sin_t, int table, const int* positions, const int* slots, void* q_out,
                              void* k_pages, void* v_pages, int tokens, int n_q, int n_kv, int d, long long n_slots, int fp32, int* status, void* stream) {
-  if (tokens < 1 || n_q < 1 || n_kv < 1 || d < 8 || d > 256 || (d & (cos_t ? 15 : 7)) || (ld & 7)) return 1003;
+  if (tokens < 1 || n_q < 1 || n_kv < 1 || d < 8 || d > 256 || (d & (cos_t ? 15 : 7)) || (ld & 7) || off_16(qkv, cos_t, sin_t, k_pages, v_pages) || (cos_t && off_16(q_out))) return 1003;
   AppendArgs p;
   p.qkv = qkv; p.ld = ld; p.cos_t = cos_t; p.sin_t = sin_t; p.positions = positions; p.slots = slots; p.q_out = q_out; p.k_pages = k_pages;
   p.v_pages = v_pages; p.tokens = tokens; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.table = table; p.n_slots = n_slots; p.status = status;
@@ -495,7 +495,7 @@ ATS_API long long ats_paged_any_splits(int tokens, int n_q, int n_kv, long long 
 ATS_API int ats_paged_attn_any(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
                                void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int d, int width, int pages, int page, float scale, int keep_tail,
                                int fp32, int splits, float* part, int* status, void* stream) {
-  if (splits < 1 || splits > ANY_MAX_SPLITS || (splits > 1 && !part) || n_q > 65535 || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || d < 8 || d > 256 || (d & 7) || (ldq & 7) || (ldo & 7) || page < 1 || (page & (page - 1))) return 1003;
+  if (splits < 1 || splits > ANY_MAX_SPLITS || (splits > 1 && !part) || n_q > 65535 || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || d < 8 || d > 256 || (d & 7) || (ldq & 7) || (ldo & 7) || page < 1 || (page & (page - 1)) || off_16(k_pages, v_pages)) return 1003;
   const int groups = (n_q / n_kv + ANY_HEADS - 1) / ANY_HEADS;
   if ((long long)n_kv * groups > 65535) return 1003;
   PagedAnyArgs p;

@@ -688,7 +688,7 @@ ATS_API long long ats_paged_portion_scratch(int D) { return 32 + PC_CTAS * (long
 ATS_API int ats_paged_portion(const void* q, long long ldq, const void* k_pages, const void* v_pages, const int* starts, const int* lengths, const int* tables,
                               void* out, long long ldo, int tokens, int R, int n_q, int n_kv, int D, int width, int pages, int page, int limit, float scale,
                               int zero_tail, void* scratch, int* status, void* stream) {
-  if ((D != 64 && D != 128) || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || n_q / n_kv > 128 || (ldq & 7) || (ldo & 7) || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(scratch) & 31) ||
+  if ((D != 64 && D != 128) || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || n_q / n_kv > 128 || (ldq & 7) || (ldo & 7) || off_16(q, k_pages, v_pages, out) || (reinterpret_cast<uintptr_t>(scratch) & 31) ||
       page < 8 || (page & (page - 1)) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256 || tokens > (1 << 30))
     return 1003;
   static thread_local bool ctx_bound = false;

@@ -25,6 +25,12 @@ inline int make_tmap_pages(CUtensorMap* out, const void* base, uint64_t rows, ui
   return make_tmap_tokens(out, base, rows, n_kv, d, n_kv * d, 1, box_rows);
 }
 
+// Operands that are read or written 16 bytes at a time begin at multiples of 16 bytes.
+template <typename... P>
+inline bool off_16(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15) != 0;
+}
+
 // Launches a kernel that begins with pdl_prologue() right behind one of the same operator that asks for it (griddepcontrol.launch_dependents behind its own
 // wait): it is set up while that one ends, whatever launches the thread makes else.
 template <typename... KArgs, typename... Args>

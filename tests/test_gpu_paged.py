@@ -435,3 +435,32 @@ def test_attention_general_form_of_long_rows(n_q, n_kv, d, page, dtype, hints):
     """Rows whose keys several thread blocks share, beside rows shorter than one block's share, tokens of no row and a row without new tokens."""
     _attend_case([9000, 0, 130, 2047, 50], [1, 1, 2, 1, 0], page, n_q, n_kv, d, dtype, tail=2, hints=hints)
     _attend_case([20011], [1], page, n_q, n_kv, d, dtype, hints=hints, strided=True)
+
+
+def _off(t, elements=1):
+    """``t``'s values, contiguous, that many elements behind a multiple of sixteen bytes."""
+    room = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)
+    start = (-room.data_ptr() % 16) // t.element_size() + elements
+    return room[start:start + t.numel()].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("n_q,n_kv,d,dtype", [(8, 2, 64, torch.bfloat16), (4, 4, 128, torch.bfloat16), (6, 2, 96, torch.bfloat16), (4, 2, 64, torch.float32)])
+@pytest.mark.parametrize("old,new", [([200, 5, 63], [1, 1, 1]), ([40], [1]), ([0, 100, 40], [150, 1, 20])])
+def test_operands_that_start_off_16_bytes_or_lie_on_one_another(old, new, n_q, n_kv, d, dtype):
+    """The bits of the same operands in rows of their own that start at whole 16 bytes."""
+    plan, pages = make_plan(old, new, 16, "cuda", tail=2)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(pages, 16, n_kv, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    T, width = sum(new) + 2, (n_q + 2 * n_kv) * d
+    q, qkv = torch.randn(T, n_q, d, generator=g, device="cuda").to(dtype), torch.randn(T, width, generator=g, device="cuda").to(dtype)
+    want = ops.paged_attention(q, k, v, plan)
+    for odd in (_off(q), _off(q, 3), torch.cat([q.flatten(1), q[:, 0]], 1).as_strided((T, n_q, d), ((n_q + 1) * d, d, 1))):
+        assert torch.equal(ops.paged_attention(odd, k, v, plan), want)
+    same = q[:1].expand(T, -1, -1)
+    assert torch.equal(ops.paged_attention(same, k, v, plan), ops.paged_attention(same.contiguous(), k, v, plan))
+    with pytest.raises(ValueError, match="16 bytes"):
+        ops.paged_attention(q, k, v, plan, out=_off(q))
+    for cos, sin in ((None, None), ops.rope_tables(600, d, 10000.0, device="cuda")):
+        a, b = (k.clone(), v.clone()), (k.clone(), v.clone())
+        x, y = ops.paged_append(qkv, cos, sin, plan, *a, n_q, n_kv, d), ops.paged_append(_off(qkv), cos, sin, plan, *b, n_q, n_kv, d)
+        assert torch.equal(x, y) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

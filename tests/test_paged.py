@@ -186,3 +186,54 @@ def test_sample_rows_takes_any_top_k():
     everything = ops.sample_rows(logits, u)
     for k in (40, 1 << 31, 1 << 40, -5, torch.tensor([1 << 40, -(1 << 40), 0])):
         assert torch.equal(ops.sample_rows(logits, u, top_k=k), everything)
+
+
+def _off(t, elements=1):
+    """``t``'s values, contiguous, that many elements behind a multiple of sixteen bytes."""
+    room = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)
+    start = (-room.data_ptr() % 16) // t.element_size() + elements
+    return room[start:start + t.numel()].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_operands_that_start_off_16_bytes_are_copied(dtype):
+    from adaptivetrainingsystem_b200.ops.paged import _rows_of
+    wide = torch.randn(6, 5 * 64 + 8).to(dtype)
+    cases = [_off(torch.randn(4, 8, 64).to(dtype)), _off(torch.randn(4, 320).to(dtype), 2), wide[:1, 1:321], wide[:, 1:321], wide[:, 8:328][:, :320].unflatten(1, (5, 64))[..., ::2],
+             wide[:1, :320].expand(4, 320), torch.randn(9 * 64).to(dtype).as_strided((4, 5, 64), (64, 64, 1)), wide[0, :320].view(1, 5, 64).expand(3, 5, 64)]
+    for t in cases:
+        got = _rows_of(t)
+        assert got is not t and got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, t)
+    for t in (wide, wide[:, 8:328], wide[:, 8:328].unflatten(1, (5, 64)), wide[:1, 8:328], wide[3:4].view(1, 41, 8)):   # nothing to copy
+        assert _rows_of(t) is t
+    plan, pages = make_plan([3], [2], 4, "cpu")
+    k = torch.zeros(pages, 4, 2, 16, dtype=dtype)
+    q = torch.zeros(2, 4, 16, dtype=dtype)
+    with pytest.raises(ValueError, match="16 bytes"):
+        ops.paged_attention(q, k, k, plan, out=_off(q))
+
+
+def test_entry_points_refuse_operands_off_16_bytes():
+    """Before they look at what the operands point to."""
+    import ctypes
+    import os
+    from adaptivetrainingsystem_b200.ops import _lib, paged
+    if not os.path.exists(_lib.CUDA_LIB):
+        pytest.skip("the CUDA library has not been built")
+    lib = ctypes.CDLL(_lib.CUDA_LIB)
+
+    def call(name, *args):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = ctypes.c_int, paged._SIGNATURES[name]
+        return f(*args)
+    at = 1 << 20
+    for bad in range(6):   # queries and projections, pages, outputs, tables, scratch
+        q, k, v, out, cos, scratch = (at + (2 if i == bad else 0) for i in range(6))
+        attend = (q, 256, k, v, at, at, at, out, 256, 3, 1, 4, 2, 64, 4, 8, 16)
+        if bad < 5:
+            assert bad == 4 or call("ats_paged_portion", *attend, 8, 1.0, 0, at, at, None) == 1003
+            assert call("ats_paged_append", q, 512, cos, at, 64, at, at, out, k, v, 3, 4, 2, 64, 128, 0, at, None) == 1003
+        if bad != 4:
+            assert call("ats_paged_decode", *attend, 64, 1, 8, 1.0, 0, 0, scratch, at, None) == 1003
+        if bad in (1, 2):
+            assert call("ats_paged_attn_any", *attend, 1.0, 0, 0, 1, None, at, None) == 1003
