@@ -186,12 +186,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ unsigned long long s_sum[PC_THREADS / 32], s_base;
   __shared__ int s_row;
-  // per piece: keys whose values each of the two warps cleared, 128 bits a block from the first block on the diagonal on.  They are ahead of the warps
-  // that read these by the stages of the ring at most.
-  __shared__ uint32_t s_cleared[8][2][PC_EDGE * 4], s_any[8][2];
-  // The pieces, told by the producer: it is ahead of the others by the stages of the ring at most (every piece takes one), so eight places are enough.
+  // The pieces, told by the producer, which writes a place again when all that read it have said so (nothing else holds it back for the soft-max warps of
+  // a tile without keys or the clearing warps of a piece without a diagonal block).
   __shared__ PcPiece s_piece[8];
-  __shared__ uint64_t s_told[8];
+  __shared__ uint64_t s_told[8], s_through[8];
+  // of each: keys whose values the two clearing warps cleared, 128 bits a block from the first block on the diagonal on
+  __shared__ uint32_t s_cleared[8][2][PC_EDGE * 4], s_any[8][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedRows& rows = p.rows;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -212,7 +212,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       mbar_init(&p_full[x], 4);
       mbar_init(&o_done[x], 1);
     }
-    for (int x = 0; x < 8; ++x) mbar_init(&s_told[x], 1);
+    for (int x = 0; x < 8; ++x) {
+      mbar_init(&s_told[x], 1);
+      mbar_init(&s_through[x], 11);   // 8 soft-max warps, MMA, 2 clearing warps
+    }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_q);
@@ -262,11 +265,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
   if (lo < hi) start.find(p, s_row, s_base, lo);
   else start.base = hi;
   if (tid == 0) p.begins[blockIdx.x] = start;
-  auto next_piece = [&](uint32_t n) -> const PcPiece* {   // the n-th, or null behind the last one (and where a wait ran out)
+  auto next_piece = [&](uint32_t n) -> const PcPiece* {   // the n-th, until piece_done(n), or null behind the last one (and where a wait ran out)
     if (!mbar_wait_bounded(&s_told[n & 7], (n >> 3) & 1, abort_flag, p.status, kTimeoutFull)) return nullptr;
     const PcPiece* s = &s_piece[n & 7];
     return s->j0 < s->j1 ? s : nullptr;
   };
+  auto piece_done = [&](uint32_t n) { mbar_arrive(&s_through[n & 7]); };   // one lane of each warp
   // columns: S_A [0,128)  S_B [128,256)  O_A [256, 256 + D)  O_B [256 + D, 256 + 2 D)
 
   if (warp == 8) {
@@ -280,6 +284,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
     while (ok) {
       const bool more = walk.next(s);
       if (!more) s.j0 = s.j1 = 0;
+      if (!(ok = mbar_wait_warp(&s_through[n_pieces & 7], ((n_pieces >> 3) & 1) ^ 1, abort_flag, p.status, kTimeoutEmpty))) break;
       if (lane == 0) {
         s_piece[n_pieces & 7] = s;
         mbar_arrive(&s_told[n_pieces & 7]);
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         ok = mbar_wait_bounded(q_full, n_pieces & 1, abort_flag, p.status, kTimeoutFull);
         ok = ok && mbar_wait_bounded(&k_full[n_blocks % ST], (n_blocks / ST) & 1, abort_flag, p.status, kTimeoutFull);
         if (!ok) break;
-        ++n_pieces;
+        piece_done(n_pieces++);
         tc_fence_after();
         for (int x = 0; x < 2; ++x)
           if (j0 < ends[x]) issue_s(x, n_blocks % ST);
@@ -441,6 +446,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
       }
+      if (ok && lane == 0) piece_done(n_pieces);
     }
   } else {
     // -------------------------------------------------------------------- soft-max groups
@@ -456,7 +462,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
     for (; ok; ++n_pieces) {
       const PcPiece* told = next_piece(n_pieces);
       if (!__all_sync(0xffffffffu, told != nullptr)) break;
-      const PcPiece& s = *told;   // (stays until the warp is through with it)
+      const PcPiece& s = *told;
       const int tile_tok = s.tok0 + x * p.tile, tok = tile_tok + my_tok;
       const bool live = my_tok < p.tile && tok < s.fresh;
       const int first_pos = s.keys - s.fresh + tile_tok;        // of the tile's first token
@@ -564,7 +570,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
                             make_uint4(o[8 * e + 4], o[8 * e + 5], o[8 * e + 6], o[8 * e + 7]));
           }
         };
-        if ((s_any[n_pieces & 7][0] | s_any[n_pieces & 7][1]) == 0) {
+        if (end <= s.edge(p) || (s_any[n_pieces & 7][0] | s_any[n_pieces & 7][1]) == 0) {   // (written before the values of the first diagonal block were released)
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -596,6 +602,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
         }
         tc_fence_before();   // O has been read: the next piece's first P, which this warp announces, may be followed by a P V over it
       }
+      __syncwarp();
+      if (lane == 0) piece_done(n_pieces);
     }
   }
   tc_fence_before();

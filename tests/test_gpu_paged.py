@@ -464,3 +464,29 @@ def test_operands_that_start_off_16_bytes_or_lie_on_one_another(old, new, n_q, n
         a, b = (k.clone(), v.clone()), (k.clone(), v.clone())
         x, y = ops.paged_append(qkv, cos, sin, plan, *a, n_q, n_kv, d), ops.paged_append(_off(qkv), cos, sin, plan, *b, n_q, n_kv, d)
         assert torch.equal(x, y) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_short_portions_behind_values_that_are_not_finite(d):
+    """Every fourteenth row is two tiles of tokens whose values hold an infinity each, which its second tile adds one by one; the portions between them have
+    one tile, so that a CTA's other warps run ahead of that one's.  Rows beside them stay as they are."""
+    new = [256 if r % 14 == 0 else 17 + r % 5 for r in range(2100)]
+    plan, pages = make_plan([0] * len(new), new, 16, "cuda")
+    plan.max_new = plan.max_len = 256
+    g = torch.Generator(device="cuda").manual_seed(d)
+    k, v = (torch.randn(pages, 16, 1, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    T = sum(new)
+    q = torch.randn(T, 1, d, generator=g, device="cuda").bfloat16()
+    ref, mass = attend64(q, k, v, plan, 1 / math.sqrt(d))
+    inf = torch.zeros(T, d, dtype=torch.bool, device="cuda")
+    tokens = torch.arange(256, device="cuda")
+    for r in range(0, len(new), 14):
+        v.view(-1, d)[plan.slots[int(plan.starts[r]) + tokens].long(), tokens % d] = float("inf")
+        inf[int(plan.starts[r]) + tokens] = torch.arange(d, device="cuda")[None] <= tokens[:, None]   # token i sees the values of 0 to i
+    bound = _attention_bound(torch.bfloat16, ref, mass, 256, d)
+    first = ops.paged_attention(q, k, v, plan)
+    for out in (first, ops.paged_attention(q, k, v, plan)):
+        assert torch.equal(out[:, 0] == float("inf"), inf)
+        assert bool(((out.double() - ref).abs() <= bound)[:, 0][~inf].all())
+        assert torch.equal(out, first)
+    ops.check_status()
