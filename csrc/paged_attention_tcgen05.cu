@@ -470,10 +470,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       const int end = s.end(x);
       float m = -1e30f, l = 0.f;
       for (int j = s.j0; j < end; ++j, ++n_s) {
-        if (!mbar_wait_bounded(&s_full[x], n_s & 1, abort_flag, p.status, kTimeoutTmemFull)) {
-          ok = false;
-          break;
-        }
+        if (!(ok = mbar_wait_warp(&s_full[x], n_s & 1, abort_flag, p.status, kTimeoutTmemFull))) break;
         tc_fence_after();
         uint32_t v[128];
 #pragma unroll
@@ -535,7 +532,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       if (!ok) break;
       const bool any = end > s.j0;   // the tile sees keys of this piece
       if (any) {
-        if (!mbar_wait_bounded(&o_done[x], n_o & 1, abort_flag, p.status, kTimeoutTmemFull)) break;
+        if (!mbar_wait_warp(&o_done[x], n_o & 1, abort_flag, p.status, kTimeoutTmemFull)) break;
         ++n_o;
         tc_fence_after();
       }

@@ -237,3 +237,17 @@ def test_entry_points_refuse_operands_off_16_bytes():
             assert call("ats_paged_decode", *attend, 64, 1, 8, 1.0, 0, 0, scratch, at, None) == 1003
         if bad in (1, 2):
             assert call("ats_paged_attn_any", *attend, 1.0, 0, 0, 1, None, at, None) == 1003
+
+
+def test_warps_of_the_portion_kernel_give_up_a_wait_together():
+    """Roles of whole warps go on with instructions that all lanes take part in: where a wait runs out, none of them may go on alone.  (One lane issues products.)"""
+    import pathlib
+    import adaptivetrainingsystem_b200
+    text = (pathlib.Path(adaptivetrainingsystem_b200.__file__).parents[1] / "csrc" / "paged_attention_tcgen05.cu").read_text()
+    kernel = text[text.index("paged_portion_kernel("):text.index("paged_portion_join_kernel")]
+    roles = kernel.split("  // ------------------------------------------------------------------")
+    assert len(roles) == 5
+    for role in roles[1:]:
+        assert ("mbar_wait_bounded" in role) == role.lstrip("- ").startswith("MMA issuer"), role[:80]
+    for told in kernel.split("next_piece(n_pieces);")[2:]:
+        assert told.lstrip().startswith("if (!__all_sync(0xffffffffu, told != nullptr)) break;")
