@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
       const int first_pos = s.keys - s.fresh + tile_tok;        // of the tile's first token
       const int my_pos = live ? s.keys - s.fresh + tok : -1;
       const int end = s.end(x);
-      float m = -1e30f, l = 0.f;
+      float m = -3.402823466e38f, l = 0.f;   // (no finite score is below)
       for (int j = s.j0; j < end; ++j, ++n_s) {
         if (!(ok = mbar_wait_warp(&s_full[x], n_s & 1, abort_flag, p.status, kTimeoutTmemFull))) break;
         tc_fence_after();
@@ -491,25 +491,34 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_portion_kernel(const __gr
           mx3 = fmaxf(mx3, fmaxf(__uint_as_float(v[c + 6]), __uint_as_float(v[c + 7])));
         }
         const float mnew = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * p.scale_log2);
-        if (j == s.j0) {
-          m = mnew;
-        } else if (__any_sync(0xffffffffu, live && mnew > m + 8.f)) {   // (what lies behind the portion in the tile has no say)
+        // score * scale - m in one rounding leaves the rounding of m in every exponent: a common factor, at most 2^32 up to an m of 2^30.  Beyond, the scores
+        // are scaled first, rounded like m itself.
+        constexpr float BIG = 1073741824.f;
+        float scale = p.scale_log2;
+        if (__any_sync(0xffffffffu, live && (mnew > m + 8.f || fabsf(mnew) > BIG))) {   // (what lies behind the portion in the tile has no say)
           const float alpha = exp2f(m - mnew);  // the previous P V of this tile has completed: S(j) was computed after it
           m = mnew;
           l *= alpha;
+          if (j > s.j0) {
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_32x16(tmem_O + c * 16, o);
-            tmem_ld_wait();
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x16(tmem_O + c * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x16(tmem_O + c * 16, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_32x16(tmem_O + c * 16, o);
+            }
+            tmem_st_wait();
           }
-          tmem_st_wait();
+          if (__any_sync(0xffffffffu, live && fabsf(m) > BIG)) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * scale);
+            scale = 1.f;
+          }
         }
         float2 rsa = make_float2(0.f, 0.f), rsb = make_float2(0.f, 0.f);
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m, -m);
+        const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-m, -m);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];

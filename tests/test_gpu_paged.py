@@ -490,3 +490,29 @@ def test_attention_short_portions_behind_values_that_are_not_finite(d):
         assert bool(((out.double() - ref).abs() <= bound)[:, 0][~inf].all())
         assert torch.equal(out, first)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n_q,n_kv,d", [(8, 2, 64), (4, 4, 128), (6, 2, 96)])
+@pytest.mark.parametrize("old,new", [([700, 0, 130], [1, 1, 2]), ([700, 0, 130], [300, 150, 40]), ([9000], [20])])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("size", [1e4, 1e11, 4e30, 1e37])
+def test_attention_scores_of_any_size(size, sign, old, new, n_q, n_kv, d, dtype):
+    """Two scores, the smaller one further below than any probability reaches, and minus infinity: an even share of the values at the larger one's keys."""
+    plan, pages = make_plan(old, new, 16, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(d)
+    v = torch.randn(pages, 16, n_kv, d, generator=g, device="cuda").to(dtype)
+    k = torch.zeros(pages, 16, n_kv, d, device="cuda", dtype=dtype)
+    root = 2.0 ** round(math.log2(size) / 2)
+    near, far = (1.7109375, 2.5) if sign < 0 else (2.5, 1.7109375)          # (in all their digits: products with the scale are rounded)
+    low = torch.rand(pages, 16, n_kv, generator=g, device="cuda") < 0.5
+    for r in range(len(old)):   # every row's first key has the larger score: every token sees one
+        low[int(plan.tables[r, 0]), 0] = False
+    k[..., 3] = sign * root * torch.where(low, far, near)
+    gone = torch.rand(low.shape, generator=g, device="cuda") < 0.1
+    k[..., 3] = torch.where(gone & low, float("-inf"), k[..., 3])
+    q = torch.zeros(sum(new), n_q, d, device="cuda", dtype=dtype)
+    q[..., 3] = 1.6640625 * root
+    ref, mass = attend64(q, k, v, plan, 1.1)
+    out = ops.paged_attention(q, k, v, plan, scale=1.1)
+    assert ref.isfinite().all() and bool(((out.double() - ref).abs() <= _attention_bound(dtype, ref, mass, max(o + n for o, n in zip(old, new)), d)).all())
