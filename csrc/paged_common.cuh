@@ -1,4 +1,4 @@
-// What the tensor-core kernels over paged caches share.
+// What the kernels that serve from paged caches share.
 #pragma once
 #include "common.cuh"
 #include <atomic>

@@ -28,7 +28,7 @@
 // 290, rows of all kinds 145; 64 x 100,003 fp32, all with top-k 34; 4 x 32,000 11.7.  With bounds from counts alone and a second sum for what they leave open the rows
 // of all kinds took 170 us (top-p alone 154 to 365), with two tokens at a time in the passes with exponentials 158; the first form, a bisection with a pass over the
 // row per step, took 8,146, 2,761 and 543 us.
-#include "common.cuh"
+#include "paged_common.cuh"
 
 namespace ats {
 
@@ -44,6 +44,7 @@ constexpr int SR_MAX_K = 1024;
 constexpr int SR_FEW = SR_THREADS / 2;
 constexpr int SR_CHUNK = 256;
 constexpr int SR_MAX_CLUSTER = 8;
+constexpr int SR_CACHED = 131072 + SR_CHUNK * 8;   // bytes of a slice that is kept in shared memory at most
 
 struct SampleRowsArgs {
   const void* logits;   // [B, ld] bf16 or fp32
@@ -799,9 +800,10 @@ static int launch_sample_rows(SampleRowsArgs& p, int B, cudaStream_t s) {
   while (C < SR_MAX_CLUSTER && (long long)p.V * sizeof(T) > C * 65536ll) C *= 2;
   while (C < SR_MAX_CLUSTER && 2 * C * B <= 148 && p.V > C * 2048) C *= 2;
   p.slice = (p.V + 7 + C * SR_CHUNK - 1) / (C * SR_CHUNK) * SR_CHUNK;   // (up to seven places in front of the first token)
-  p.cached = (long long)p.slice * sizeof(T) <= 131072 + SR_CHUNK * 8;
+  p.cached = (long long)p.slice * sizeof(T) <= SR_CACHED;
   const SampleRowsSmem<T> at(p.slice, p.cached);
-  cudaError_t ce = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, at.total);
+  static DeviceOnce once;   // (for the largest slice, whatever this call's: the limit is one for all threads.  A slice that is not kept takes a third of it)
+  cudaError_t ce = once.smem(sample_rows_kernel<T>, SampleRowsSmem<T>(SR_CACHED / sizeof(T), true).total);
   if (ce != cudaSuccess) return int(ce);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, B);

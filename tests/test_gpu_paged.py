@@ -516,3 +516,29 @@ def test_attention_scores_of_any_size(size, sign, old, new, n_q, n_kv, d, dtype)
     ref, mass = attend64(q, k, v, plan, 1.1)
     out = ops.paged_attention(q, k, v, plan, scale=1.1)
     assert ref.isfinite().all() and bool(((out.double() - ref).abs() <= _attention_bound(dtype, ref, mass, max(o + n for o, n in zip(old, new)), d)).all())
+
+
+def test_sample_rows_from_two_threads():
+    """Threads that sample vocabularies of different sizes at the same time do not get in each other's way (the entry point itself, so that they meet in it)."""
+    import threading
+    from adaptivetrainingsystem_b200.ops import paged
+    sizes, wrong = (33, 131072), []
+    x = [torch.randn(2, V, generator=torch.Generator().manual_seed(V)).bfloat16().cuda() for V in sizes]
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    want = [ops.sample_rows(t, u, 1.0, 40) for t in x]
+    out = [torch.zeros_like(t) for t in want]
+    streams = [torch.cuda.Stream() for _ in sizes]
+    torch.cuda.synchronize()
+    entry = paged._fn("ats_sample_rows")
+
+    def work(i):
+        args = (x[i].data_ptr(), 0, sizes[i], 2, sizes[i], u.data_ptr(), 0, 1.0, 0, 40, 0, 1.0, 0, 0.0, 0, 1.0, 0, 0, 0, out[i].data_ptr(), streams[i].cuda_stream)
+        wrong.extend(code for code in (entry(*args) for _ in range(30000)) if code)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, (len(wrong), wrong[0])
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
