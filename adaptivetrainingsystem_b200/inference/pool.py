@@ -149,12 +149,15 @@ class PagedPool:
         del self.lengths[slot], self.reserved[slot]
         self.slots.free(torch.tensor([slot]))
 
-    def _grow(self, more: Dict[int, int]) -> None:
+    def _check_room(self, more: Dict[int, int]) -> None:
         for slot, n in more.items():
             if self.lengths[slot] + n > self.max_len:
                 raise RuntimeError(f"cache overflow: {self.lengths[slot]}+{n} > {self.max_len}")
             if self.cache.pool.pages_for(self.lengths[slot] + n) > self.reserved[slot]:
                 raise RuntimeError(f"row {slot} was opened for {self.reserved[slot]} pages and holds {self.lengths[slot]} tokens: no room for {n} more")
+
+    def _grow(self, more: Dict[int, int]) -> None:
+        """The step has been planned on the device: rows hold these tokens more."""
         for slot, n in more.items():
             self.lengths[slot] += n
 
@@ -165,13 +168,15 @@ class PagedPool:
         ids = {slot: torch.as_tensor(part, dtype=torch.long).flatten() for slot, part in portions}
         if len(ids) != len(portions) or not portions or any(t.numel() == 0 for t in ids.values()):
             raise ValueError("portions of at least one token, of different rows, are needed")
-        self._grow({slot: part.numel() for slot, part in ids.items()})
+        more = {slot: part.numel() for slot, part in ids.items()}
+        self._check_room(more)
         order = sorted(ids)                                # rows lie in the packed batch in their own order
         fresh = torch.zeros(self.rows, dtype=torch.int32)
         fresh[order] = torch.tensor([ids[s].numel() for s in order], dtype=torch.int32)
         ends = fresh[order].cumsum(0) - 1
         packed = torch.cat([ids[s] for s in order]).to(self.device)
-        self.cache.plan(fresh.to(self.device), packed.numel(), max_new=int(fresh.max()), max_len=max(self.lengths[s] for s in order))
+        self.cache.plan(fresh.to(self.device), packed.numel(), max_new=int(fresh.max()), max_len=max(self.lengths[s] + more[s] for s in order))
+        self._grow(more)
         at = dict(zip(order, ends.tolist()))
         return self.model(packed.view(1, -1), cache=self.cache, logits_at=[at[slot] for slot, _ in portions], return_aux_loss=False)[0]
 
@@ -179,8 +184,9 @@ class PagedPool:
         """Runs the next portion of a sequence -> logits [1, V] of its last token."""
         return self.extend_many([(slot, ids)])
 
-    def _decode(self) -> torch.Tensor:
+    def _decode(self, slots: Sequence[int] = ()) -> torch.Tensor:
         plan = self.cache.plan(self.fresh, self.rows, single=True)
+        self._grow({s: 1 for s in slots})
         place = plan.starts[:-1].long()                    # of a row's token in the packed batch
         packed = torch.zeros(self.rows + 1, dtype=torch.long, device=self.device).scatter_(0, torch.where(self.fresh > 0, place, self.rows), self.last)[:-1]
         # (several ranks: their barriers keep launches in order)
@@ -209,7 +215,7 @@ class PagedPool:
         buffer that the next step overwrites)."""
         if len(set(slots)) != len(slots):
             raise ValueError("every row decodes one token of a step")
-        self._grow({s: 1 for s in slots})
+        self._check_room({s: 1 for s in slots})
         if self.use_graph and self._graph is None:
             self._capture()
         if self._live != tuple(slots):
@@ -218,6 +224,7 @@ class PagedPool:
             self.fresh.copy_(live)
             self._live = tuple(slots)
         if not self.use_graph:
-            return self._decode()
+            return self._decode(slots)
         self._graph.replay()
+        self._grow({s: 1 for s in slots})
         return self._logits

@@ -152,12 +152,12 @@ class ContinuousBatcher:
                 self.prefilling.append(r)
             n = min(left, r.prompt.numel() - r.prefilled)
             taken.append((r, r.prompt[r.prefilled:r.prefilled + n]))
-            r.prefilled += n
             left -= n
         if not taken:
             return 0
         logits = self.pool.extend_many([(r.slot, part) for r, part in taken])
-        for i, (r, _) in enumerate(taken):
+        for i, (r, part) in enumerate(taken):
+            r.prefilled += part.numel()
             if r.prefilled == r.prompt.numel():
                 self.prefilling.remove(r)
                 self._first_token(r, logits[i:i + 1])

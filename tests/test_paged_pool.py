@@ -151,3 +151,33 @@ def test_rows_whose_length_is_no_multiple_of_a_page():
     got = model(ids[None], cache=cache, return_aux_loss=False)[0]
     want = model(ids[None], return_aux_loss=False)[0]
     assert torch.allclose(got, want, atol=2e-4)
+
+
+def test_steps_that_do_not_come_to_be_planned_leave_the_rows_as_they_were(monkeypatch):
+    model = _model()
+    pool = PagedPool(model, 2, 300000, pages=5000, page_size=64, use_graph=False)
+    row, other = pool.open(270000), pool.open(100)
+    pool.extend(other, [1, 2, 3])
+    with pytest.raises(ValueError, match="tokens in a step"):
+        pool.extend(row, torch.zeros((1 << 18) + 1, dtype=torch.long))
+    assert pool.lengths == {row: 0, other: 3}
+    plan = type(pool.cache).plan
+
+    def fail(self, *args, **kw):
+        raise RuntimeError("out of memory")
+    monkeypatch.setattr(type(pool.cache), "plan", fail)
+    with pytest.raises(RuntimeError, match="memory"):
+        pool.decode([other])
+    assert pool.lengths == {row: 0, other: 3}
+    # a batcher goes on where it was
+    monkeypatch.setattr(PagedPool, "_capture", lambda self: setattr(self, "use_graph", False))
+    eng = GenerationEngine(model)
+    batcher = ContinuousBatcher(eng, max_batch=2, max_len=40, params=SamplingParams.from_mode("greedy"), page_size=4)
+    rid = batcher.submit([5, 6, 7, 8, 9], 6)
+    with pytest.raises(RuntimeError, match="memory"):
+        batcher.step()
+    monkeypatch.setattr(type(pool.cache), "plan", plan)
+    while batcher.pending:
+        batcher.step()
+    want = eng.generate(torch.tensor([[5, 6, 7, 8, 9]]), SamplingParams.from_mode("greedy", max_new_tokens=6), use_graph=False)["tokens"][0].tolist()
+    assert batcher.finished[rid].tokens == want
