@@ -12,7 +12,8 @@ The rows live in a :class:`SequencePool` (one cache of ``max_batch`` rows and on
 
 With ``page_size`` the rows live in a :class:`PagedPool` instead: a request takes pages for its own prompt and budget rather than a row of
 ``max_len``, and the portions that a step admits run as one packed batch.  A request may bring sampling numbers of its own
-(:meth:`ContinuousBatcher.submit`); then the step's tokens are drawn by ``ops.sample_rows``, still in one launch.
+(:meth:`ContinuousBatcher.submit`); the step's tokens of such requests are drawn by ``ops.sample_rows`` in one launch, those of the others in
+another, from random numbers of their own: what one kind draws does not depend on the other.
 
 The reference's own generator serves one sequence at a time and re-runs the context for every token (``Chat.py:355-465``); its
 vendored serving engine keeps a slot table per batch (``colossalai/inference/kv_cache/kvcache_manager.py:11-106`` allocator,
@@ -68,13 +69,13 @@ class ContinuousBatcher:
         self._stop = set(int(t) for t in (self.params.stop_token_ids or ()))
         self._own = 0                                  # requests under way that bring sampling numbers of their own
         self._numbers: Optional[Dict[str, torch.Tensor]] = None   # per row, once such a request has come
+        self._brings: Optional[torch.Tensor] = None    # rows of such requests
         self.steps = 0
-        self.generator = torch.Generator(device=self.device).manual_seed(self.params.seed) if self.params.seed is not None else None
+        self.generator, self.own_generator = (torch.Generator(device=self.device).manual_seed(self.params.seed) if self.params.seed is not None else None for _ in range(2))
 
     # -- requests --------------------------------------------------------------------------------------------------
     def submit(self, prompt: Sequence[int], max_new_tokens: Optional[int] = None, params: Optional[SamplingParams] = None) -> int:
-        """``params``: sampling numbers, stop tokens and token budget of this request (its ``repetition_window`` is the batcher's, as are the random
-        numbers)."""
+        """``params``: sampling numbers, stop tokens and token budget of this request (its ``repetition_window`` and seed are the batcher's)."""
         ids = torch.as_tensor(prompt, dtype=torch.long).flatten()
         budget = int(max_new_tokens if max_new_tokens is not None else (params or self.params).max_new_tokens)
         if self.paged and self.pool.cache.pool.pages_for(ids.numel() + budget) > self.pool.pages:
@@ -94,20 +95,29 @@ class ContinuousBatcher:
     _FIELDS: Tuple[Tuple[str, torch.dtype], ...] = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32),
                                                     ("repetition_penalty", torch.float32))
 
-    def _set_numbers(self, slot: int, params: SamplingParams) -> None:
-        if self._numbers is None:
-            self._numbers = {n: torch.full((self.max_batch,), getattr(self.params, n), dtype=t, device=self.device) for n, t in self._FIELDS}
-        for n, _ in self._FIELDS:
-            self._numbers[n][slot] = getattr(params, n)
+    _NOT_ASKED = SamplingParams.from_mode("greedy")   # of rows without numbers of their own: the least work
 
-    def _sample(self, logits: torch.Tensor, slot: Optional[int] = None) -> torch.Tensor:
-        """Tokens of all rows, or of row ``slot`` alone."""
-        history = self.history if slot is None else self.history[slot:slot + 1]
-        if not self._own:
-            return sample_next(logits, self.params, history, self.generator)
-        n = {k: v if slot is None else v[slot:slot + 1] for k, v in self._numbers.items()}
-        uniform = torch.rand(logits.shape[0], device=self.device, generator=self.generator)
-        return ops.sample_rows(logits, uniform, n["temperature"], n["top_k"], n["top_p"], n["min_p"], n["repetition_penalty"], history)
+    def _set_numbers(self, slot: int, params: Optional[SamplingParams]) -> None:
+        if self._numbers is None:
+            if params is None:
+                return
+            self._numbers = {n: torch.full((self.max_batch,), getattr(self._NOT_ASKED, n), dtype=t, device=self.device) for n, t in self._FIELDS}
+            self._brings = torch.zeros(self.max_batch, dtype=torch.bool, device=self.device)
+        self._brings[slot] = params is not None
+        for n, _ in self._FIELDS:
+            self._numbers[n][slot] = getattr(params or self._NOT_ASKED, n)
+
+    def _sample(self, logits: torch.Tensor, rows: slice, own: int, others: int) -> torch.Tensor:
+        """Tokens of ``rows``, of which ``own`` bring numbers of their own and ``others`` do not (the rest is not asked).  Either kind is drawn as though the
+        other were not there: with its own sampler, from a generator of its own."""
+        history = self.history[rows]
+        tokens = sample_next(logits, self.params, history, self.generator) if others else None
+        if not own:
+            return tokens
+        n = {k: v[rows] for k, v in self._numbers.items()}
+        uniform = torch.rand(logits.shape[0], device=self.device, generator=self.own_generator)
+        mine = ops.sample_rows(logits, uniform, n["temperature"], n["top_k"], n["top_p"], n["min_p"], n["repetition_penalty"], history)
+        return mine if tokens is None else torch.where(self._brings[rows], mine, tokens)
 
     # -- one scheduling step ---------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -169,9 +179,8 @@ class ContinuousBatcher:
         self.history[slot].fill_(int(r.prompt[0]))     # left padding of a short prompt repeats its first token
         self.history[slot, -min(n, w):] = ids[-min(n, w):]
         self._own += r.params is not None
-        if r.params is not None or self._numbers is not None:
-            self._set_numbers(slot, r.params or self.params)
-        first = self._sample(logits, slot)
+        self._set_numbers(slot, r.params)
+        first = self._sample(logits, slice(slot, slot + 1), r.params is not None, r.params is None)
         self.pool.last[slot:slot + 1] = first
         self.history[slot] = torch.roll(self.history[slot], -1)
         self.history[slot, -1:] = first
@@ -201,7 +210,7 @@ class ContinuousBatcher:
         if not live:
             return 0
         logits = self.pool.decode(live)
-        nxt_dev = self._sample(logits)
+        nxt_dev = self._sample(logits, slice(None), self._own, len(live) - self._own)
         self.pool.last.copy_(nxt_dev)
         self.history = torch.roll(self.history, -1, dims=1)
         self.history[:, -1] = nxt_dev

@@ -109,3 +109,23 @@ def test_requests_with_numbers_of_their_own():
     want = eng.generate(torch.tensor([ids], device="cuda"), SamplingParams.from_mode("greedy", max_new_tokens=10))["tokens"][0].tolist()
     assert batcher.finished[greedy].tokens == batcher.finished[sure].tokens == batcher.finished[tiny].tokens == want
     assert batcher.finished[wild].tokens != want
+
+
+@torch.no_grad()
+def test_rows_of_either_kind_are_drawn_by_their_own_sampler():
+    """Rows without numbers of their own draw what they draw alone, beside rows with numbers, which draw what ``ops.sample_rows`` draws for all of them."""
+    params = SamplingParams(temperature=1.0, top_k=20, top_p=0.9, repetition_penalty=1.1, seed=2)
+    batcher = ContinuousBatcher(GenerationEngine(_model()), max_batch=8, max_len=64, params=params, page_size=16)
+    logits = (2 * torch.randn(8, 512, device="cuda")).round().bfloat16()     # ties, for which the samplers have different rules
+    for slot in (0, 3, 4):
+        batcher._set_numbers(slot, SamplingParams(temperature=2.0, top_k=100, top_p=1.0, min_p=0.01, repetition_penalty=1.0))
+    states = [g.get_state() for g in (batcher.generator, batcher.own_generator)]
+
+    def draw(*counts):
+        for g, s in zip((batcher.generator, batcher.own_generator), states):
+            g.set_state(s)
+        return batcher._sample(logits, slice(None), *counts)
+    plain, own, mixed = draw(0, 8), draw(3, 0), draw(3, 5)
+    rows = torch.tensor([True, False, False, True, True, False, False, False], device="cuda")
+    assert torch.equal(mixed, torch.where(rows, own, plain)) and not torch.equal(own, plain)
+    assert batcher.own_generator.get_state().equal(states[1]) is False

@@ -181,3 +181,40 @@ def test_steps_that_do_not_come_to_be_planned_leave_the_rows_as_they_were(monkey
         batcher.step()
     want = eng.generate(torch.tensor([[5, 6, 7, 8, 9]]), SamplingParams.from_mode("greedy", max_new_tokens=6), use_graph=False)["tokens"][0].tolist()
     assert batcher.finished[rid].tokens == want
+
+
+def test_neighbours_do_not_choose_how_a_request_is_drawn():
+    """Requests without sampling numbers of their own draw the same tokens whether or not ones with numbers are served beside them, and the other way round."""
+    eng = GenerationEngine(_model())
+    loud = SamplingParams(temperature=6.0, top_k=0, top_p=1.0, repetition_penalty=1.0, max_new_tokens=12, seed=5)
+    own = SamplingParams(temperature=4.0, top_k=60, top_p=0.95, repetition_penalty=1.0, max_new_tokens=12)
+
+    def serve(kinds):
+        batcher = ContinuousBatcher(eng, max_batch=3, max_len=40, params=loud, page_size=8)
+        batcher.pool.use_graph = False
+        rids = [batcher.submit([3, 1, 4, 1, 5], 12 if kind else 1, params=own if kind == "own" else None) for kind in kinds]   # (None: gone after its first token)
+        while batcher.pending:
+            batcher.step()
+        return [batcher.finished[r].tokens for r in rids]
+    both = serve(["plain", "own"])
+    assert both[0] == serve(["plain"])[0] and len(set(both[0])) > 3
+    assert both[1] == serve([None, "own"])[1] and len(set(both[1])) > 3
+
+
+@torch.no_grad()
+def test_rows_of_either_kind_are_drawn_by_their_own_sampler():
+    eng = GenerationEngine(_model())
+    params = SamplingParams(temperature=1.0, top_k=5, top_p=1.0, repetition_penalty=1.0, seed=2)
+    batcher = ContinuousBatcher(eng, max_batch=6, max_len=16, params=params, page_size=8)
+    logits = torch.zeros(6, 97)     # nothing but ties: the samplers' rules for them differ
+    for slot in (1, 4):
+        batcher._set_numbers(slot, SamplingParams(temperature=1.0, top_k=5, top_p=1.0, repetition_penalty=1.0))
+    assert batcher._brings.tolist() == [False, True, False, False, True, False]
+    state = batcher.generator.get_state()
+    alone = batcher._sample(logits, slice(None), 0, 6)
+    batcher.generator.set_state(state)
+    mixed = batcher._sample(logits, slice(None), 2, 4)
+    others = [0, 2, 3, 5]
+    assert torch.equal(mixed[others], alone[others]) and (mixed[[1, 4]] < 5).all()
+    batcher._set_numbers(4, None)
+    assert batcher._brings.tolist() == [False, True, False, False, False, False]
