@@ -191,7 +191,8 @@ class ContinuousBatcher:
         """Host-side bookkeeping of one generated token (the device-side state was updated for all rows at once)."""
         r = self.by_slot[slot]
         r.tokens.append(token)
-        stop = self._stop if r.params is None else r.params.stop_token_ids
+        own = r.params and r.params.stop_token_ids
+        stop = self._stop if r.params is None else () if own is None else own
         if token in stop or len(r.tokens) >= r.max_new_tokens:
             self._retire(slot)
 

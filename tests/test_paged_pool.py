@@ -218,3 +218,14 @@ def test_rows_of_either_kind_are_drawn_by_their_own_sampler():
     assert torch.equal(mixed[others], alone[others]) and (mixed[[1, 4]] < 5).all()
     batcher._set_numbers(4, None)
     assert batcher._brings.tolist() == [False, True, False, False, False, False]
+
+
+def test_a_request_may_say_that_it_has_no_stop_tokens():
+    eng = GenerationEngine(_model())
+    batcher = ContinuousBatcher(eng, max_batch=2, max_len=40, params=SamplingParams.from_mode("greedy", stop_token_ids=None), page_size=8)
+    batcher.pool.use_graph = False
+    rids = [batcher.submit([1, 2, 3], 5), batcher.submit([1, 2, 3], params=SamplingParams.from_mode("greedy", stop_token_ids=None, max_new_tokens=5))]
+    while batcher.pending:
+        batcher.step()
+    first, second = (batcher.finished[r].tokens for r in rids)
+    assert first == second and len(first) == 5
