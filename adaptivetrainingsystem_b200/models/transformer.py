@@ -266,8 +266,8 @@ class MoEFFNLayer(nn.Module):
         self.register_buffer("dropped_slots", torch.zeros((), dtype=torch.float64), persistent=False)
         self.ep = None  # set by parallel.expert_parallel.attach when world size > 1
 
-    def forward(self, h: torch.Tensor, residual: Optional[torch.Tensor] = None, next_norm=None):
-        """-> (output, auxiliary loss); with ``next_norm`` = (weight, eps) on a decode-sized step whose combine launch also
+    def forward(self, h: torch.Tensor, residual: Optional[torch.Tensor] = None, next_norm=None, drop_tokens: Optional[bool] = None):
+        """-> (output, auxiliary loss); ``drop_tokens``: instead of the configuration's.  With ``next_norm`` = (weight, eps) on a decode-sized step whose combine launch also
         normalised its result for the next block -> (output, None, normalised output)."""
         shape = h.shape
         x = h.reshape(-1, shape[-1])
@@ -305,7 +305,7 @@ class MoEFFNLayer(nn.Module):
             # router z-loss: mean squared log-partition of the (un-noised) gate logits; it keeps the logits from drifting to magnitudes
             # where the soft-max saturates (reference: colossalai/moe/routers.py:94-110)
             aux = aux + self.router_z_loss_weight * torch.logsumexp(logits.float(), dim=-1).pow(2).mean()
-        cap = moe_ops.expert_capacity(T, E, k, self.capacity_factor, self.cfg.drop_tokens)
+        cap = moe_ops.expert_capacity(T, E, k, self.capacity_factor, self.cfg.drop_tokens if drop_tokens is None else drop_tokens)
         res2 = residual.reshape(-1, shape[-1]) if residual is not None else None
         if self.ep is not None:
             out, totals = self.ep.moe_ffn(x, idx, w.to(torch.float32), self.experts_w1, self.experts_w2, cap, res2)
@@ -470,10 +470,15 @@ class TransformerBlock(nn.Module):
         if self.ffn_kind == "mod":
             x, aux = self.ffn(h, x, decode=decode)
         else:
-            x, aux = self.ffn(h, x)
+            x, aux = self.ffn(h, x, **self._ffn_options(cache))
         if aux is None:
             aux = x.new_zeros((), dtype=torch.float32)
         return x, aux
+
+    def _ffn_options(self, cache) -> Dict[str, Any]:
+        """A step over a paged cache packs tokens of many sequences, and rows of none: what an expert has no room for would depend on a sequence's
+        neighbours, so every token keeps its experts (as in decode-sized steps over any cache)."""
+        return {"drop_tokens": False} if self.ffn_kind == "moe" and isinstance(cache, PagedKVCache) else {}
 
     def takes_scaled_rows(self, rope, cache) -> bool:
         """Whether this block's projection divides by the norm of its input itself (``ops.serving.ScaledRows``)."""
@@ -498,7 +503,7 @@ class TransformerBlock(nn.Module):
             h, x = self.post_attn_norm.with_skip(x)
         h_next = None
         if self.ffn_kind == "moe":
-            res = self.ffn(h, x, next_norm=next_norm)
+            res = self.ffn(h, x, next_norm=next_norm, **self._ffn_options(cache))
             x = res[0]
             h_next = res[2] if len(res) > 2 else None
         elif self.ffn_kind == "mod":
@@ -667,7 +672,8 @@ class DeepSeekTransformer(nn.Module):
         return KVCache(self.config.num_layers, batch, max_len, n_kv, self.config.head_dim, dtype or p.dtype, device or p.device)
 
     def make_paged_cache(self, rows: int, max_len: int, pages: int, page_size: int = 64) -> PagedKVCache:
-        """A cache of ``rows`` rows of up to ``max_len`` tokens that share ``pages`` pages."""
+        """A cache of ``rows`` rows of up to ``max_len`` tokens that share ``pages`` pages.  Steps over it drop no token of a mixture of experts, whatever
+        ``drop_tokens`` says, so that a sequence's logits do not depend on its neighbours."""
         if self.get_mod_layers():
             raise ValueError("a step over a paged cache packs tokens of many sequences; Mixture-of-Depths layers choose tokens per sequence")
         p = self.embed_tokens.weight

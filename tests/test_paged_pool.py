@@ -229,3 +229,23 @@ def test_a_request_may_say_that_it_has_no_stop_tokens():
         batcher.step()
     first, second = (batcher.finished[r].tokens for r in rids)
     assert first == second and len(first) == 5
+
+
+@torch.no_grad()
+def test_experts_drop_no_token_of_a_packed_batch():
+    """An expert's room is counted per batch: prompts that fit it one by one would not together, and a request's logits would depend on its neighbours."""
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=97, hidden_size=32, num_layers=2, num_heads=4, num_kv_heads=2, intermediate_size=64, seq_length=128, use_moe=True, num_experts=4,
+                      moe_top_k=2, capacity_factor=0.25, routing_noise_std=0.0)
+    model = DeepSeekTransformer(cfg).eval()
+    g = torch.Generator().manual_seed(1)
+    seqs = [torch.randint(0, 97, (100,), generator=g) for _ in range(6)]
+    pool = PagedPool(model, 200, 128, pages=250, page_size=16, use_graph=False)
+    rows = [pool.open(102) for _ in seqs]
+    packed = pool.extend_many(list(zip(rows, seqs)))
+    for s, got in zip(seqs, packed):
+        assert torch.allclose(got, model(s[None], return_aux_loss=False)[0, -1], atol=2e-4)
+    pool.last[rows] = torch.tensor([5] * 6)
+    out = pool.decode(rows)          # 200 rows, 194 of them empty
+    for r, s in zip(rows, seqs):
+        assert torch.allclose(out[r], model(torch.cat([s, torch.tensor([5])])[None], return_aux_loss=False)[0, -1], atol=2e-4)
