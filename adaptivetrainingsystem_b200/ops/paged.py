@@ -238,6 +238,8 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, l
     pages, ps, n_kv, d = k_pages.shape
     if not (pages and n_kv and d):
         raise ValueError("pages without tokens, heads or columns")
+    if torch.is_grad_enabled() and (like.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise RuntimeError("the paged operators have no backward pass: call them under torch.no_grad(), or with tensors that ask for no gradient")
     if (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
         raise ValueError("k_pages, v_pages: they have to begin at a multiple of 16 bytes")
     if pages * ps > MAX_SLOTS:
@@ -284,7 +286,8 @@ def paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[t
     of ``k_pages`` / ``v_pages`` [pages, page_size, n_kv, d] (slot -1: nowhere).  Queries and keys are rotated at ``plan.positions`` with the
     tables ``cos`` / ``sin`` [max position, d / 2] fp32 (halves of a head, d a multiple of 16); with ``cos`` = ``None`` they are rotated already and the
     queries are a view of ``qkv``.  No two tokens of a step have the same slot (a plan's never have).  A slot outside the pages or a position behind the
-    tables is reported by ``ops.check_status``, and nothing of that token is written.  For serving: no gradients."""
+    tables is reported by ``ops.check_status``, and nothing of that token is written.  For serving: tensors that
+    ask for a gradient are refused."""
     T = qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] != (n_q + 2 * n_kv) * d:
         raise ValueError(f"qkv: [tokens, {(n_q + 2 * n_kv) * d}] is needed")
@@ -338,7 +341,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     row's tokens up to itself, in the pages of ``plan.tables``; its keys and values are there already.  ``scale`` (default 1 / sqrt(d)) times the scores.
     Tokens behind the last row come out as zeros, or keep what ``out`` holds where it is given (``q`` itself may be: answers replace their queries).  Heads of up to 256 dimensions (multiples of 8).
     A table entry outside the pool is reported by ``ops.check_status`` and nothing is read there (what its row gets has no meaning).  bf16: scores, statistics and sums in fp32, probabilities rounded to
-    bf16 for their product with the values; fp32 in true 32-bit.  For serving: no gradients."""
+    bf16 for their product with the values; fp32 in true 32-bit.  For serving: tensors that ask for a gradient are refused."""
     if q.dim() != 3:
         raise ValueError("q: [tokens, heads, d] is needed")
     pages, ps, n_kv, d = _check_pages(k_pages, v_pages, plan, q)

@@ -251,3 +251,23 @@ def test_warps_of_the_portion_kernel_give_up_a_wait_together():
         assert ("mbar_wait_bounded" in role) == role.lstrip("- ").startswith("MMA issuer"), role[:80]
     for told in kernel.split("next_piece(n_pieces);")[2:]:
         assert told.lstrip().startswith("if (!__all_sync(0xffffffffu, told != nullptr)) break;")
+
+
+def test_operators_refuse_tensors_that_ask_for_gradients():
+    plan, pages = make_plan([3], [2], 4, "cpu")
+    k, v = torch.zeros(pages, 4, 2, 16), torch.zeros(pages, 4, 2, 16)
+    q, qkv = torch.zeros(2, 4, 16), torch.zeros(2, 128)
+    for bad in (q, k, v):
+        bad.requires_grad_(True)
+        with pytest.raises(RuntimeError, match="backward"):
+            ops.paged_attention(q, k, v, plan)
+        if bad is not q:
+            with pytest.raises(RuntimeError, match="backward"):
+                ops.paged_append(qkv, None, None, plan, k, v, 4, 2, 16)
+        with torch.no_grad():
+            assert not ops.paged_attention(q, k, v, plan).requires_grad
+        bad.requires_grad_(False)
+    qkv.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="backward"):
+        ops.paged_append(qkv, None, None, plan, k, v, 4, 2, 16)
+    assert not k.requires_grad
