@@ -705,11 +705,7 @@ ATS_API int ats_paged_portion(const void* q, long long ldq, const void* k_pages,
   if ((D != 64 && D != 128) || tokens < 1 || R < 1 || n_kv < 1 || n_q % n_kv || n_q / n_kv > 128 || (ldq & 7) || (ldo & 7) || off_16(q, k_pages, v_pages, out) || (reinterpret_cast<uintptr_t>(scratch) & 31) ||
       page < 8 || (page & (page - 1)) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256 || tokens > (1 << 30))
     return 1003;
-  static thread_local bool ctx_bound = false;
-  if (!ctx_bound) {
-    cudaFree(0);
-    ctx_bound = true;
-  }
+  bind_context();
   PagedPortionArgs p;
   p.rows = {starts, lengths, tables, R, width, pages, __builtin_ctz(page), tokens};
   p.v_pages = static_cast<const __nv_bfloat16*>(v_pages); p.out = static_cast<__nv_bfloat16*>(out); p.ldo = ldo;

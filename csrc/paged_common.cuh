@@ -48,6 +48,18 @@ inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Makes the device's context the calling thread's (tensor maps are encoded by the driver).  In the mode in which it may be asked for during a capture, this thread's
+// or another's: the first call of a thread may be a captured one.
+inline void bind_context() {
+  static thread_local bool bound = false;
+  if (bound) return;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaFree(0);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  bound = true;
+}
+
 // A kernel's shared-memory limit, raised once per device.
 struct DeviceOnce {
   std::atomic<unsigned long long> done{0};

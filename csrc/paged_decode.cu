@@ -564,11 +564,7 @@ ATS_API int ats_paged_decode(const void* q, long long ldq, const void* k_pages, 
   if ((D != 64 && D != 128) || tokens < 1 || R < 1 || R > 65535 || n_kv < 1 || n_kv > 65535 || n_q % n_kv || (ldq & 7) || (ldo & 7) || page < 8 || (page & (page - 1)) ||
       (limit != 8 && limit != 16) || off_16(q, k_pages, v_pages, out, scratch) || max_new < 1 || max_keys < 1 || ((long long)width * page / 16 + 1) * R * n_kv >= (1ll << 32) || (long long)pages * page >= (1ll << 31) - 256 || (long long)width * page >= (1ll << 31) - 256)
     return 1003;
-  static thread_local bool ctx_bound = false;
-  if (!ctx_bound) {
-    cudaFree(0);
-    ctx_bound = true;
-  }
+  bind_context();
   const int unit = 2048 / D;
   CUtensorMap mk, mv;
   int e;

@@ -542,3 +542,31 @@ def test_sample_rows_from_two_threads():
     torch.cuda.synchronize()
     assert not wrong, (len(wrong), wrong[0])
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("old,new", [([100, 50], [1, 1]), ([0, 40], [200, 60])])
+def test_first_call_of_a_thread_may_be_a_captured_one(old, new):
+    import threading
+    plan, pages = make_plan(old, new, 16, "cuda")
+    plan.max_new = max(new)
+    k, v = (torch.randn(pages, 16, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(sum(new), 8, 64, device="cuda").bfloat16()
+    want, got = ops.paged_attention(q, k, v, plan), []
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            with torch.cuda.stream(stream):
+                with torch.cuda.graph(graph, stream=stream):
+                    out = ops.paged_attention(q, k, v, plan)
+                graph.replay()
+            torch.cuda.synchronize()
+            got.append(out)
+        except Exception as e:
+            got.append(e)
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    assert torch.equal(got[0], want)
