@@ -104,8 +104,9 @@ class ContinuousBatcher:
             self._numbers = {n: torch.full((self.max_batch,), getattr(self._NOT_ASKED, n), dtype=t, device=self.device) for n, t in self._FIELDS}
             self._brings = torch.zeros(self.max_batch, dtype=torch.bool, device=self.device)
         self._brings[slot] = params is not None
-        for n, _ in self._FIELDS:
-            self._numbers[n][slot] = getattr(params or self._NOT_ASKED, n)
+        for n, t in self._FIELDS:
+            v = getattr(params or self._NOT_ASKED, n)
+            self._numbers[n][slot] = v if t.is_floating_point else min(max(v, 0), torch.iinfo(t).max)   # (0, and more than there are: all tokens)
 
     def _sample(self, logits: torch.Tensor, rows: slice, own: int, others: int) -> torch.Tensor:
         """Tokens of ``rows``, of which ``own`` bring numbers of their own and ``others`` do not (the rest is not asked).  Either kind is drawn as though the

@@ -249,3 +249,13 @@ def test_experts_drop_no_token_of_a_packed_batch():
     out = pool.decode(rows)          # 200 rows, 194 of them empty
     for r, s in zip(rows, seqs):
         assert torch.allclose(out[r], model(torch.cat([s, torch.tensor([5])])[None], return_aux_loss=False)[0, -1], atol=2e-4)
+
+
+def test_a_request_may_ask_for_any_top_k():
+    eng = GenerationEngine(_model())
+    batcher = ContinuousBatcher(eng, max_batch=2, max_len=40, params=SamplingParams.from_mode("greedy", seed=1), page_size=8)
+    batcher.pool.use_graph = False
+    rids = [batcher.submit([1, 2, 3], params=SamplingParams(temperature=2.0, top_k=k, max_new_tokens=4)) for k in (1 << 40, -(1 << 40))]
+    while batcher.pending:
+        batcher.step()
+    assert all(len(batcher.finished[r].tokens) == 4 for r in rids)
