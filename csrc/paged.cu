@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(APP_MAX_THREADS) paged_append_kernel(const App
 // and the latency of its loads.  Few tokens: a row's blocks of 128 keys are shared out over `splits` CTAs, as many as make eight
 // an SM but no more than the longest row has blocks; their sums are joined in order by a second launch.  One row of 32,000 keys x 8 heads of 96 in bf16 111 us (one
 // CTA a token and group 4,800), 64 rows of 200 to 2,000 keys x 8 of 96 251 (373), x 4 of 64 in fp32 186 (282); with four an SM 112, 372, 283 and 8 rows of 4,000 x 8 of
-// 128 in fp32 164 instead of 179; with twelve 113, 244, 180 and 188.
+// 128 in fp32 164 instead of 179; with twelve 113, 244, 180 and 188.  Portions: a CTA a token, each of which reads its keys again (from L2): 500 tokens x 8 heads of 96 245 us, 2,000 3,026.
 // Tokens behind the last row get zeros (or stay, `keep_tail`), as does a token that sees no key.
 // ------------------------------------------------------------------------------------------------
 constexpr int ANY_WARPS = 4, ANY_HEADS = 4, ANY_BLOCK = 32 * ANY_WARPS, ANY_MAX_SPLITS = 64;

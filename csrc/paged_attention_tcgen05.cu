@@ -5,11 +5,11 @@
 // A tile of 128 query rows holds consecutive new tokens of one row with all query heads of a group (token, head), so that a key head's
 // pages are read once for the whole group and short portions fill tiles too.  A CTA works on two tiles that share the K / V stream and
 // ping-pong on the tensor cores, as in gqa_attention_tcgen05.cu: one query row per soft-max thread, P overwrites S in tensor memory and is
-// the A operand of P V, O stays in tensor memory and is rescaled only when the running maximum grows by more than 2^8.
+// the A operand of P V (rounded to bf16, the type of the other operand; outputs are 0.0020 to 0.0022 off 64 bits, relative, where their own rounding makes 0.0016), O stays in tensor memory and is rescaled only when the running maximum grows by more than 2^8.
 // Bound by the chain of a tile's block, scores -> soft-max -> P V, of which two overlap (2.4 us a pair of blocks of 128 keys and 128 dimensions, 1.1 of them
 // products), and in it by the soft-max warps' instructions: an eighth of the exponentials as polynomials on the FMA lanes takes 3 % longer, half of them 19 %,
-// and a P V that begins under the last exponentials gains nothing.  32 / 8 heads of 128: 1,000 tokens behind 15,000 (255 GFLOP) 251 us = 1,000 TFLOP/s, 0.6 of the library
-// product's rate; six prompts of 300 to 2,500 tokens (96 GFLOP) 158 us = 610, which counts no product of a block that the diagonal halves and all beginnings and
+// and a P V that begins under the last exponentials gains nothing.  32 / 8 heads of 128, whole calls: 1,000 tokens behind 15,000 (255 GFLOP) 247 us = 1,030 TFLOP/s, 0.6
+// of the library product's rate; six prompts of 300 to 2,500 tokens (96 GFLOP) 167 us = 575 (162 before scores of any size were told apart), which counts no product of a block that the diagonal halves and all beginnings and
 // ends of pieces.  Two soft-max threads a row took 180 us for the latter (from 153), products cut to the diagonal's columns 176 (from 164).
 //
 // Rows, portions and caches are of any length, so work is dealt out in key blocks: all (row, key head, pair of tiles), each as long as the keys
@@ -20,7 +20,9 @@
 // A block on the diagonal, or with the row's last key, holds values that some or all rows of the tiles must not see: a probability of zero does not
 // keep a NaN or an infinity out of a product.  Two warps of their own clear such values in shared memory before the product (those that no row
 // sees altogether), and a query that does see them adds them to its output at the end; 5 us of the six prompts'.
-// Every wait is bounded (status word + clean unwind); no load uses cluster multicast.
+// Pairs whose second tile is empty (few tokens of a wide group) have one chain under way: 8 rows of 5,000 keys, two tokens each on 52 / 4 heads of 128 39 us = 2.1 TB/s,
+// four on 32 / 4 of 64 33 us = 1.2 TB/s.
+// Every wait is bounded, whole warps give one up together, and the CTA then unwinds with the status word set; no load uses cluster multicast.
 #include "paged_common.cuh"
 
 namespace ats {

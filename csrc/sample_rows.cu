@@ -23,9 +23,10 @@
 // Up to 256 collected tokens are compared with one another, up to 2,048 are cut by weights counted over 512 places of the keys' range, then over the place that holds
 // the cut (sorting them took 30 us instead of 5).  Cuts whose brackets hold more (thousands of equal scores, k above 1,024) are found by bisection over the 64-bit order.
 // The draw works on sums per 256 consecutive tokens and looks into one of them.
-// Bound by the exponentials of rows without top-k (13 FP64 operations and 45 others a token), their shared-memory counts (rows of equal scores meet in a bin), else
-// by latency: three to five cluster barriers.  256 x 131,072 bf16 (67 MB, 10 us at a copy's rate): greedy 30 us, top-k 50 66, no cut 88, k = 1,000 119, top-p alone 160 to
-// 290, rows of all kinds 145; 64 x 100,003 fp32, all with top-k 34; 4 x 32,000 11.7.  With bounds from counts alone and a second sum for what they leave open the rows
+// Bound by latency rather than by a unit: over rows of all kinds memory is busy to 6 %, the FP64 pipe to 9, the SMs' issue to 32; warps wait at barriers first (three to
+// five of the cluster; while one CTA cuts the list the others have nothing to do), and 256 rows are 3.5 waves of clusters.  Rows without top-k add 13 FP64 operations and
+// 45 others a token and counts in shared memory (rows of equal scores meet in a bin).  64 registers a thread, for two CTAs an SM, leave 30 words of it in local memory.  256 x 131,072 bf16 (67 MB, 10 us at a copy's rate): greedy 30 us, top-k 50 66, no cut 88, k = 1,000 119, top-p alone 160 to
+// 290, rows of all kinds 145 to 149; 64 x 100,003 fp32, all with top-k 34 to 36; 4 x 32,000 12.  With bounds from counts alone and a second sum for what they leave open the rows
 // of all kinds took 170 us (top-p alone 154 to 365), with two tokens at a time in the passes with exponentials 158; the first form, a bisection with a pass over the
 // row per step, took 8,146, 2,761 and 543 us.
 #include "paged_common.cuh"
