@@ -204,10 +204,11 @@ class PagedPool:
             for _ in range(2):
                 self._decode()
         torch.cuda.current_stream(self.device).wait_stream(side)
-        self._graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self._graph), torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():
             self._logits = self._decode()
             self._plan = self.cache.step                   # (the graph writes it again whenever it is replayed)
+        self._graph = graph                                # (only a whole one)
 
     @torch.no_grad()
     def decode(self, slots: Sequence[int]) -> torch.Tensor:

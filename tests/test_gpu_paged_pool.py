@@ -129,3 +129,25 @@ def test_rows_of_either_kind_are_drawn_by_their_own_sampler():
     rows = torch.tensor([True, False, False, True, True, False, False, False], device="cuda")
     assert torch.equal(mixed, torch.where(rows, own, plain)) and not torch.equal(own, plain)
     assert batcher.own_generator.get_state().equal(states[1]) is False
+
+
+@torch.no_grad()
+def test_a_capture_that_fails_is_made_again(monkeypatch):
+    model = _model()
+    pool, plain = PagedPool(model, 2, 64, page_size=16), PagedPool(model, 2, 64, page_size=16, use_graph=False)
+    for p in (pool, plain):
+        p.extend(p.open(40), [5, 6, 7])
+        p.last[0] = 9
+    decode, calls = PagedPool._decode, []
+
+    def fail(self, *args):
+        calls.append(1)
+        if len(calls) == 3:
+            raise RuntimeError("out of memory")
+        return decode(self, *args)
+    monkeypatch.setattr(PagedPool, "_decode", fail)
+    with pytest.raises(RuntimeError, match="memory"):
+        pool.decode([0])
+    assert pool.lengths == {0: 3} and pool.cache.pool.lengths.tolist() == [3, 0]
+    monkeypatch.undo()
+    assert torch.equal(pool.decode([0])[0], plain.decode([0])[0]) and pool.lengths == {0: 4}
